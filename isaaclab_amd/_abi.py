@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import threading
 
 import torch
 
@@ -71,6 +72,22 @@ def stream() -> int:
     if _raw_stream is not None:   # the same handle without building a torch.cuda.Stream object per launch (~3 us each)
         return _raw_stream(-1)
     return torch.cuda.current_stream().cuda_stream
+
+
+_recording = threading.local()   # .kept: the tensors that the command list being recorded on this thread holds on to
+
+
+def recording() -> bool:
+    """Whether this thread is inside ``CommandList.record``."""
+    return getattr(_recording, "kept", None) is not None
+
+
+def keep(t):
+    """``t``; while a command list is recorded the list holds it, so that its memory is still this tensor's at a replay."""
+    kept = getattr(_recording, "kept", None)
+    if kept is not None and t is not None:
+        kept.append(t)
+    return t
 
 
 def f32c(t: torch.Tensor) -> torch.Tensor:

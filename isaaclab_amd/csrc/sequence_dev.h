@@ -1,0 +1,65 @@
+// What the sequence kernels share: element types, their conversions, and the scalar functions of a gate and a step size.
+#pragma once
+
+#include "common.h"
+
+#include "../../include/isaaclab_amd_sequence.h"
+
+namespace ilx {
+
+typedef __bf16 bf16_t;
+typedef _Float16 f16_t;
+
+template <typename T> __device__ __forceinline__ float to_f32(T v) { return static_cast<float>(v); }
+template <typename T> __device__ __forceinline__ T from_f32(float v) { return static_cast<T>(v); }   // to nearest, ties to even
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// e^x and 1/x on the hardware's exponential and reciprocal (1 ulp each; the product with log2 e adds |x| 2^-24 relative).
+__device__ __forceinline__ float exp_fast(float x) { return __builtin_amdgcn_exp2f(x * kLog2e); }
+__device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcpf(x); }
+
+__device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.0f + exp_fast(-x)); }
+
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|), the second term as 2 artanh(e / (2 + e)) with e in (0, 1]: its argument is at
+// most 1/3, so the series in odd powers up to the 15th is short by less than 2^-26 of the value at every x (a logarithm of
+// 1 + e would lose e's last bits, which for a step size of 1e-4 are all it has).
+__device__ __forceinline__ float softplus_f(float x) {
+    const float e = exp_fast(-__builtin_fabsf(x));
+    const float s = e * rcp_fast(2.0f + e), q = s * s;
+    float p = 1.0f / 15;
+    p = __builtin_fmaf(p, q, 1.0f / 13);
+    p = __builtin_fmaf(p, q, 1.0f / 11);
+    p = __builtin_fmaf(p, q, 1.0f / 9);
+    p = __builtin_fmaf(p, q, 1.0f / 7);
+    p = __builtin_fmaf(p, q, 1.0f / 5);
+    p = __builtin_fmaf(p, q, 1.0f / 3);
+    p = p * q;
+    const float l = 2.0f * __builtin_fmaf(p, s, s);
+    return x != x ? x : __builtin_fmaxf(x, 0.0f) + l;
+}
+
+// V neighbouring channels of one row, as one load or store.
+template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+
+template <int V, typename T> __device__ __forceinline__ void load_channels(const T* p, float (&v)[V]) {
+    const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(p);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(w.v[k]);
+}
+template <int V, typename T> __device__ __forceinline__ void store_channels(T* p, const float (&v)[V]) {
+    Pack<T, V> w;
+#pragma unroll
+    for (int k = 0; k < V; ++k) w.v[k] = from_f32<T>(v[k]);
+    *reinterpret_cast<Pack<T, V>*>(p) = w;
+}
+
+inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
+
+// The end of a parameter's gradient: `count` rows of (n0 + 1 + 1) x channels partial sums, one row per workgroup that kept
+// some, are added in a fixed order, in 64 bits.  Value k of channel d goes to out0[d, k] for k < n0, then out1[d], out2[d];
+// outputs that are NULL are left out.
+void launch_parameter_sums(const float* partial, int64_t count, int32_t channels, int32_t n0, float* out0, float* out1, float* out2,
+                           hipStream_t stream);
+
+}  // namespace ilx

@@ -1,0 +1,470 @@
+// Short causal convolution over time, depthwise (one filter per channel), with a carried state and episode starts:
+//   p_t = bias + sum_j w[W-1-j] x_{t-j},  out = p or p sigmoid(p);   rows t < 0 are the carried state.
+// All three kernels move each input once and have 2 W + 6 flops per element, so they are bound by memory.  A thread owns V
+// neighbouring channels (one 8- or 16-byte access per row) of a segment of rows and keeps the last W - 1 rows in
+// registers; a segment re-reads the W - 1 rows ahead of it, which the thread beside it has just brought into the cache.  An
+// episode start clears the registers, so no row looks past it.
+#include "sequence_dev.h"
+
+namespace ilx {
+
+constexpr int kConvThreads = 256;
+
+struct ConvArgs {
+    ilx_short_conv c;
+    int groups;        // of V channels
+    int cx_log2;       // lanes side by side over channel groups; 256 >> cx_log2 rows of threads over segments
+    int channel_blocks;
+    int segment;       // rows per segment
+    int64_t segments;  // per sequence
+    int64_t items;     // batch * segments
+    int64_t slots;     // rows of threads in the grid / rows per block (backward: partial sums)
+};
+
+struct ConvThread {
+    int d0;
+    int64_t item, b, t0, t1, len;
+};
+
+__device__ __forceinline__ int64_t sequence_length(const int32_t* lengths, int64_t b, int64_t length) {
+    if (!lengths) return length;
+    const int64_t n = lengths[b];
+    return n < 0 ? 0 : (n > length ? length : n);
+}
+
+template <int W, int V>
+__device__ __forceinline__ void load_weights(const ConvArgs& a, int d0, float (&w)[W][V], float (&bias)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        bias[v] = a.c.bias ? a.c.bias[d0 + v] : 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) w[k][v] = a.c.weight[static_cast<int64_t>(d0 + v) * W + k];
+    }
+}
+
+// The W - 1 rows ahead of row t0, oldest first, those from before an episode start as zeros.
+template <typename T, int W, int V>
+__device__ __forceinline__ void load_window(const ConvArgs& a, int d0, int64_t b, int64_t t0, float (&win)[W][V]) {
+    const T* x = static_cast<const T*>(a.c.x) + b * a.c.x_batch;
+#pragma unroll
+    for (int i = 0; i < W - 1; ++i) {
+        const int64_t t = t0 - (W - 1) + i;
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[i][v] = 0.0f;
+        if (t >= 0) {
+            if (a.c.starts && a.c.starts[b * a.c.starts_batch + t * a.c.starts_time]) {
+#pragma unroll
+                for (int k = 0; k < i; ++k)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) win[k][v] = 0.0f;
+            }
+            load_channels<V>(x + t * a.c.x_time + d0, win[i]);
+        } else if (a.c.state) {
+            load_channels<V>(a.c.state + (b * (W - 1) + (W - 1 + t)) * a.c.channels + d0, win[i]);
+        }
+    }
+}
+
+template <int W, int V>
+__device__ __forceinline__ void filter(const float (&w)[W][V], const float (&bias)[V], const float (&win)[W][V], float (&p)[V]) {
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        p[v] = bias[v];
+#pragma unroll
+        for (int k = 0; k < W; ++k) p[v] = __builtin_fmaf(w[k][v], win[k][v], p[v]);
+    }
+}
+
+template <int W, int V> __device__ __forceinline__ void shift(float (&win)[W][V]) {
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[k][v] = win[k + 1][v];
+}
+template <int W, int V> __device__ __forceinline__ void forget(float (&win)[W][V]) {
+#pragma unroll
+    for (int k = 0; k + 1 < W; ++k)
+#pragma unroll
+        for (int v = 0; v < V; ++v) win[k][v] = 0.0f;
+}
+
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kConvThreads) short_conv_forward_kernel(ConvArgs a) {
+    const int cx = threadIdx.x & ((1 << a.cx_log2) - 1), row = threadIdx.x >> a.cx_log2;
+    const int group = static_cast<int>(blockIdx.x % a.channel_blocks) * (1 << a.cx_log2) + cx;
+    const int64_t item = static_cast<int64_t>(blockIdx.x / a.channel_blocks) * (kConvThreads >> a.cx_log2) + row;
+    if (group >= a.groups || item >= a.items) return;
+    const int d0 = group * V;
+    const int64_t b = item / a.segments, t0 = (item - b * a.segments) * a.segment;
+    const int64_t t1 = t0 + a.segment < a.c.length ? t0 + a.segment : a.c.length;
+    const int64_t len = sequence_length(a.c.lengths, b, a.c.length), te = t1 < len ? t1 : len;
+    T* out = static_cast<T*>(a.c.out) + b * a.c.out_batch + d0;
+    if (t0 < len || t0 == 0) {
+        float w[W][V], bias[V], win[W][V];
+        load_weights<W, V>(a, d0, w, bias);
+        load_window<T, W, V>(a, d0, b, t0, win);
+        const T* x = static_cast<const T*>(a.c.x) + b * a.c.x_batch + d0;
+        for (int64_t t = t0; t < te; ++t) {
+            if (a.c.starts && a.c.starts[b * a.c.starts_batch + t * a.c.starts_time]) forget<W, V>(win);
+            load_channels<V>(x + t * a.c.x_time, win[W - 1]);
+            float p[V];
+            filter<W, V>(w, bias, win, p);
+            if (a.c.silu) {
+#pragma unroll
+                for (int v = 0; v < V; ++v) p[v] *= sigmoid_fast(p[v]);
+            }
+            store_channels<V>(out + t * a.c.out_time, p);
+            shift<W, V>(win);
+        }
+        if (a.c.last && (len == 0 || (te == len && t0 < len))) {   // the segment that ends the sequence
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) store_channels<V>(a.c.last + (b * (W - 1) + k) * a.c.channels + d0, win[k]);
+        }
+    }
+    float zero[V];
+#pragma unroll
+    for (int v = 0; v < V; ++v) zero[v] = 0.0f;
+    for (int64_t t = te > t0 ? te : t0; t < t1; ++t) store_channels<V>(out + t * a.c.out_time, zero);
+}
+
+// Backward.  With dp_t = dout_t act'(p_t):  dx_t = sum_j w[W-1-j] dp_{t+j} over the rows t + j that no start parts from t.
+// A thread walks its segment and the W - 1 rows behind it, recomputing p; acc[j] gathers dx of row t - j and is stored
+// when the walk has passed its last reader.  open[j] says whether row t still reaches row t - j.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvArgs a) {
+    extern __shared__ float sums[];   // [rows of threads][lanes][(W + 1) * V]
+    const int cx = threadIdx.x & ((1 << a.cx_log2) - 1), row = threadIdx.x >> a.cx_log2, rows = kConvThreads >> a.cx_log2;
+    const int group = static_cast<int>(blockIdx.x % a.channel_blocks) * (1 << a.cx_log2) + cx;
+    const int64_t slot = blockIdx.x / a.channel_blocks;
+    const bool active = group < a.groups;
+    const int d0 = (active ? group : a.groups - 1) * V;
+    float w[W][V], bias[V], dw[W][V], db[V];
+    load_weights<W, V>(a, d0, w, bias);
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+        db[v] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < W; ++k) dw[k][v] = 0.0f;
+    }
+    for (int64_t item = active ? slot * rows + row : a.items; item < a.items; item += a.slots * rows) {
+        const int64_t b = item / a.segments, t0 = (item - b * a.segments) * a.segment;
+        const int64_t t1 = t0 + a.segment < a.c.length ? t0 + a.segment : a.c.length;
+        const int64_t len = sequence_length(a.c.lengths, b, a.c.length);
+        const T* x = static_cast<const T*>(a.c.x) + b * a.c.x_batch + d0;
+        const T* dy = static_cast<const T*>(a.c.grad_out) + b * a.c.grad_out_batch + d0;
+        T* dx = static_cast<T*>(a.c.grad_x) + b * a.c.grad_x_batch + d0;
+        auto emit = [&](int64_t t, const float (&g)[V]) {
+            if (t >= t0) {
+                if (t < t1) store_channels<V>(dx + t * a.c.grad_x_time, g);
+            } else if (t < 0 && t0 == 0 && a.c.grad_state) {
+                store_channels<V>(a.c.grad_state + (b * (W - 1) + (W - 1 + t)) * a.c.channels + d0, g);
+            }
+        };
+        if (t0 < len || t0 == 0) {
+            float win[W][V], acc[W][V];
+            bool open[W];
+            load_window<T, W, V>(a, d0, b, t0, win);
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                open[j] = true;
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[j][v] = 0.0f;
+            }
+            const int64_t te = t1 + W - 1 < len ? t1 + W - 1 : len;
+            for (int64_t t = t0; t < te; ++t) {
+                if (a.c.starts && a.c.starts[b * a.c.starts_batch + t * a.c.starts_time]) {
+                    forget<W, V>(win);
+#pragma unroll
+                    for (int j = 1; j < W; ++j) open[j] = false;
+                }
+                load_channels<V>(x + t * a.c.x_time, win[W - 1]);
+                float g[V], p[V];
+                load_channels<V>(dy + t * a.c.grad_out_time, g);
+                filter<W, V>(w, bias, win, p);
+                if (a.c.silu) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        const float s = sigmoid_fast(p[v]);
+                        g[v] *= s * __builtin_fmaf(p[v], 1.0f - s, 1.0f);
+                    }
+                }
+#pragma unroll
+                for (int j = 0; j < W; ++j)
+#pragma unroll
+                    for (int v = 0; v < V; ++v) acc[j][v] = open[j] ? __builtin_fmaf(w[W - 1 - j][v], g[v], acc[j][v]) : acc[j][v];
+                if (t < t1) {
+#pragma unroll
+                    for (int v = 0; v < V; ++v) {
+                        db[v] += g[v];
+#pragma unroll
+                        for (int k = 0; k < W; ++k) dw[k][v] = __builtin_fmaf(g[v], win[k][v], dw[k][v]);
+                    }
+                }
+                emit(t - (W - 1), acc[W - 1]);
+                shift<W, V>(win);
+#pragma unroll
+                for (int j = W - 1; j > 0; --j) {
+                    open[j] = open[j - 1];
+#pragma unroll
+                    for (int v = 0; v < V; ++v) acc[j][v] = acc[j - 1][v];
+                }
+                open[0] = true;
+#pragma unroll
+                for (int v = 0; v < V; ++v) acc[0][v] = 0.0f;
+            }
+            if (te == len) {   // rows whose last readers are the carried-out state
+#pragma unroll
+                for (int j = W - 1; j > 0; --j) {
+                    if (a.c.grad_last && open[j]) {
+                        float g[V];
+                        load_channels<V>(a.c.grad_last + (b * (W - 1) + (W - 1 - j)) * a.c.channels + d0, g);
+#pragma unroll
+                        for (int v = 0; v < V; ++v) acc[j][v] += g[v];
+                    }
+                    emit(len - j, acc[j]);
+                }
+            }
+        }
+        float zero[V];
+#pragma unroll
+        for (int v = 0; v < V; ++v) zero[v] = 0.0f;
+        for (int64_t t = len > t0 ? len : t0; t < t1; ++t) store_channels<V>(dx + t * a.c.grad_x_time, zero);
+    }
+    // the workgroup's part of dw and db: one row of partial sums, added over the rows of threads in order
+    constexpr int P = (W + 1) * V;
+    float* mine = sums + threadIdx.x * P;
+#pragma unroll
+    for (int v = 0; v < V; ++v) {
+#pragma unroll
+        for (int k = 0; k < W; ++k) mine[k * V + v] = dw[k][v];
+        mine[W * V + v] = db[v];
+    }
+    __syncthreads();
+    const int lanes = 1 << a.cx_log2;
+    for (int i = threadIdx.x; i < lanes * P; i += kConvThreads) {
+        const int lane = i / P, kv = i - lane * P, k = kv / V, v = kv - k * V;
+        const int g = static_cast<int>(blockIdx.x % a.channel_blocks) * lanes + lane;
+        if (g >= a.groups) continue;
+        float s = 0.0f;
+        for (int r = 0; r < rows; ++r) s += sums[(r * lanes + lane) * P + kv];
+        a.c.workspace[(slot * (W + 1) + k) * a.c.channels + g * V + v] = s;
+    }
+}
+
+// One row per sequence; the state moves up by one row in place.
+template <typename T, int W, int V>
+__global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvArgs a) {
+    const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvThreads + threadIdx.x;
+    if (i >= a.items) return;
+    const int64_t b = i / a.groups;
+    const int d0 = static_cast<int>(i - b * a.groups) * V;
+    float w[W][V], bias[V], win[W][V], p[V];
+    const bool start = a.c.starts && a.c.starts[b * a.c.starts_batch];
+    float* last = a.c.last + b * (W - 1) * a.c.channels + d0;
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) load_channels<V>(last + k * static_cast<int64_t>(a.c.channels), win[k]);
+    load_channels<V>(static_cast<const T*>(a.c.x) + b * a.c.x_batch + d0, win[W - 1]);
+    load_weights<W, V>(a, d0, w, bias);
+    if (start) forget<W, V>(win);
+    filter<W, V>(w, bias, win, p);
+    if (a.c.silu) {
+#pragma unroll
+        for (int v = 0; v < V; ++v) p[v] *= sigmoid_fast(p[v]);
+    }
+    store_channels<V>(static_cast<T*>(a.c.out) + b * a.c.out_batch + d0, p);
+#pragma unroll
+    for (int k = 0; k < W - 1; ++k) store_channels<V>(last + k * static_cast<int64_t>(a.c.channels), win[k + 1]);
+}
+
+// out0[d, k] = sum over the partial rows of value (k, d): 64 columns per workgroup, sixteen threads to a column.
+__global__ void __launch_bounds__(1024) parameter_sums_kernel(const float* partial, int64_t count, int channels, int n0, int columns,
+                                                              float* out0, float* out1, float* out2) {
+    __shared__ double sums[16][64];
+    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
+    const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    double s = 0.0;
+    if (col < columns)
+        for (int64_t r = part; r < count; r += 16) s += static_cast<double>(partial[r * columns + col]);
+    sums[part][lane] = s;
+    __syncthreads();
+    if (part != 0 || col >= columns) return;
+    s = 0.0;
+#pragma unroll
+    for (int k = 0; k < 16; ++k) s += sums[k][lane];
+    const int k = static_cast<int>(col / channels), d = static_cast<int>(col - static_cast<int64_t>(k) * channels);
+    if (k < n0)
+        out0[static_cast<int64_t>(d) * n0 + k] = static_cast<float>(s);
+    else if (k == n0) {
+        if (out1) out1[d] = static_cast<float>(s);
+    } else if (out2)
+        out2[d] = static_cast<float>(s);
+}
+
+void launch_parameter_sums(const float* partial, int64_t count, int32_t channels, int32_t n0, float* out0, float* out1, float* out2,
+                           hipStream_t stream) {
+    const int columns = channels * (n0 + 1 + (out2 ? 1 : 0));
+    ILX_LAUNCH(parameter_sums_kernel, dim3(blocks_for(columns, 64)), dim3(1024), 0, stream, partial, count, static_cast<int>(channels),
+               static_cast<int>(n0), columns, out0, out1, out2);
+}
+
+}  // namespace ilx
+
+using namespace ilx;
+
+namespace {
+
+size_t conv_item_bytes(int dtype) { return dtype == ILX_F32 ? 4 : 2; }
+
+// V channels to an access need every row of every operand on its boundary.
+bool conv_rows_aligned(const void* p, int64_t batch, int64_t time, int64_t batches, int64_t rows, size_t item, int v) {
+    return !p || (aligned_to(p, item * v) && (batches <= 1 || batch % v == 0) && (rows <= 1 || time % v == 0));
+}
+
+int conv_vector(const ilx_short_conv& c, bool backward) {
+    const size_t item = conv_item_bytes(c.dtype);
+    const int v = 4;
+    const auto rows = [&](const void* p, int64_t sb, int64_t st) { return conv_rows_aligned(p, sb, st, c.batch, c.length, item, v); };
+    bool ok = c.channels % v == 0 && rows(c.x, c.x_batch, c.x_time) && rows(c.out, c.out_batch, c.out_time) && aligned_to(c.state, 16) &&
+              aligned_to(c.last, 16);
+    if (backward)
+        ok = ok && rows(c.grad_out, c.grad_out_batch, c.grad_out_time) && rows(c.grad_x, c.grad_x_batch, c.grad_x_time) &&
+             aligned_to(c.grad_last, 16) && aligned_to(c.grad_state, 16);
+    return ok ? v : 1;
+}
+
+ConvArgs conv_args(const ilx_short_conv& c, int v, bool backward) {
+    ConvArgs a{};
+    a.c = c;
+    a.groups = c.channels / v;
+    a.cx_log2 = 0;
+    while (a.cx_log2 < 6 && (1 << a.cx_log2) < a.groups) ++a.cx_log2;
+    a.channel_blocks = (a.groups + (1 << a.cx_log2) - 1) >> a.cx_log2;
+    a.segment = 32;
+    a.segments = c.length > 0 ? (c.length + a.segment - 1) / a.segment : 1;
+    a.items = c.batch * a.segments;
+    const int rows = kConvThreads >> a.cx_log2;
+    a.slots = (a.items + rows - 1) / rows;
+    if (backward) {
+        const int64_t most = 1024 / a.channel_blocks > 0 ? 1024 / a.channel_blocks : 1;
+        if (a.slots > most) a.slots = most;
+    }
+    return a;
+}
+
+int conv_check(const ilx_short_conv& c, const char* name) {
+    ILX_REQUIRE(c.batch >= 0 && c.length >= 0 && c.channels > 0, ILX_EINVAL, "%s: bad shape (%lld, %lld, %d)", name, (long long)c.batch,
+                (long long)c.length, c.channels);
+    ILX_REQUIRE(c.width >= 1 && c.width <= ILX_CONV_MAX_WIDTH, ILX_ESHAPE, "%s: width %d (1..%d supported)", name, c.width,
+                ILX_CONV_MAX_WIDTH);
+    ILX_REQUIRE(c.dtype >= ILX_F32 && c.dtype <= ILX_F16, ILX_EINVAL, "%s: unknown type %d", name, c.dtype);
+    ILX_REQUIRE(c.batch <= INT32_MAX && c.length <= INT32_MAX && c.batch * (c.length + 1) < (int64_t{1} << 40), ILX_ESHAPE,
+                "%s: shape (%lld, %lld) too large", name, (long long)c.batch, (long long)c.length);
+    return ILX_OK;
+}
+
+enum ConvKind { kForward, kBackward, kStep };
+
+template <typename T, int W, int V> void conv_launch(ConvKind kind, const ConvArgs& a, hipStream_t s) {
+    const unsigned threads = kConvThreads;
+    if (kind == kStep) {
+        ILX_LAUNCH((short_conv_step_kernel<T, W, V>), dim3(blocks_for(a.items, kConvThreads)), dim3(threads), 0, s, a);
+    } else if (kind == kForward) {
+        ILX_LAUNCH((short_conv_forward_kernel<T, W, V>), dim3(static_cast<unsigned>(a.slots * a.channel_blocks)), dim3(threads), 0, s, a);
+    } else {
+        ILX_LAUNCH((short_conv_backward_kernel<T, W, V>), dim3(static_cast<unsigned>(a.slots * a.channel_blocks)), dim3(threads),
+                   static_cast<unsigned>(kConvThreads * (W + 1) * V * sizeof(float)), s, a);
+    }
+}
+
+template <typename T, int V> void conv_width(ConvKind kind, const ConvArgs& a, hipStream_t s) {
+    switch (a.c.width) {
+        case 1: return conv_launch<T, 1, V>(kind, a, s);
+        case 2: return conv_launch<T, 2, V>(kind, a, s);
+        case 3: return conv_launch<T, 3, V>(kind, a, s);
+        case 4: return conv_launch<T, 4, V>(kind, a, s);
+        case 5: return conv_launch<T, 5, V>(kind, a, s);
+        case 6: return conv_launch<T, 6, V>(kind, a, s);
+        case 7: return conv_launch<T, 7, V>(kind, a, s);
+        default: return conv_launch<T, 8, V>(kind, a, s);
+    }
+}
+
+template <typename T> void conv_vector_width(ConvKind kind, const ConvArgs& a, int v, hipStream_t s) {
+    if (v == 4)
+        conv_width<T, 4>(kind, a, s);
+    else
+        conv_width<T, 1>(kind, a, s);
+}
+
+void conv_dispatch(ConvKind kind, const ConvArgs& a, int v, hipStream_t s) {
+    switch (a.c.dtype) {
+        case ILX_F32: return conv_vector_width<float>(kind, a, v, s);
+        case ILX_BF16: return conv_vector_width<bf16_t>(kind, a, v, s);
+        default: return conv_vector_width<f16_t>(kind, a, v, s);
+    }
+}
+
+}  // namespace
+
+extern "C" int ilx_short_conv_forward(const ilx_short_conv* conv, void* stream) {
+    ILX_REQUIRE(conv, ILX_EINVAL, "ilx_short_conv_forward: descriptor is NULL");
+    const ilx_short_conv& c = *conv;
+    const int rc = conv_check(c, "ilx_short_conv_forward");
+    if (rc != ILX_OK) return rc;
+    if (c.batch == 0) return ILX_OK;
+    ILX_REQUIRE(c.weight && (c.length == 0 || (c.x && c.out)), ILX_EINVAL, "ilx_short_conv_forward: NULL operand");
+    ILX_REQUIRE(!c.last || c.last != c.state, ILX_EINVAL, "ilx_short_conv_forward: last and state are the same buffer");
+    const int v = conv_vector(c, false);
+    const ConvArgs a = conv_args(c, v, false);
+    ILX_REQUIRE(a.slots * a.channel_blocks <= INT32_MAX, ILX_ESHAPE, "ilx_short_conv_forward: shape too large for one launch");
+    conv_dispatch(kForward, a, v, as_stream(stream));
+    ILX_LAUNCH_CHECK("ilx_short_conv_forward");
+    return ILX_OK;
+}
+
+extern "C" int ilx_short_conv_workspace(const ilx_short_conv* conv, int64_t* floats) {
+    ILX_REQUIRE(conv && floats, ILX_EINVAL, "ilx_short_conv_workspace: NULL argument");
+    const int rc = conv_check(*conv, "ilx_short_conv_workspace");
+    if (rc != ILX_OK) return rc;
+    const ConvArgs a = conv_args(*conv, conv_vector(*conv, true), true);
+    *floats = a.slots * (conv->width + 1) * conv->channels;
+    return ILX_OK;
+}
+
+extern "C" int ilx_short_conv_backward(const ilx_short_conv* conv, void* stream) {
+    ILX_REQUIRE(conv, ILX_EINVAL, "ilx_short_conv_backward: descriptor is NULL");
+    const ilx_short_conv& c = *conv;
+    const int rc = conv_check(c, "ilx_short_conv_backward");
+    if (rc != ILX_OK) return rc;
+    ILX_REQUIRE(c.weight && c.grad_weight && (c.batch == 0 || c.length == 0 || (c.x && c.grad_out && c.grad_x)), ILX_EINVAL,
+                "ilx_short_conv_backward: NULL operand");
+    const int v = conv_vector(c, true);
+    const ConvArgs a = conv_args(c, v, true);
+    ILX_REQUIRE(c.workspace_floats >= a.slots * (c.width + 1) * c.channels && (c.workspace || a.slots == 0), ILX_EINVAL,
+                "ilx_short_conv_backward: workspace of %lld floats, %lld needed", (long long)c.workspace_floats,
+                (long long)(a.slots * (c.width + 1) * c.channels));
+    hipStream_t s = as_stream(stream);
+    if (c.batch > 0) conv_dispatch(kBackward, a, v, s);
+    launch_parameter_sums(c.workspace, a.slots, c.channels, c.width, c.grad_weight, c.grad_bias, nullptr, s);
+    ILX_LAUNCH_CHECK("ilx_short_conv_backward");
+    return ILX_OK;
+}
+
+extern "C" int ilx_short_conv_step(const ilx_short_conv* conv, void* stream) {
+    ILX_REQUIRE(conv, ILX_EINVAL, "ilx_short_conv_step: descriptor is NULL");
+    ilx_short_conv c = *conv;
+    c.length = 1;
+    const int rc = conv_check(c, "ilx_short_conv_step");
+    if (rc != ILX_OK) return rc;
+    if (c.batch == 0) return ILX_OK;
+    ILX_REQUIRE(c.x && c.weight && c.out && (c.width == 1 || (c.state && c.last)), ILX_EINVAL, "ilx_short_conv_step: NULL operand");
+    ILX_REQUIRE(c.state == c.last, ILX_EINVAL, "ilx_short_conv_step: the state is updated in place, last must be state");
+    ILX_REQUIRE(!c.lengths, ILX_EINVAL, "ilx_short_conv_step: lengths must be NULL");
+    const int v = conv_vector(c, false);
+    ConvArgs a = conv_args(c, v, false);
+    a.items = c.batch * a.groups;
+    ILX_REQUIRE((a.items + kConvThreads - 1) / kConvThreads <= INT32_MAX, ILX_ESHAPE, "ilx_short_conv_step: shape too large for one launch");
+    conv_dispatch(kStep, a, v, as_stream(stream));
+    ILX_LAUNCH_CHECK("ilx_short_conv_step");
+    return ILX_OK;
+}

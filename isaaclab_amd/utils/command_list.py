@@ -22,6 +22,7 @@ from .. import _abi
 class CommandList:
     def __init__(self):
         self._handle = None
+        self._kept = []   # buffers that recorded calls allocated for themselves
 
     @contextlib.contextmanager
     def record(self):
@@ -31,12 +32,15 @@ class CommandList:
         handle = ctypes.c_void_p()
         _abi.check(_abi.commands_begin(ctypes.byref(handle)), "ilx_commands_begin")
         self._handle = handle
+        _abi._recording.kept = self._kept
         try:
             yield self
         except BaseException:
+            _abi._recording.kept = None
             _abi.commands_end()
             self.destroy()
             raise
+        _abi._recording.kept = None
         _abi.check(_abi.commands_end(), "ilx_commands_end")
 
     def __len__(self) -> int:
@@ -55,6 +59,7 @@ class CommandList:
         if self._handle is not None:
             _abi.commands_destroy(self._handle)
             self._handle = None
+        self._kept = []
 
     def __del__(self):
         try:

@@ -1,0 +1,471 @@
+"""The memory of a recurrent policy or actuator over time: a short causal convolution and a selective state space recurrence
+on the HIP kernels ``ilx_short_conv_*`` / ``ilx_state_space_*`` (include/isaaclab_amd_sequence.h).
+
+No counterpart in the reference, whose recurrent models are torch modules of the RL libraries.  Like the modifiers and the
+LSTM actuator each operator keeps a state per environment, and it comes in two forms that agree:
+
+* over a sequence (``short_convolution``, ``state_space_scan``): a rollout of all environments or a recording at once, with
+  gradients for training;
+* one environment step (``short_convolution_step``, ``state_space_step``): one row per environment on a carried state, which is
+  updated in place; no gradients.
+
+    out, last = state_space_scan(x, delta, A, B, C, D=D, gate=z, state=state, starts=dones_before, return_state=True)
+    ...
+    out = state_space_step(x, delta, last, A, B, C, D=D, gate=z, starts=env.reset_buf)
+
+Activations are (batch, length, channels) in float32, bfloat16 or float16, with any batch and time strides: a time-major
+rollout buffer goes in as ``buffer.transpose(0, 1)``, and the output has its layout.  Parameters and states are float32, and
+everything is computed in float32.  ``starts`` (batch, length) marks the rows on which an episode begins: nothing from before
+such a row, the carried state included, reaches it.  ``lengths`` (batch) says where a padded sequence ends: rows behind are
+not read, their outputs and gradients are zero, and the state skips them.
+
+As everywhere in this package there is no CPU fallback.  Inside ``CommandList.record`` the calls are recorded with the buffers
+they allocate, which the list keeps; a call whose operands need gradients is refused there (its backward pass runs on
+another thread).
+"""
+
+from __future__ import annotations
+
+import ctypes
+from ctypes import c_int32, c_int64, c_void_p
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _abi
+
+MAX_WIDTH = 8
+MAX_STATES = 32
+_BLOCK = 16   # ILX_SCAN_BLOCK
+_DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class ShortConvDesc(ctypes.Structure):
+    """Mirror of ``ilx_short_conv`` (include/isaaclab_amd_sequence.h)."""
+
+    _fields_ = [
+        ("x", c_void_p), ("x_batch", c_int64), ("x_time", c_int64), ("weight", c_void_p), ("bias", c_void_p), ("state", c_void_p),
+        ("starts", c_void_p), ("starts_batch", c_int64), ("starts_time", c_int64), ("lengths", c_void_p),
+        ("out", c_void_p), ("out_batch", c_int64), ("out_time", c_int64), ("last", c_void_p), ("batch", c_int64), ("length", c_int64),
+        ("channels", c_int32), ("width", c_int32), ("dtype", c_int32), ("silu", c_int32),
+        ("grad_out", c_void_p), ("grad_out_batch", c_int64), ("grad_out_time", c_int64), ("grad_last", c_void_p),
+        ("grad_x", c_void_p), ("grad_x_batch", c_int64), ("grad_x_time", c_int64), ("grad_weight", c_void_p), ("grad_bias", c_void_p),
+        ("grad_state", c_void_p), ("workspace", c_void_p), ("workspace_floats", c_int64),
+    ]
+
+
+class StateSpaceDesc(ctypes.Structure):
+    """Mirror of ``ilx_state_space`` (include/isaaclab_amd_sequence.h)."""
+
+    _fields_ = [
+        ("x", c_void_p), ("x_batch", c_int64), ("x_time", c_int64), ("delta", c_void_p), ("delta_batch", c_int64), ("delta_time", c_int64),
+        ("gate", c_void_p), ("gate_batch", c_int64), ("gate_time", c_int64), ("A", c_void_p),
+        ("B", c_void_p), ("B_batch", c_int64), ("B_time", c_int64), ("C", c_void_p), ("C_batch", c_int64), ("C_time", c_int64),
+        ("D", c_void_p), ("delta_bias", c_void_p), ("state", c_void_p), ("starts", c_void_p), ("starts_batch", c_int64),
+        ("starts_time", c_int64), ("lengths", c_void_p), ("out", c_void_p), ("out_batch", c_int64), ("out_time", c_int64),
+        ("last", c_void_p), ("saved", c_void_p), ("batch", c_int64), ("length", c_int64), ("channels", c_int32), ("states", c_int32),
+        ("groups", c_int32), ("dtype", c_int32), ("bc_dtype", c_int32), ("softplus", c_int32),
+        ("grad_out", c_void_p), ("grad_out_batch", c_int64), ("grad_out_time", c_int64), ("grad_last", c_void_p),
+        ("grad_x", c_void_p), ("grad_x_batch", c_int64), ("grad_x_time", c_int64),
+        ("grad_delta", c_void_p), ("grad_delta_batch", c_int64), ("grad_delta_time", c_int64),
+        ("grad_gate", c_void_p), ("grad_gate_batch", c_int64), ("grad_gate_time", c_int64),
+        ("grad_A", c_void_p), ("grad_B", c_void_p), ("grad_C", c_void_p), ("grad_D", c_void_p), ("grad_delta_bias", c_void_p),
+        ("grad_state", c_void_p), ("workspace", c_void_p), ("workspace_floats", c_int64),
+    ]
+
+
+_P = c_void_p
+_conv_forward = _abi._sig("ilx_short_conv_forward", _P, _P)
+_conv_workspace = _abi._sig("ilx_short_conv_workspace", _P, _P)
+_conv_backward = _abi._sig("ilx_short_conv_backward", _P, _P)
+_conv_step = _abi._sig("ilx_short_conv_step", _P, _P)
+_scan_forward = _abi._sig("ilx_state_space_forward", _P, _P)
+_scan_workspace = _abi._sig("ilx_state_space_workspace", _P, c_int32, _P)
+_scan_backward = _abi._sig("ilx_state_space_backward", _P, _P)
+_scan_step = _abi._sig("ilx_state_space_step", _P, _P)
+
+
+def _launch(fn, desc, what: str, device: torch.device):
+    """One call on the tensors' device and its current stream."""
+    if device.index == torch.cuda.current_device():
+        _abi.check(fn(ctypes.byref(desc), _abi.stream()), what)
+    else:
+        with torch.cuda.device(device):
+            _abi.check(fn(ctypes.byref(desc), _abi.stream()), what)
+
+
+def _p(t: torch.Tensor | None):
+    return None if t is None else t.data_ptr()
+
+
+def _copy(t: torch.Tensor, name: str, **how) -> torch.Tensor:
+    """A dense copy (``how``: in another type).  A recorded call would go on reading the values of the recording."""
+    if _abi.recording():
+        raise _abi.IlxError(f"{name} would be copied before the call, which a command list does not record: pass it dense, and 16-bit B and C with an even number of states")
+    return t.to(**how).contiguous()
+
+
+def _check_activation(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+    """``t`` with unit channel stride (copied only if it has another)."""
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype != like.dtype:
+        raise ValueError(f"{name} is {t.dtype} beside {like.dtype} activations")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the activations on {like.device}")
+    return t if t.stride(-1) == 1 or t.shape[-1] == 1 else _copy(t, name)
+
+
+def _check_parameter(t: torch.Tensor | None, name: str, shape: tuple, device) -> torch.Tensor | None:
+    if t is None:
+        return None
+    if tuple(t.shape) != shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
+    if t.dtype != torch.float32:
+        raise ValueError(f"{name} is {t.dtype}: parameters and states are float32")
+    if t.device != device:
+        raise ValueError(f"{name} is on {t.device}, the activations on {device}")
+    return t if t.is_contiguous() else _copy(t, name)
+
+
+def _check_x(x: torch.Tensor, dims: int):
+    if not x.is_cuda:
+        raise _abi.IlxError("isaaclab_amd kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
+    if x.dim() != dims:
+        raise ValueError(f"x has shape {tuple(x.shape)}, expected {'(batch, length, channels)' if dims == 3 else '(batch, channels)'}")
+    if x.dtype not in _DTYPES:
+        raise ValueError(f"activations are float32, bfloat16 or float16, got {x.dtype}")
+    if x.shape[-1] == 0:
+        raise ValueError("x has no channels")
+
+
+def _check_starts(starts: torch.Tensor | None, shape: tuple, device) -> torch.Tensor | None:
+    if starts is None:
+        return None
+    if tuple(starts.shape) != shape or starts.dtype not in (torch.bool, torch.uint8):
+        raise ValueError(f"starts is {starts.dtype} {tuple(starts.shape)}, expected bool {shape}")
+    if starts.device != device:
+        raise ValueError(f"starts is on {starts.device}, the activations on {device}")
+    return starts
+
+
+def _check_lengths(lengths: torch.Tensor | None, batch: int, device) -> torch.Tensor | None:
+    if lengths is None:
+        return None
+    if tuple(lengths.shape) != (batch,) or lengths.dtype not in (torch.int32, torch.int64):
+        raise ValueError(f"lengths is {lengths.dtype} {tuple(lengths.shape)}, expected int32 or int64 {(batch,)}")
+    if lengths.device != device:
+        raise ValueError(f"lengths is on {lengths.device}, the activations on {device}")
+    return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else _copy(lengths, "lengths", dtype=torch.int32)
+
+
+def _check_state(state: torch.Tensor, shape: tuple, x: torch.Tensor):
+    """A state that is updated in place: it cannot be a copy."""
+    if not isinstance(state, torch.Tensor):
+        raise ValueError("a step needs its carried state (zeros for a new sequence)")
+    if not state.is_contiguous():
+        raise ValueError("state is updated in place and must be contiguous")
+    _check_parameter(state, "state", shape, x.device)
+
+
+def _no_gradients(what: str, *tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or use the form over sequences")
+
+
+def _needs_gradients(*tensors) -> bool:
+    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+        return False
+    if _abi.recording():
+        raise _abi.IlxError("a call that needs gradients cannot be recorded in a command list (its backward pass runs on another thread)")
+    return True
+
+
+def _check_out(out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
+    if out is None:
+        return _abi.keep(torch.empty_like(x))
+    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
+        raise ValueError(f"out must be like x ({tuple(x.shape)}, {x.dtype}) with unit channel stride")
+    return out
+
+
+def _written(t: torch.Tensor):
+    """Autograd sees the in-place update: a backward pass that needs the value from before it fails loudly."""
+    if not t.is_inference():
+        torch.autograd.graph.increment_version(t)
+
+
+# ---- short convolution ----------------------------------------------------------------------------------------------
+def _silu(activation) -> int:
+    if activation not in (None, "silu"):
+        raise ValueError(f"unsupported activation '{activation}', expected None or 'silu'")
+    return int(activation == "silu")
+
+
+def _conv_desc(x, weight, bias, state, starts, lengths, silu) -> ShortConvDesc:
+    batch, length, channels = x.shape
+    return ShortConvDesc(
+        x=x.data_ptr(), x_batch=x.stride(0), x_time=x.stride(1), weight=weight.data_ptr(), bias=_p(bias), state=_p(state), starts=_p(starts),
+        starts_batch=starts.stride(0) if starts is not None else 0, starts_time=starts.stride(1) if starts is not None else 0,
+        lengths=_p(lengths), batch=batch, length=length, channels=channels, width=weight.shape[1], dtype=_DTYPES[x.dtype], silu=silu)
+
+
+def _conv_call(x, weight, bias, state, starts, lengths, silu, want_last):
+    desc = _conv_desc(x, weight, bias, state, starts, lengths, silu)
+    out = _abi.keep(torch.empty_like(x))
+    last = _abi.keep(torch.empty(x.shape[0], weight.shape[1] - 1, x.shape[2], device=x.device)) if want_last else None
+    desc.out, desc.out_batch, desc.out_time, desc.last = out.data_ptr(), out.stride(0), out.stride(1), _p(last)
+    _launch(_conv_forward, desc, "ilx_short_conv_forward", x.device)
+    return out, last
+
+
+class _ShortConvolution(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, weight, bias, state, starts, lengths, silu, want_last):
+        ctx.set_materialize_grads(False)
+        ctx.save_for_backward(x, weight, bias, state, starts, lengths)
+        ctx.silu = silu
+        return _conv_call(x, weight, bias, state, starts, lengths, silu, want_last)
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_last):
+        x, weight, bias, state, starts, lengths = ctx.saved_tensors
+        grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", tuple(x.shape), x)
+        grad_last = None if grad_last is None else grad_last.contiguous()
+        grad_x, grad_weight = torch.empty_like(x), torch.empty_like(weight)
+        grad_bias = None if bias is None else torch.empty_like(bias)
+        grad_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
+        d = _conv_desc(x, weight, bias, state, starts, lengths, ctx.silu)
+        d.grad_out, d.grad_out_batch, d.grad_out_time, d.grad_last = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1), _p(grad_last)
+        d.grad_x, d.grad_x_batch, d.grad_x_time = grad_x.data_ptr(), grad_x.stride(0), grad_x.stride(1)
+        d.grad_weight, d.grad_bias, d.grad_state = grad_weight.data_ptr(), _p(grad_bias), _p(grad_state)
+        need = c_int64()
+        _abi.check(_conv_workspace(ctypes.byref(d), ctypes.byref(need)), "ilx_short_conv_workspace")
+        workspace = torch.empty(need.value, device=x.device)
+        d.workspace, d.workspace_floats = workspace.data_ptr(), need.value
+        _launch(_conv_backward, d, "ilx_short_conv_backward", x.device)
+        return grad_x, grad_weight, grad_bias, grad_state, None, None, None, None
+
+
+def short_convolution(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
+                      state: torch.Tensor | None = None, starts: torch.Tensor | None = None, lengths: torch.Tensor | None = None,
+                      return_state: bool = False):
+    """Causal convolution over time, one filter per channel: ``out[b, t] = act(bias + sum_j weight[:, W - 1 - j] * x[b, t - j])``.
+
+    ``x`` (batch, length, channels), ``weight`` (channels, W) with W up to 8, ``activation`` None or ``"silu"``.  ``state``
+    (batch, W - 1, channels) holds the rows ahead of the first, oldest first (zeros if None).  With ``return_state`` the
+    result is ``(out, last)``, ``last`` being the state ahead of the next row.  Differentiable in ``x``, ``weight``,
+    ``bias`` and ``state``."""
+    _check_x(x, 3)
+    batch, length, channels = x.shape
+    silu = _silu(activation)
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (channels, width) with a width of 1..{MAX_WIDTH}")
+    x = _check_activation(x, "x", (batch, length, channels), x)
+    weight = _check_parameter(weight, "weight", (channels, weight.shape[1]), x.device)
+    bias = _check_parameter(bias, "bias", (channels,), x.device)
+    state = _check_parameter(state, "state", (batch, weight.shape[1] - 1, channels), x.device)
+    starts = _check_starts(starts, (batch, length), x.device)
+    lengths = _check_lengths(lengths, batch, x.device)
+    args = (x, weight, bias, state, starts, lengths, silu, return_state)
+    out, last = _ShortConvolution.apply(*args) if _needs_gradients(x, weight, bias, state) else _conv_call(*args)
+    return (out, last) if return_state else out
+
+
+def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
+                           activation: str | None = None, starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One row of :func:`short_convolution` per sequence: ``x`` (batch, channels), ``state`` (batch, W - 1, channels) updated in
+    place, ``starts`` (batch) the environments whose episode begins with this row.  ``out`` may name the result's buffer."""
+    _check_x(x, 2)
+    _no_gradients("short_convolution_step", x, weight, bias, state)
+    batch, channels = x.shape
+    silu = _silu(activation)
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (channels, width) with a width of 1..{MAX_WIDTH}")
+    x = _abi.keep(_check_activation(x, "x", (batch, channels), x))
+    weight = _abi.keep(_check_parameter(weight, "weight", (channels, weight.shape[1]), x.device))
+    bias = _abi.keep(_check_parameter(bias, "bias", (channels,), x.device))
+    _check_state(state, (batch, weight.shape[1] - 1, channels), x)
+    starts = _check_starts(starts, (batch,), x.device)
+    out = _check_out(out, x)
+    desc = ShortConvDesc(
+        x=x.data_ptr(), x_batch=x.stride(0), weight=weight.data_ptr(), bias=_p(bias), state=state.data_ptr(), starts=_p(starts),
+        starts_batch=starts.stride(0) if starts is not None else 0, out=out.data_ptr(), out_batch=out.stride(0), last=state.data_ptr(),
+        batch=batch, length=1, channels=channels, width=weight.shape[1], dtype=_DTYPES[x.dtype], silu=silu)
+    _launch(_conv_step, desc, "ilx_short_conv_step", x.device)
+    _written(state)
+    return out
+
+
+# ---- state space recurrence -------------------------------------------------------------------------------------------
+def _shared(t: torch.Tensor, name: str, lead: tuple, like: torch.Tensor) -> torch.Tensor:
+    """B or C as (*lead, groups, states), dense over the last two: in the activations' type or float32."""
+    if t.dim() == len(lead) + 1:
+        t = t.unsqueeze(-2)
+    if t.dim() != len(lead) + 2 or tuple(t.shape[:-2]) != lead:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {lead} + (groups, states) or (states,)")
+    if t.dtype not in (like.dtype, torch.float32):
+        raise ValueError(f"{name} is {t.dtype} beside {like.dtype} activations")
+    if t.device != like.device:
+        raise ValueError(f"{name} is on {t.device}, the activations on {like.device}")
+    g, n = t.shape[-2:]
+    return t if (n == 1 or t.stride(-1) == 1) and (g == 1 or t.stride(-2) == n) else _copy(t, name)
+
+
+def _readable(t: torch.Tensor) -> torch.Tensor:
+    """16-bit rows are read in pairs: an odd number of states, odd strides or an odd address go through a float32 copy."""
+    if t.dtype == torch.float32 or (t.shape[-1] % 2 == 0 and all(s % 2 == 0 for s in t.stride()[:-2]) and t.data_ptr() % 4 == 0):
+        return t
+    return _copy(t, "B or C", dtype=torch.float32)
+
+
+def _pair(B: torch.Tensor, C: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
+    B, C = _readable(B), _readable(C)
+    if B.dtype != C.dtype:
+        B, C = (t if t.dtype == torch.float32 else _copy(t, "B or C", dtype=torch.float32) for t in (B, C))
+    return B, C
+
+
+def _scan_desc(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus) -> StateSpaceDesc:
+    batch, length, channels = x.shape
+    d = StateSpaceDesc(
+        x=x.data_ptr(), x_batch=x.stride(0), x_time=x.stride(1), delta=delta.data_ptr(), delta_batch=delta.stride(0), delta_time=delta.stride(1),
+        A=A.data_ptr(), B=B.data_ptr(), B_batch=B.stride(0), B_time=B.stride(1), C=C.data_ptr(), C_batch=C.stride(0), C_time=C.stride(1),
+        D=_p(D), delta_bias=_p(delta_bias), state=_p(state), starts=_p(starts), lengths=_p(lengths), batch=batch, length=length,
+        channels=channels, states=A.shape[1], groups=B.shape[2], dtype=_DTYPES[x.dtype], bc_dtype=_DTYPES[B.dtype], softplus=softplus)
+    if gate is not None:
+        d.gate, d.gate_batch, d.gate_time = gate.data_ptr(), gate.stride(0), gate.stride(1)
+    if starts is not None:
+        d.starts_batch, d.starts_time = starts.stride(0), starts.stride(1)
+    return d
+
+
+def _scan_scratch(desc: StateSpaceDesc, backward: int, device) -> torch.Tensor | None:
+    need = c_int64()
+    _abi.check(_scan_workspace(ctypes.byref(desc), backward, ctypes.byref(need)), "ilx_state_space_workspace")
+    if need.value == 0:
+        return None
+    workspace = _abi.keep(torch.empty(need.value, device=device))
+    desc.workspace, desc.workspace_floats = workspace.data_ptr(), need.value
+    return workspace
+
+
+def _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last, save=False):
+    B, C = _pair(B, C)
+    _abi.keep(B), _abi.keep(C)
+    desc = _scan_desc(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus)
+    batch, length, channels = x.shape
+    out = _abi.keep(torch.empty_like(x))
+    last = _abi.keep(torch.empty(batch, A.shape[1], channels, device=x.device)) if want_last else None
+    saved = torch.empty(batch, (length + _BLOCK - 1) // _BLOCK, A.shape[1], channels, device=x.device) if save else None
+    desc.out, desc.out_batch, desc.out_time, desc.last, desc.saved = out.data_ptr(), out.stride(0), out.stride(1), _p(last), _p(saved)
+    workspace = _scan_scratch(desc, 0, x.device)  # noqa: F841  (alive until the launch is queued)
+    _launch(_scan_forward, desc, "ilx_state_space_forward", x.device)
+    return out, last, saved
+
+
+class _StateSpaceScan(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last):
+        ctx.set_materialize_grads(False)
+        out, last, saved = _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last, True)
+        ctx.save_for_backward(x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved)
+        ctx.softplus, ctx.has_state = softplus, state is not None
+        return out, last
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, grad_out, grad_last):
+        x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved = ctx.saved_tensors
+        grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", tuple(x.shape), x)
+        grad_last = None if grad_last is None else grad_last.contiguous()
+        rB, rC = _pair(B, C)
+        d = _scan_desc(x, delta, A, rB, rC, D, gate, delta_bias, None, starts, lengths, ctx.softplus)
+        gx, gdelta, gA = torch.empty_like(x), torch.empty_like(delta), torch.empty_like(A)
+        gB, gC = torch.empty(rB.shape, dtype=rB.dtype, device=x.device), torch.empty(rC.shape, dtype=rC.dtype, device=x.device)
+        gD, ggate, gbias = (None if t is None else torch.empty_like(t) for t in (D, gate, delta_bias))
+        gstate = torch.empty(x.shape[0], A.shape[1], x.shape[2], device=x.device) if ctx.has_state and ctx.needs_input_grad[8] else None
+        d.saved = saved.data_ptr()
+        for name, t in (("grad_out", grad_out), ("grad_x", gx), ("grad_delta", gdelta), ("grad_gate", ggate)):
+            if t is not None:
+                setattr(d, name, t.data_ptr())
+                setattr(d, name + "_batch", t.stride(0))
+                setattr(d, name + "_time", t.stride(1))
+        d.grad_last, d.grad_A, d.grad_B, d.grad_C = _p(grad_last), gA.data_ptr(), gB.data_ptr(), gC.data_ptr()
+        d.grad_D, d.grad_delta_bias, d.grad_state = _p(gD), _p(gbias), _p(gstate)
+        workspace = _scan_scratch(d, 1, x.device)  # noqa: F841
+        _launch(_scan_backward, d, "ilx_state_space_backward", x.device)
+        return gx, gdelta, gA, gB.to(B.dtype), gC.to(C.dtype), gD, ggate, gbias, gstate, None, None, None, None
+
+
+def _scan_operands(x, delta, A, B, C, D, gate, delta_bias):
+    lead, channels = tuple(x.shape[:-1]), x.shape[-1]
+    if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATES:
+        raise ValueError(f"A has shape {tuple(A.shape)}, expected (channels, states) with 1..{MAX_STATES} states")
+    x = _check_activation(x, "x", tuple(x.shape), x)
+    delta = _check_activation(delta, "delta", tuple(x.shape), x)
+    gate = None if gate is None else _check_activation(gate, "gate", tuple(x.shape), x)
+    A = _check_parameter(A, "A", (channels, A.shape[1]), x.device)
+    D = _check_parameter(D, "D", (channels,), x.device)
+    delta_bias = _check_parameter(delta_bias, "delta_bias", (channels,), x.device)
+    B, C = _shared(B, "B", lead, x), _shared(C, "C", lead, x)
+    if B.shape != C.shape or B.shape[-1] != A.shape[1] or B.shape[-2] < 1 or channels % B.shape[-2]:
+        raise ValueError(f"B {tuple(B.shape)} and C {tuple(C.shape)} must have {A.shape[1]} states and groups that divide {channels} channels")
+    return x, delta, A, B, C, D, gate, delta_bias
+
+
+def state_space_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                     D: torch.Tensor | None = None, gate: torch.Tensor | None = None, delta_bias: torch.Tensor | None = None,
+                     softplus: bool = True, state: torch.Tensor | None = None, starts: torch.Tensor | None = None,
+                     lengths: torch.Tensor | None = None, return_state: bool = False):
+    """Selective state space recurrence over time, per channel d (of group g) with N states::
+
+        dt = softplus(delta + delta_bias)           (or the sum itself)
+        h  = exp(dt * A[d]) * h + dt * B[b, t, g] * x,     y = (C[b, t, g] * h).sum() + D[d] * x
+        out = y, or y * gate * sigmoid(gate)
+
+    ``x``, ``delta``, ``gate`` (batch, length, channels); ``A`` (channels, N), N up to 32; ``B``, ``C`` (batch, length, groups, N)
+    or (batch, length, N) shared by all channels, in x's type or float32; ``D``, ``delta_bias`` (channels).  ``state`` (batch,
+    N, channels) is the state ahead of the first row (zeros if None); with ``return_state`` the result is ``(out, last)``.
+    Differentiable in every operand but ``starts`` and ``lengths``; between a forward and its backward pass one state in 16
+    rows is kept."""
+    _check_x(x, 3)
+    batch, length, channels = x.shape
+    x, delta, A, B, C, D, gate, delta_bias = _scan_operands(x, delta, A, B, C, D, gate, delta_bias)
+    state = _check_parameter(state, "state", (batch, A.shape[1], channels), x.device)
+    starts = _check_starts(starts, (batch, length), x.device)
+    lengths = _check_lengths(lengths, batch, x.device)
+    args = (x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, int(bool(softplus)), return_state)
+    if _needs_gradients(x, delta, A, B, C, D, gate, delta_bias, state):
+        out, last = _StateSpaceScan.apply(*args)
+    else:
+        out, last, _ = _scan_call(*args)
+    return (out, last) if return_state else out
+
+
+def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
+                     D: torch.Tensor | None = None, gate: torch.Tensor | None = None, delta_bias: torch.Tensor | None = None,
+                     softplus: bool = True, starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
+    """One row of :func:`state_space_scan` per sequence: ``x``, ``delta``, ``gate`` (batch, channels), ``B``, ``C`` (batch, groups,
+    N) or (batch, N), ``state`` (batch, N, channels) updated in place, ``starts`` (batch) the environments whose episode begins
+    with this row.  ``out`` may name the result's buffer."""
+    _check_x(x, 2)
+    _no_gradients("state_space_step", x, delta, state, A, B, C, D, gate, delta_bias)
+    batch, channels = x.shape
+    x, delta, A, B, C, D, gate, delta_bias = _scan_operands(x, delta, A, B, C, D, gate, delta_bias)
+    B, C = _pair(B, C)
+    for t in (x, delta, A, B, C, D, gate, delta_bias):
+        _abi.keep(t)
+    _check_state(state, (batch, A.shape[1], channels), x)
+    starts = _check_starts(starts, (batch,), x.device)
+    out = _check_out(out, x)
+    desc = StateSpaceDesc(
+        x=x.data_ptr(), x_batch=x.stride(0), delta=delta.data_ptr(), delta_batch=delta.stride(0), gate=_p(gate),
+        gate_batch=gate.stride(0) if gate is not None else 0, A=A.data_ptr(), B=B.data_ptr(), B_batch=B.stride(0), C=C.data_ptr(), C_batch=C.stride(0),
+        D=_p(D), delta_bias=_p(delta_bias), state=state.data_ptr(), starts=_p(starts), starts_batch=starts.stride(0) if starts is not None else 0,
+        out=out.data_ptr(), out_batch=out.stride(0), last=state.data_ptr(), batch=batch, length=1, channels=channels, states=A.shape[1],
+        groups=B.shape[1], dtype=_DTYPES[x.dtype], bc_dtype=_DTYPES[B.dtype], softplus=int(bool(softplus)))
+    _launch(_scan_step, desc, "ilx_state_space_step", x.device)
+    _written(state)
+    return out
