@@ -106,7 +106,7 @@ typedef struct ilx_state_space {
     int64_t batch, length;
     int32_t channels, states, groups;
     int32_t dtype;    /* of x, delta, gate, out and their gradients */
-    int32_t bc_dtype; /* of B and C: dtype or ILX_F32; 16 bit needs even strides, states and 4-byte aligned pointers */
+    int32_t bc_dtype; /* of B and C: dtype or ILX_F32 */
     int32_t softplus;
     /* backward only; the gradient of every operand but B and C has the strides named here, those of B and C are dense */
     const void* grad_out;

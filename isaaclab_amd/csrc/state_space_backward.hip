@@ -41,11 +41,12 @@ __device__ __forceinline__ float sum_lanes(const float (&v)[8], int lane) {
     return dpp_add<0xb1>(s); // quad_perm 1,0,3,2
 }
 
-template <typename T, typename TB, int NW, bool FULL>
-__global__ void __launch_bounds__(64 * NW) scan_backward_kernel(ScanArgs a) {
+template <typename T, typename TB, int NW>
+__global__ void __launch_bounds__(64 * NW, NW < 8 ? 8 / NW : 1) scan_backward_kernel(ScanArgs a) {
     constexpr int E = kRows / NW;   // rows a wave prepares and finishes per block
-    __shared__ float s_dt[kRows][64], s_x[kRows][64], s_dy[kRows][64];
-    __shared__ float s_rb[NW][kRows][64], s_ra[NW][kRows][64], s_y[NW][kRows][64];
+    __shared__ float4 s_row[kRows][64];           // dt, dt x, dy, x
+    __shared__ float2 s_sum[NW][kRows][64];       // sum r B and sum r p A over the wave's states
+    __shared__ float s_y[NW][kRows][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = w * kStates;
     const int block = blockIdx.x % a.blocks;
     const int64_t slot = blockIdx.x / a.blocks;
@@ -54,152 +55,201 @@ __global__ void __launch_bounds__(64 * NW) scan_backward_kernel(ScanArgs a) {
     const ilx_state_space& s = a.s;
     const int64_t channels = s.channels;
     float A[kStates], A2[kStates], dA[kStates];
+    uint32_t state_at[kStates];   // of the wave's states in a (states, channels) array; past the last state: its last
 #pragma unroll
     for (int n = 0; n < kStates; ++n) {
-        A[n] = FULL || n0 + n < s.states ? s.A[static_cast<int64_t>(c.d) * s.states + n0 + n] : 0.0f;
+        const bool in = n0 + n < s.states;
+        A[n] = in ? s.A[static_cast<int64_t>(c.d) * s.states + n0 + n] : 0.0f;
         A2[n] = A[n] * kLog2e;
         dA[n] = 0.0f;
+        state_at[n] = static_cast<uint32_t>((in ? n0 + n : s.states - 1) * s.channels + c.d);
     }
     const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f, skip = s.D ? s.D[c.d] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
     const int value = (lane >> 5 & 1) + 2 * (lane >> 4 & 1) + 4 * (lane >> 3 & 1);   // what sum_lanes leaves here
     const int shared_column = (value >> 2) * (NW * kStates) + n0 + (value & 3);
+    // B and C of four rows and the wave's four states in every 16 lanes
+    const int bc_row = lane >> 2 & 3, bc_state = n0 + (lane & 3);
+    const bool bc_in = bc_state < s.states;
+    const int bc_at = bc_in ? bc_state : s.states - 1;
 
-    for (int64_t b = slot; b < s.batch; b += a.slots) {
-        const int64_t len = scan_length(s, b);
-        const T* px = static_cast<const T*>(s.x) + b * s.x_batch + c.d;
-        const T* pd = static_cast<const T*>(s.delta) + b * s.delta_batch + c.d;
-        const T* pz = s.gate ? static_cast<const T*>(s.gate) + b * s.gate_batch + c.d : nullptr;
-        const T* pg = static_cast<const T*>(s.grad_out) + b * s.grad_out_batch + c.d;
+    const uint32_t parts = static_cast<uint32_t>(a.parts);
+    for (int64_t item = slot; item < s.batch * a.parts; item += a.slots) {
+        const int64_t b = static_cast<uint32_t>(item) / parts, part = static_cast<uint32_t>(item) % parts;
+        const int64_t len = scan_length(s, b), begin = part * a.part_rows;
+        const int64_t limit = begin + a.part_rows < s.length ? begin + a.part_rows : s.length, end = limit < len ? limit : len;
+        const T* px = static_cast<const T*>(s.x) + b * s.x_batch;
+        const T* pd = static_cast<const T*>(s.delta) + b * s.delta_batch;
+        const T* pz = s.gate ? static_cast<const T*>(s.gate) + b * s.gate_batch : nullptr;
+        const T* pg = static_cast<const T*>(s.grad_out) + b * s.grad_out_batch;
         const TB* pB = static_cast<const TB*>(s.B) + b * s.B_batch + c.group * s.states;
         const TB* pC = static_cast<const TB*>(s.C) + b * s.C_batch + c.group * s.states;
-        T* gx = static_cast<T*>(s.grad_x) + b * s.grad_x_batch + c.d;
-        T* gd = static_cast<T*>(s.grad_delta) + b * s.grad_delta_batch + c.d;
-        T* gz = s.gate ? static_cast<T*>(s.grad_gate) + b * s.grad_gate_batch + c.d : nullptr;
+        T* gx = static_cast<T*>(s.grad_x) + b * s.grad_x_batch;
+        T* gd = static_cast<T*>(s.grad_delta) + b * s.grad_delta_batch;
+        T* gz = s.gate ? static_cast<T*>(s.grad_gate) + b * s.grad_gate_batch : nullptr;
+        const float* enters = a.parts > 1 ? a.part_state + item * s.states * channels : s.grad_last ? s.grad_last + b * s.states * channels : nullptr;
         float r[kStates];
 #pragma unroll
-        for (int n = 0; n < kStates; ++n)
-            r[n] = s.grad_last && c.active && (FULL || n0 + n < s.states) ? s.grad_last[(b * s.states + n0 + n) * channels + c.d] : 0.0f;
-        for (int64_t t = len + w; t < s.length; t += NW) {
+        for (int n = 0; n < kStates; ++n) r[n] = enters && c.active && n0 + n < s.states ? enters[state_at[n]] : 0.0f;
+        for (int64_t t = (begin > len ? begin : len) + w; t < limit; t += NW) {
             if (!c.active) break;
-            gx[t * s.grad_x_time] = from_f32<T>(0.0f);
-            gd[t * s.grad_delta_time] = from_f32<T>(0.0f);
-            if (gz) gz[t * s.grad_gate_time] = from_f32<T>(0.0f);
+            (gx + t * s.grad_x_time)[c.d] = from_f32<T>(0.0f);
+            (gd + t * s.grad_delta_time)[c.d] = from_f32<T>(0.0f);
+            if (gz) (gz + t * s.grad_gate_time)[c.d] = from_f32<T>(0.0f);
         }
-        for (int64_t blk = (len + kRows - 1) / kRows - 1; blk >= 0; --blk) {
-            const int64_t t0 = blk * kRows;
-            const int count = len - t0 < kRows ? static_cast<int>(len - t0) : kRows;
+        // the inputs of a block, read while the block behind it is worked on
+        T in_d[E], in_x[E], in_g[E], in_z[E];
+        TB in_B[kRows / 4], in_C[kRows / 4];
+        float in_h[kStates];
+        uint64_t in_starts = 0;
+        auto read = [&](int64_t t0) {
+            const int count = end - t0 < kRows ? static_cast<int>(end - t0) : kRows;
+#pragma unroll
+            for (int e = 0; e < E; ++e) {
+                const int i = e * NW + w;
+                const uint32_t t = static_cast<uint32_t>(t0 + (i < count ? i : count - 1));
+                in_d[e] = (pd + row_offset(t, s.delta_time))[c.d];
+                in_x[e] = (px + row_offset(t, s.x_time))[c.d];
+                in_g[e] = (pg + row_offset(t, s.grad_out_time))[c.d];
+                if (pz) in_z[e] = (pz + row_offset(t, s.gate_time))[c.d];
+            }
+#pragma unroll
+            for (int k = 0; k < kRows / 4; ++k) {
+                const int i = 4 * k + bc_row;
+                const uint32_t t = static_cast<uint32_t>(t0 + (i < count ? i : count - 1));
+                in_B[k] = pB[row_offset(t, s.B_time) + bc_at];
+                in_C[k] = pC[row_offset(t, s.C_time) + bc_at];
+            }
+            const float* save = s.saved + (b * a.saved_blocks + t0 / kRows) * s.states * channels;
+#pragma unroll
+            for (int n = 0; n < kStates; ++n) in_h[n] = save[state_at[n]];
+            in_starts = start_bits(s, b, t0, count, lane);
+        };
+        const int64_t last_block = begin < end ? begin + (end - begin - 1) / kRows * kRows : begin - kRows;
+        if (last_block >= begin) read(last_block);
+        for (int64_t t0 = last_block; t0 >= begin; t0 -= kRows) {
+            const int count = end - t0 < kRows ? static_cast<int>(end - t0) : kRows;
             // rows past the end act as rows that leave the state alone: dt = x = dy = 0
             float slope[E], dgate[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int i = e * NW + w;
                 const bool in = i < count && c.active;
-                const int64_t t = t0 + (i < count ? i : count - 1);
-                const float raw = to_f32(pd[t * s.delta_time]) + bias, x = to_f32(px[t * s.x_time]), g = to_f32(pg[t * s.grad_out_time]);
+                const float raw = to_f32(in_d[e]) + bias, x = in ? to_f32(in_x[e]) : 0.0f, g = to_f32(in_g[e]);
                 float dy = g;
                 dgate[e] = 0.0f;
                 if (pz) {
-                    const float z = to_f32(pz[t * s.gate_time]), sig = sigmoid_fast(z);
+                    const float z = to_f32(in_z[e]), sig = sigmoid_fast(z);
                     dy = g * z * sig;
                     dgate[e] = g * sig * __builtin_fmaf(z, 1.0f - sig, 1.0f);
                 }
                 slope[e] = s.softplus ? sigmoid_fast(raw) : 1.0f;
-                s_dt[i][lane] = in ? (s.softplus ? softplus_f(raw) : raw) : 0.0f;
-                s_x[i][lane] = in ? x : 0.0f;
-                s_dy[i][lane] = in ? dy : 0.0f;
+                const float dt = in ? (s.softplus ? softplus_f(raw) : raw) : 0.0f;
+                s_row[i][lane] = make_float4(dt, dt * x, in ? dy : 0.0f, x);
             }
-            const uint64_t starts = start_bits(s, b, t0, count, lane);
-            float h[kStates], decay[kRows][kStates], p[kRows][kStates];
-            const float* save = s.saved + (b * a.saved_blocks + blk) * s.states * channels + c.d;
+            float B[kRows / 4], C[kRows / 4], h0[kStates], decay[kRows][kStates], h[kRows][kStates];
 #pragma unroll
-            for (int n = 0; n < kStates; ++n) h[n] = FULL || n0 + n < s.states ? save[(n0 + n) * channels] : 0.0f;
+            for (int k = 0; k < kRows / 4; ++k) B[k] = bc_in ? to_f32(in_B[k]) : 0.0f, C[k] = bc_in ? to_f32(in_C[k]) : 0.0f;
+#pragma unroll
+            for (int n = 0; n < kStates; ++n) h0[n] = n0 + n < s.states ? in_h[n] : 0.0f;
+            const uint64_t starts = in_starts;
             __syncthreads();
-#pragma unroll
-            for (int i = 0; i < kRows; ++i) {
-                const int64_t t = t0 + (i < count ? i : count - 1);
-                float B[kStates], C[kStates];
-                load_uniform<kStates, FULL>(pB + t * s.B_time, n0, s.states, B);
-                load_uniform<kStates, FULL>(pC + t * s.C_time, n0, s.states, C);
-                const float dt = s_dt[i][lane], u = dt * s_x[i][lane];
-                const bool start = starts >> i & 1;
-                float y = 0.0f;
-#pragma unroll
-                for (int n = 0; n < kStates; ++n) {
-                    decay[i][n] = start ? 0.0f : __builtin_amdgcn_exp2f(dt * A2[n]);
-                    p[i][n] = start ? 0.0f : decay[i][n] * h[n];
-                    h[n] = __builtin_fmaf(u, B[n], p[i][n]);
-                    y = __builtin_fmaf(C[n], h[n], y);
-                }
-                s_y[w][i][lane] = y;
-            }
+            if (t0 > begin) read(t0 - kRows);
             float kept = 0.0f;
-#pragma unroll
-            for (int i = kRows - 1; i >= 0; --i) {
-                const int64_t t = t0 + (i < count ? i : count - 1);
-                float B[kStates], C[kStates], v[2 * kStates];
-                load_uniform<kStates, FULL>(pB + t * s.B_time, n0, s.states, B);
-                load_uniform<kStates, FULL>(pC + t * s.C_time, n0, s.states, C);
-                const float dt = s_dt[i][lane], u = dt * s_x[i][lane], dy = s_dy[i][lane];
-                float rb = 0.0f, ra = 0.0f;
-#pragma unroll
-                for (int n = 0; n < kStates; ++n) {
-                    r[n] = __builtin_fmaf(dy, C[n], r[n]);
-                    rb = __builtin_fmaf(r[n], B[n], rb);
-                    const float q = r[n] * p[i][n];
-                    ra = __builtin_fmaf(q, A[n], ra);
-                    dA[n] = __builtin_fmaf(q, dt, dA[n]);
-                    v[n] = r[n] * u;
-                    v[kStates + n] = dy * __builtin_fmaf(u, B[n], p[i][n]);
-                    r[n] *= decay[i][n];
-                }
-                s_rb[w][i][lane] = rb;
-                s_ra[w][i][lane] = ra;
-                const float sum = sum_lanes(v, lane);
-                kept = (lane & 7) == (i & 7) ? sum : kept;
-                if ((i & 7) == 0 && i + (lane & 7) < count) {
-                    const int64_t row = ((group_block * s.batch + b) * s.length + t0 + i + (lane & 7)) * s.groups + c.group;
-                    a.shared[row * (2 * NW * kStates) + shared_column] = kept;
-                }
-            }
+            auto walk = [&](auto with_starts) {
+                static_for<kRows>([&](auto row) {
+                    constexpr int i = row;
+                    if constexpr (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
+                    const float4 v = s_row[i][lane];
+                    const bool start = decltype(with_starts)::value && (starts >> i & 1);
+                    static_for<kStates>([&](auto state) {
+                        constexpr int n = state;
+                        const float before = i == 0 ? h0[n] : h[i == 0 ? 0 : i - 1][n];
+                        const float e = __builtin_amdgcn_exp2f(v.x * A2[n]);
+                        decay[i][n] = start ? 0.0f : e;
+                        h[i][n] = __builtin_fmaf(decay[i][n], start ? 0.0f : before, v.y * from_lane<4 * (i & 3) + n>(B[i >> 2]));
+                    });
+                    if (pz) {
+                        float y = 0.0f;
+                        dot_four<4 * (i & 3)>(y, C[i >> 2], h[i]);
+                        s_y[w][i][lane] = y;
+                    }
+                });
+                uint64_t starts_again = starts;   // (kept apart: the compiler would hold what the two walks share in registers)
+                asm volatile("" : "+s"(starts_again) : : "memory");
+                static_for<kRows>([&](auto row) {
+                    constexpr int i = kRows - 1 - row;
+                    if constexpr (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
+                    const float4 u = s_row[i][lane];
+                    const bool start = decltype(with_starts)::value && (starts_again >> i & 1);
+                    float v[2 * kStates], rb = 0.0f, ra = 0.0f;
+                    add_four<4 * (i & 3)>(r, C[i >> 2], u.z);
+                    dot_four<4 * (i & 3)>(rb, B[i >> 2], r);
+                    static_for<kStates>([&](auto state) {
+                        constexpr int n = state;
+                        v[n] = r[n] * u.y;
+                        v[kStates + n] = u.z * h[i][n];
+                        r[n] = start ? 0.0f : r[n] * decay[i][n];
+                        const float q = r[n] * (start ? 0.0f : i == 0 ? h0[n] : h[i == 0 ? 0 : i - 1][n]);
+                        ra = __builtin_fmaf(q, A[n], ra);
+                        dA[n] = __builtin_fmaf(q, u.x, dA[n]);
+                    });
+                    s_sum[w][i][lane] = make_float2(rb, ra);
+                    const float sum = sum_lanes(v, lane);
+                    kept = (lane & 7) == (i & 7) ? sum : kept;
+                    if constexpr ((i & 7) == 0) {
+                        if (i + (lane & 7) < count) {
+                            const int64_t at = ((group_block * s.batch + b) * s.length + t0 + i + (lane & 7)) * s.groups + c.group;
+                            a.shared[at * (2 * NW * kStates) + shared_column] = kept;
+                        }
+                    }
+                });
+            };
+            if (starts)
+                walk(std::true_type{});
+            else
+                walk(std::false_type{});
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int i = e * NW + w;
                 if (i < count && c.active) {
-                    const int64_t t = t0 + i;
+                    const uint32_t t = static_cast<uint32_t>(t0 + i);
                     float rb = 0.0f, ra = 0.0f, y = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < NW; ++k) rb += s_rb[k][i][lane], ra += s_ra[k][i][lane], y += s_y[k][i][lane];
-                    const float dt = s_dt[i][lane], x = s_x[i][lane], dy = s_dy[i][lane];
-                    const float draw = __builtin_fmaf(x, rb, ra) * slope[e];
-                    gx[t * s.grad_x_time] = from_f32<T>(__builtin_fmaf(dt, rb, skip * dy));
-                    gd[t * s.grad_delta_time] = from_f32<T>(draw);
-                    if (gz) gz[t * s.grad_gate_time] = from_f32<T>(dgate[e] * __builtin_fmaf(skip, x, y));
-                    dD = __builtin_fmaf(dy, x, dD);
+                    for (int k = 0; k < NW; ++k) {
+                        const float2 v = s_sum[k][i][lane];
+                        rb += v.x, ra += v.y;
+                        if (pz) y += s_y[k][i][lane];
+                    }
+                    const float4 v = s_row[i][lane];
+                    const float draw = __builtin_fmaf(v.w, rb, ra) * slope[e];
+                    (gx + row_offset(t, s.grad_x_time))[c.d] = from_f32<T>(__builtin_fmaf(v.x, rb, skip * v.z));
+                    (gd + row_offset(t, s.grad_delta_time))[c.d] = from_f32<T>(draw);
+                    if (gz) (gz + row_offset(t, s.grad_gate_time))[c.d] = from_f32<T>(dgate[e] * __builtin_fmaf(skip, v.w, y));
+                    dD = __builtin_fmaf(v.z, v.w, dD);
                     dbias += draw;
                 }
             }
             __syncthreads();
         }
-        if (s.grad_state && c.active) {
+        if (part == 0 && s.grad_state && c.active) {
 #pragma unroll
             for (int n = 0; n < kStates; ++n)
-                if (FULL || n0 + n < s.states) s.grad_state[(b * s.states + n0 + n) * channels + c.d] = r[n];
+                if (n0 + n < s.states) s.grad_state[b * s.states * channels + state_at[n]] = r[n];
         }
     }
-    s_dt[w][lane] = dD;
-    s_x[w][lane] = dbias;
+    s_sum[0][w][lane] = make_float2(dD, dbias);
     __syncthreads();
     if (!c.active) return;
-    float* sums = a.sums + slot * (s.states + 2) * channels + c.d;
+    float* sums = a.sums + slot * (s.states + 2) * channels;
 #pragma unroll
     for (int n = 0; n < kStates; ++n)
-        if (FULL || n0 + n < s.states) sums[(n0 + n) * channels] = dA[n];
+        if (n0 + n < s.states) sums[state_at[n]] = dA[n];
     if (w == 0) {
-        for (int k = 1; k < NW; ++k) dD += s_dt[k][lane], dbias += s_x[k][lane];
-        sums[s.states * channels] = dD;
-        sums[(s.states + 1) * channels] = dbias;
+        for (int k = 1; k < NW; ++k) dD += s_sum[0][k][lane].x, dbias += s_sum[0][k][lane].y;
+        sums[s.states * channels + c.d] = dD;
+        sums[(s.states + 1) * channels + c.d] = dbias;
     }
 }
 
@@ -232,22 +282,19 @@ int waves_for(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <=
 
 ScanArgs backward_args(const ilx_state_space& s, int64_t* floats) {
     ScanArgs a = scan_args(s);
-    const int64_t most = 1024 / a.blocks > 0 ? 1024 / a.blocks : 1;
-    a.slots = s.batch < most ? s.batch : most;
+    const int64_t part_floats = divide_scan(a, s.workspace);
+    const int64_t most = 2048 / a.blocks > 0 ? 2048 / a.blocks : 1, items = s.batch * a.parts;
+    a.slots = items < most ? items : most;
     const int64_t sums = a.slots * (s.states + 2) * s.channels;
     const int64_t shared = a.group_blocks * s.batch * s.length * s.groups * 2 * waves_for(s.states) * kStates;
-    a.sums = s.workspace;
-    a.shared = s.workspace + sums;
-    *floats = sums + shared;
+    a.sums = s.workspace + part_floats;
+    a.shared = a.sums + sums;
+    *floats = part_floats + sums + shared;
     return a;
 }
 
 template <typename T, typename TB, int NW> void backward_launch(const ScanArgs& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(a.slots * a.blocks)), threads(64 * NW);
-    if (a.s.states == NW * kStates)
-        ILX_LAUNCH((scan_backward_kernel<T, TB, NW, true>), grid, threads, 0, s, a);
-    else
-        ILX_LAUNCH((scan_backward_kernel<T, TB, NW, false>), grid, threads, 0, s, a);
+    ILX_LAUNCH((scan_backward_kernel<T, TB, NW>), dim3(static_cast<unsigned>(a.slots * a.blocks)), dim3(64 * NW), 0, s, a);
 }
 
 template <typename T, typename TB> void backward_states(const ScanArgs& a, hipStream_t s) {
@@ -268,8 +315,12 @@ extern "C" int ilx_state_space_workspace(const ilx_state_space* scan, int backwa
     ILX_REQUIRE(scan && floats, ILX_EINVAL, "ilx_state_space_workspace: NULL argument");
     const int rc = scan_check(*scan, "ilx_state_space_workspace");
     if (rc != ILX_OK) return rc;
-    *floats = 0;
-    if (backward) backward_args(*scan, floats);
+    if (backward) {
+        backward_args(*scan, floats);
+    } else {
+        ScanArgs a = scan_args(*scan);
+        *floats = divide_scan(a, nullptr);
+    }
     return ILX_OK;
 }
 
@@ -286,10 +337,11 @@ extern "C" int ilx_state_space_backward(const ilx_state_space* scan, void* strea
     const ScanArgs a = backward_args(s, &needed);
     ILX_REQUIRE(s.workspace_floats >= needed && (s.workspace || needed == 0), ILX_EINVAL,
                 "ilx_state_space_backward: workspace of %lld floats, %lld needed", (long long)s.workspace_floats, (long long)needed);
-    ILX_REQUIRE(a.slots * a.blocks <= INT32_MAX && s.batch * s.length * s.groups * s.states / 256 < INT32_MAX, ILX_ESHAPE,
+    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX && s.batch * s.length * s.groups * s.states / 256 < INT32_MAX, ILX_ESHAPE,
                 "ilx_state_space_backward: shape too large for one launch");
     hipStream_t st = as_stream(stream);
     if (s.batch > 0) {
+        if (a.parts > 1) launch_part_states(a, true, st);
         const bool wide = s.bc_dtype == ILX_F32;
         switch (s.dtype) {
             case ILX_F32: backward_states<float, float>(a, st); break;

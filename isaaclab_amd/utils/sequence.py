@@ -101,7 +101,7 @@ def _p(t: torch.Tensor | None):
 def _copy(t: torch.Tensor, name: str, **how) -> torch.Tensor:
     """A dense copy (``how``: in another type).  A recorded call would go on reading the values of the recording."""
     if _abi.recording():
-        raise _abi.IlxError(f"{name} would be copied before the call, which a command list does not record: pass it dense, and 16-bit B and C with an even number of states")
+        raise _abi.IlxError(f"{name} would be copied before the call, which a command list does not record: pass it dense, and B and C in one type")
     return t.to(**how).contiguous()
 
 
@@ -313,15 +313,8 @@ def _shared(t: torch.Tensor, name: str, lead: tuple, like: torch.Tensor) -> torc
     return t if (n == 1 or t.stride(-1) == 1) and (g == 1 or t.stride(-2) == n) else _copy(t, name)
 
 
-def _readable(t: torch.Tensor) -> torch.Tensor:
-    """16-bit rows are read in pairs: an odd number of states, odd strides or an odd address go through a float32 copy."""
-    if t.dtype == torch.float32 or (t.shape[-1] % 2 == 0 and all(s % 2 == 0 for s in t.stride()[:-2]) and t.data_ptr() % 4 == 0):
-        return t
-    return _copy(t, "B or C", dtype=torch.float32)
-
-
 def _pair(B: torch.Tensor, C: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
-    B, C = _readable(B), _readable(C)
+    """In one type: in float32 where one is."""
     if B.dtype != C.dtype:
         B, C = (t if t.dtype == torch.float32 else _copy(t, "B or C", dtype=torch.float32) for t in (B, C))
     return B, C

@@ -94,9 +94,8 @@ def test_state_space_refusals():
     fails(S._scan_forward(scan(groups=0), None), EINVAL, "0 groups")
     fails(S._scan_forward(scan(dtype=7), None), EINVAL, "unknown type 7")
     fails(S._scan_forward(scan(dtype=1, bc_dtype=2), None), EINVAL, "B and C of type 2")
-    fails(S._scan_forward(scan(dtype=1, bc_dtype=1, states=3), None), ESHAPE, "pairs")
-    fails(S._scan_forward(scan(dtype=1, bc_dtype=1, B=FAKE + 2), None), ESHAPE, "pairs")
-    fails(S._scan_forward(scan(dtype=1, bc_dtype=1, C_time=5), None), ESHAPE, "pairs")
+    fails(S._scan_forward(scan(x_time=1 << 32), None), ESHAPE, "time stride")
+    fails(S._scan_forward(scan(length=2000, channels=64), None), EINVAL, "workspace")
     fails(S._scan_forward(scan(state=FAKE, last=FAKE), None), EINVAL, "same buffer")
     assert S._scan_forward(scan(batch=0, x=None), None) == 0
     grads = dict(grad_out=FAKE, grad_x=FAKE, grad_delta=FAKE, grad_A=FAKE, grad_B=FAKE, grad_C=FAKE, saved=FAKE)
