@@ -32,7 +32,7 @@ extern "C" {
 
 #define ILX_CONV_MAX_WIDTH 8
 #define ILX_SCAN_MAX_STATES 32
-#define ILX_SCAN_BLOCK 16 /* rows between two saved states of a forward pass that a backward pass follows */
+#define ILX_SCAN_BLOCK 8 /* rows between two saved states of a forward pass that a backward pass follows */
 
 /* ---- short causal convolution ------------------------------------------------------------------
  * p[b,t,d] = bias[d] + sum_j weight[d, width-1-j] * x[b,t-j,d],  out = p or p * sigmoid(p).
@@ -108,16 +108,14 @@ typedef struct ilx_state_space {
     int32_t dtype;    /* of x, delta, gate, out and their gradients */
     int32_t bc_dtype; /* of B and C: dtype or ILX_F32 */
     int32_t softplus;
-    /* backward only; the gradient of every operand but B and C has the strides named here, those of B and C are dense */
+    /* backward only; the gradients of x, delta and gate have one pair of strides, those of B and C are dense */
     const void* grad_out;
     int64_t grad_out_batch, grad_out_time;
     const float* grad_last; /* may be NULL */
     void* grad_x;
-    int64_t grad_x_batch, grad_x_time;
     void* grad_delta;
-    int64_t grad_delta_batch, grad_delta_time;
     void* grad_gate; /* NULL exactly if gate is */
-    int64_t grad_gate_batch, grad_gate_time;
+    int64_t grad_batch, grad_time;
     float* grad_A;          /* (channels, states) */
     void* grad_B;           /* (batch, length, groups, states) */
     void* grad_C;

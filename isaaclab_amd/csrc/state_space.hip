@@ -333,8 +333,7 @@ int scan_check(const ilx_state_space& s, const char* name) {
     ILX_REQUIRE(s.batch <= INT32_MAX && s.length <= INT32_MAX - 64 && s.batch * (s.length + 1) < (int64_t{1} << 40), ILX_ESHAPE,
                 "%s: shape (%lld, %lld) too large", name, (long long)s.batch, (long long)s.length);
     if (s.length > 1)
-        for (const int64_t stride : {s.x_time, s.delta_time, s.gate_time, s.B_time, s.C_time, s.out_time, s.grad_out_time, s.grad_x_time, s.grad_delta_time,
-                                     s.grad_gate_time})
+        for (const int64_t stride : {s.x_time, s.delta_time, s.gate_time, s.B_time, s.C_time, s.out_time, s.grad_out_time, s.grad_time})
             ILX_REQUIRE(stride >= 0 && stride <= UINT32_MAX, ILX_ESHAPE, "%s: a time stride of %lld elements", name, (long long)stride);
     return ILX_OK;
 }

@@ -4,7 +4,7 @@
 //   d dt = x sum_n r B + sum_n r p A,   d delta = d dt sigmoid(delta + bias).
 // The states are not kept by the forward pass (they are `states` times the inputs); it saves one in ILX_SCAN_BLOCK rows, and a
 // workgroup recomputes a block's forward from there, then walks it backwards.  A workgroup has 64 channels, a lane each, and a
-// wave for every four states, so a lane holds a and p of a whole block in registers (2 x 16 x 4); what is summed over the
+// wave for every four states, so a lane holds a and p of a whole block in registers (2 x 8 x 4); what is summed over the
 // states (sum r B, sum r p A, y) meets in LDS once per block, and what is summed over the channels (dB, dC) is added across the
 // lanes by a halving exchange: eight values become one register in 8 + 4 + 2 lanes' worth of instructions, not 8 x 6.
 #include "state_space_dev.h"
@@ -13,6 +13,7 @@ namespace ilx {
 
 constexpr int kRows = ILX_SCAN_BLOCK;
 constexpr int kStates = 4;   // per wave
+constexpr float kLn2 = 0.693147180559945309417f;
 
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
     const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true);
@@ -41,11 +42,18 @@ __device__ __forceinline__ float sum_lanes(const float (&v)[8], int lane) {
     return dpp_add<0xb1>(s); // quad_perm 1,0,3,2
 }
 
+// A block of rows of one part of a sequence.
+struct ScanBlock {
+    int64_t item, b, begin, end, t0;   // begin .. end: the part's rows that exist
+    int count;
+};
+
 template <typename T, typename TB, int NW>
-__global__ void __launch_bounds__(64 * NW, NW < 8 ? 8 / NW : 1) scan_backward_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(64 * NW, 3) scan_backward_kernel(ScanArgs a) {
     constexpr int E = kRows / NW;   // rows a wave prepares and finishes per block
-    __shared__ float4 s_row[kRows][64];           // dt, dt x, dy, x
-    __shared__ float2 s_sum[NW][kRows][64];       // sum r B and sum r p A over the wave's states
+    __shared__ float2 s_step[2][kRows][64];       // dt and dt x, of this block and the one before
+    __shared__ float s_dy[2][kRows][64];
+    __shared__ float2 s_sum[NW][kRows][64];       // sum r B and sum r p A log2 e over the wave's states
     __shared__ float s_y[NW][kRows][64];
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = w * kStates;
     const int block = blockIdx.x % a.blocks;
@@ -53,16 +61,13 @@ __global__ void __launch_bounds__(64 * NW, NW < 8 ? 8 / NW : 1) scan_backward_ke
     const ChannelLane c = channel_lane(a, block, lane);
     const int group_block = block - c.group * a.group_blocks;
     const ilx_state_space& s = a.s;
-    const int64_t channels = s.channels;
-    float A[kStates], A2[kStates], dA[kStates];
-    uint32_t state_at[kStates];   // of the wave's states in a (states, channels) array; past the last state: its last
+    const int64_t channels = s.channels, items = s.batch * a.parts;
+    float A2[kStates], dA[kStates];   // A2 = A log2 e
 #pragma unroll
     for (int n = 0; n < kStates; ++n) {
         const bool in = n0 + n < s.states;
-        A[n] = in ? s.A[static_cast<int64_t>(c.d) * s.states + n0 + n] : 0.0f;
-        A2[n] = A[n] * kLog2e;
+        A2[n] = in ? s.A[static_cast<int64_t>(c.d) * s.states + n0 + n] * kLog2e : 0.0f;
         dA[n] = 0.0f;
-        state_at[n] = static_cast<uint32_t>((in ? n0 + n : s.states - 1) * s.channels + c.d);
     }
     const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f, skip = s.D ? s.D[c.d] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
@@ -72,95 +77,114 @@ __global__ void __launch_bounds__(64 * NW, NW < 8 ? 8 / NW : 1) scan_backward_ke
     const int bc_row = lane >> 2 & 3, bc_state = n0 + (lane & 3);
     const bool bc_in = bc_state < s.states;
     const int bc_at = bc_in ? bc_state : s.states - 1;
-
     const uint32_t parts = static_cast<uint32_t>(a.parts);
-    for (int64_t item = slot; item < s.batch * a.parts; item += a.slots) {
-        const int64_t b = static_cast<uint32_t>(item) / parts, part = static_cast<uint32_t>(item) % parts;
-        const int64_t len = scan_length(s, b), begin = part * a.part_rows;
-        const int64_t limit = begin + a.part_rows < s.length ? begin + a.part_rows : s.length, end = limit < len ? limit : len;
-        const T* px = static_cast<const T*>(s.x) + b * s.x_batch;
-        const T* pd = static_cast<const T*>(s.delta) + b * s.delta_batch;
-        const T* pz = s.gate ? static_cast<const T*>(s.gate) + b * s.gate_batch : nullptr;
-        const T* pg = static_cast<const T*>(s.grad_out) + b * s.grad_out_batch;
-        const TB* pB = static_cast<const TB*>(s.B) + b * s.B_batch + c.group * s.states;
-        const TB* pC = static_cast<const TB*>(s.C) + b * s.C_batch + c.group * s.states;
-        T* gx = static_cast<T*>(s.grad_x) + b * s.grad_x_batch;
-        T* gd = static_cast<T*>(s.grad_delta) + b * s.grad_delta_batch;
-        T* gz = s.gate ? static_cast<T*>(s.grad_gate) + b * s.grad_gate_batch : nullptr;
-        const float* enters = a.parts > 1 ? a.part_state + item * s.states * channels : s.grad_last ? s.grad_last + b * s.states * channels : nullptr;
-        float r[kStates];
+
+    // the last block of an item, with count 0 if the item has no rows
+    auto item_end = [&](int64_t item) {
+        ScanBlock k;
+        k.item = item, k.b = static_cast<uint32_t>(item) / parts, k.begin = static_cast<uint32_t>(item) % parts * a.part_rows;
+        const int64_t len = scan_length(s, k.b);
+        k.end = k.begin + a.part_rows < len ? k.begin + a.part_rows : len;
+        k.t0 = k.begin < k.end ? k.begin + (k.end - k.begin - 1) / kRows * kRows : k.begin;
+        k.count = k.begin < k.end ? static_cast<int>(k.end - k.t0) : 0;
+        return k;
+    };
+    // a block's inputs, read while the block ahead of it in this order is worked on
+    T in_d[E], in_x[E], in_g[E], in_z[E];
+    TB in_B[kRows / 4], in_C[kRows / 4];
+    float in_h[kStates];
+    uint64_t in_starts = 0;
+    auto read = [&](const ScanBlock& k) {
+        const T* px = static_cast<const T*>(s.x) + k.b * s.x_batch;
+        const T* pd = static_cast<const T*>(s.delta) + k.b * s.delta_batch;
+        const T* pz = static_cast<const T*>(s.gate) + k.b * s.gate_batch;
+        const T* pg = static_cast<const T*>(s.grad_out) + k.b * s.grad_out_batch;
+        const TB* pB = static_cast<const TB*>(s.B) + k.b * s.B_batch + c.group * s.states;
+        const TB* pC = static_cast<const TB*>(s.C) + k.b * s.C_batch + c.group * s.states;
 #pragma unroll
-        for (int n = 0; n < kStates; ++n) r[n] = enters && c.active && n0 + n < s.states ? enters[state_at[n]] : 0.0f;
-        for (int64_t t = (begin > len ? begin : len) + w; t < limit; t += NW) {
-            if (!c.active) break;
-            (gx + t * s.grad_x_time)[c.d] = from_f32<T>(0.0f);
-            (gd + t * s.grad_delta_time)[c.d] = from_f32<T>(0.0f);
-            if (gz) (gz + t * s.grad_gate_time)[c.d] = from_f32<T>(0.0f);
+        for (int e = 0; e < E; ++e) {
+            const int i = e * NW + w;
+            const uint32_t t = static_cast<uint32_t>(k.t0 + (i < k.count ? i : k.count - 1));
+            in_d[e] = (pd + row_offset(t, s.delta_time))[c.d];
+            in_x[e] = (px + row_offset(t, s.x_time))[c.d];
+            in_g[e] = (pg + row_offset(t, s.grad_out_time))[c.d];
+            if (s.gate) in_z[e] = (pz + row_offset(t, s.gate_time))[c.d];
         }
-        // the inputs of a block, read while the block behind it is worked on
-        T in_d[E], in_x[E], in_g[E], in_z[E];
-        TB in_B[kRows / 4], in_C[kRows / 4];
-        float in_h[kStates];
-        uint64_t in_starts = 0;
-        auto read = [&](int64_t t0) {
-            const int count = end - t0 < kRows ? static_cast<int>(end - t0) : kRows;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = e * NW + w;
-                const uint32_t t = static_cast<uint32_t>(t0 + (i < count ? i : count - 1));
-                in_d[e] = (pd + row_offset(t, s.delta_time))[c.d];
-                in_x[e] = (px + row_offset(t, s.x_time))[c.d];
-                in_g[e] = (pg + row_offset(t, s.grad_out_time))[c.d];
-                if (pz) in_z[e] = (pz + row_offset(t, s.gate_time))[c.d];
+        for (int j = 0; j < kRows / 4; ++j) {
+            const int i = 4 * j + bc_row;
+            const uint32_t t = static_cast<uint32_t>(k.t0 + (i < k.count ? i : k.count - 1));
+            in_B[j] = pB[row_offset(t, s.B_time) + bc_at];
+            in_C[j] = pC[row_offset(t, s.C_time) + bc_at];
+        }
+        const float* save = s.saved + (k.b * a.saved_blocks + k.t0 / kRows) * s.states * channels;
+#pragma unroll
+        for (int n = 0; n < kStates; ++n) in_h[n] = (save + (n0 + n < s.states ? n0 + n : s.states - 1) * channels)[c.d];
+        in_starts = start_bits(s, k.b, k.t0, k.count, lane);
+    };
+
+    ScanBlock k = item_end(slot);
+    if (k.count > 0) read(k);
+    float r[kStates];
+    bool fresh = true;
+    int buffer = 0;
+    while (k.item < items) {
+        if (fresh) {   // the item's last block: what enters the part from behind, and zeros for the rows that do not exist
+            const float* enters = a.parts > 1 ? a.part_state + k.item * s.states * channels : s.grad_last ? s.grad_last + k.b * s.states * channels : nullptr;
+#pragma unroll
+            for (int n = 0; n < kStates; ++n) r[n] = enters && c.active && n0 + n < s.states ? (enters + (n0 + n) * channels)[c.d] : 0.0f;
+            const int64_t limit = k.begin + a.part_rows < s.length ? k.begin + a.part_rows : s.length;
+            for (int64_t t = (k.end > k.begin ? k.end : k.begin) + w; t < limit; t += NW) {
+                const int64_t at = k.b * s.grad_batch + t * s.grad_time + c.d;
+                if (!c.active) break;
+                static_cast<T*>(s.grad_x)[at] = from_f32<T>(0.0f);
+                static_cast<T*>(s.grad_delta)[at] = from_f32<T>(0.0f);
+                if (s.gate) static_cast<T*>(s.grad_gate)[at] = from_f32<T>(0.0f);
             }
-#pragma unroll
-            for (int k = 0; k < kRows / 4; ++k) {
-                const int i = 4 * k + bc_row;
-                const uint32_t t = static_cast<uint32_t>(t0 + (i < count ? i : count - 1));
-                in_B[k] = pB[row_offset(t, s.B_time) + bc_at];
-                in_C[k] = pC[row_offset(t, s.C_time) + bc_at];
-            }
-            const float* save = s.saved + (b * a.saved_blocks + t0 / kRows) * s.states * channels;
-#pragma unroll
-            for (int n = 0; n < kStates; ++n) in_h[n] = save[state_at[n]];
-            in_starts = start_bits(s, b, t0, count, lane);
-        };
-        const int64_t last_block = begin < end ? begin + (end - begin - 1) / kRows * kRows : begin - kRows;
-        if (last_block >= begin) read(last_block);
-        for (int64_t t0 = last_block; t0 >= begin; t0 -= kRows) {
-            const int count = end - t0 < kRows ? static_cast<int>(end - t0) : kRows;
+        }
+        ScanBlock next = k;
+        if (k.t0 > k.begin) {
+            next.t0 = k.t0 - kRows, next.count = kRows;
+        } else if (k.item + a.slots < items) {
+            next = item_end(k.item + a.slots);
+        } else {
+            next.item = items, next.count = 0;
+        }
+        if (k.count > 0) {
             // rows past the end act as rows that leave the state alone: dt = x = dy = 0
-            float slope[E], dgate[E];
+            float slope[E], dgate[E], x[E];
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int i = e * NW + w;
-                const bool in = i < count && c.active;
-                const float raw = to_f32(in_d[e]) + bias, x = in ? to_f32(in_x[e]) : 0.0f, g = to_f32(in_g[e]);
+                const bool in = i < k.count && c.active;
+                const float raw = to_f32(in_d[e]) + bias, g = to_f32(in_g[e]);
+                x[e] = in ? to_f32(in_x[e]) : 0.0f;
                 float dy = g;
                 dgate[e] = 0.0f;
-                if (pz) {
+                if (s.gate) {
                     const float z = to_f32(in_z[e]), sig = sigmoid_fast(z);
                     dy = g * z * sig;
                     dgate[e] = g * sig * __builtin_fmaf(z, 1.0f - sig, 1.0f);
                 }
                 slope[e] = s.softplus ? sigmoid_fast(raw) : 1.0f;
                 const float dt = in ? (s.softplus ? softplus_f(raw) : raw) : 0.0f;
-                s_row[i][lane] = make_float4(dt, dt * x, in ? dy : 0.0f, x);
+                s_step[buffer][i][lane] = make_float2(dt, dt * x[e]);
+                s_dy[buffer][i][lane] = in ? dy : 0.0f;
             }
             float B[kRows / 4], C[kRows / 4], h0[kStates], decay[kRows][kStates], h[kRows][kStates];
 #pragma unroll
-            for (int k = 0; k < kRows / 4; ++k) B[k] = bc_in ? to_f32(in_B[k]) : 0.0f, C[k] = bc_in ? to_f32(in_C[k]) : 0.0f;
+            for (int j = 0; j < kRows / 4; ++j) B[j] = bc_in ? to_f32(in_B[j]) : 0.0f, C[j] = bc_in ? to_f32(in_C[j]) : 0.0f;
 #pragma unroll
             for (int n = 0; n < kStates; ++n) h0[n] = n0 + n < s.states ? in_h[n] : 0.0f;
             const uint64_t starts = in_starts;
             __syncthreads();
-            if (t0 > begin) read(t0 - kRows);
+            if (next.count > 0) read(next);
             float kept = 0.0f;
             auto walk = [&](auto with_starts) {
                 static_for<kRows>([&](auto row) {
                     constexpr int i = row;
-                    if constexpr (i % 4 == 0) __builtin_amdgcn_sched_barrier(0);
-                    const float4 v = s_row[i][lane];
+                    __builtin_amdgcn_sched_barrier(0);
+                    const float2 v = s_step[buffer][i][lane];
                     const bool start = decltype(with_starts)::value && (starts >> i & 1);
                     static_for<kStates>([&](auto state) {
                         constexpr int n = state;
@@ -169,85 +193,86 @@ __global__ void __launch_bounds__(64 * NW, NW < 8 ? 8 / NW : 1) scan_backward_ke
                         decay[i][n] = start ? 0.0f : e;
                         h[i][n] = __builtin_fmaf(decay[i][n], start ? 0.0f : before, v.y * from_lane<4 * (i & 3) + n>(B[i >> 2]));
                     });
-                    if (pz) {
-                        float y = 0.0f;
-                        dot_four<4 * (i & 3)>(y, C[i >> 2], h[i]);
-                        s_y[w][i][lane] = y;
-                    }
+                    float y = 0.0f;
+                    dot_four<4 * (i & 3)>(y, C[i >> 2], h[i]);
+                    s_y[w][i][lane] = y;
                 });
                 uint64_t starts_again = starts;   // (kept apart: the compiler would hold what the two walks share in registers)
                 asm volatile("" : "+s"(starts_again) : : "memory");
                 static_for<kRows>([&](auto row) {
                     constexpr int i = kRows - 1 - row;
-                    if constexpr (i % 4 == 3) __builtin_amdgcn_sched_barrier(0);
-                    const float4 u = s_row[i][lane];
+                    __builtin_amdgcn_sched_barrier(0);
+                    const float2 u = s_step[buffer][i][lane];
+                    const float dy = s_dy[buffer][i][lane];
                     const bool start = decltype(with_starts)::value && (starts_again >> i & 1);
                     float v[2 * kStates], rb = 0.0f, ra = 0.0f;
-                    add_four<4 * (i & 3)>(r, C[i >> 2], u.z);
+                    add_four<4 * (i & 3)>(r, C[i >> 2], dy);
                     dot_four<4 * (i & 3)>(rb, B[i >> 2], r);
                     static_for<kStates>([&](auto state) {
                         constexpr int n = state;
                         v[n] = r[n] * u.y;
-                        v[kStates + n] = u.z * h[i][n];
+                        v[kStates + n] = dy * h[i][n];
                         r[n] = start ? 0.0f : r[n] * decay[i][n];
                         const float q = r[n] * (start ? 0.0f : i == 0 ? h0[n] : h[i == 0 ? 0 : i - 1][n]);
-                        ra = __builtin_fmaf(q, A[n], ra);
+                        ra = __builtin_fmaf(q, A2[n], ra);
                         dA[n] = __builtin_fmaf(q, u.x, dA[n]);
                     });
                     s_sum[w][i][lane] = make_float2(rb, ra);
                     const float sum = sum_lanes(v, lane);
-                    kept = (lane & 7) == (i & 7) ? sum : kept;
-                    if constexpr ((i & 7) == 0) {
-                        if (i + (lane & 7) < count) {
-                            const int64_t at = ((group_block * s.batch + b) * s.length + t0 + i + (lane & 7)) * s.groups + c.group;
-                            a.shared[at * (2 * NW * kStates) + shared_column] = kept;
-                        }
-                    }
+                    kept = (lane & 7) == i ? sum : kept;
                 });
             };
             if (starts)
                 walk(std::true_type{});
             else
                 walk(std::false_type{});
+            if ((lane & 7) < k.count) {
+                const int64_t at = ((group_block * s.batch + k.b) * s.length + k.t0 + (lane & 7)) * s.groups + c.group;
+                a.shared[at * (2 * NW * kStates) + shared_column] = kept;
+            }
             __syncthreads();
 #pragma unroll
             for (int e = 0; e < E; ++e) {
                 const int i = e * NW + w;
-                if (i < count && c.active) {
-                    const uint32_t t = static_cast<uint32_t>(t0 + i);
+                if (i < k.count && c.active) {
                     float rb = 0.0f, ra = 0.0f, y = 0.0f;
 #pragma unroll
-                    for (int k = 0; k < NW; ++k) {
-                        const float2 v = s_sum[k][i][lane];
+                    for (int j = 0; j < NW; ++j) {
+                        const float2 v = s_sum[j][i][lane];
                         rb += v.x, ra += v.y;
-                        if (pz) y += s_y[k][i][lane];
+                        y += s_y[j][i][lane];
                     }
-                    const float4 v = s_row[i][lane];
-                    const float draw = __builtin_fmaf(v.w, rb, ra) * slope[e];
-                    (gx + row_offset(t, s.grad_x_time))[c.d] = from_f32<T>(__builtin_fmaf(v.x, rb, skip * v.z));
-                    (gd + row_offset(t, s.grad_delta_time))[c.d] = from_f32<T>(draw);
-                    if (gz) (gz + row_offset(t, s.grad_gate_time))[c.d] = from_f32<T>(dgate[e] * __builtin_fmaf(skip, v.w, y));
-                    dD = __builtin_fmaf(v.z, v.w, dD);
+                    const float dt = s_step[buffer][i][lane].x, dy = s_dy[buffer][i][lane], draw = __builtin_fmaf(x[e], rb, ra * kLn2) * slope[e];
+                    const int64_t at = k.b * s.grad_batch + row_offset(static_cast<uint32_t>(k.t0 + i), s.grad_time);
+                    (static_cast<T*>(s.grad_x) + at)[c.d] = from_f32<T>(__builtin_fmaf(dt, rb, skip * dy));
+                    (static_cast<T*>(s.grad_delta) + at)[c.d] = from_f32<T>(draw);
+                    if (s.gate) (static_cast<T*>(s.grad_gate) + at)[c.d] = from_f32<T>(dgate[e] * __builtin_fmaf(skip, x[e], y));
+                    dD = __builtin_fmaf(dy, x[e], dD);
                     dbias += draw;
                 }
             }
-            __syncthreads();
+            buffer ^= 1;   // (the next block's rows go where nobody still reads; its sums are written behind a barrier)
+        } else if (next.count > 0) {
+            read(next);
         }
-        if (part == 0 && s.grad_state && c.active) {
+        fresh = next.item != k.item;
+        if (fresh && k.begin == 0 && s.grad_state && c.active) {
 #pragma unroll
             for (int n = 0; n < kStates; ++n)
-                if (n0 + n < s.states) s.grad_state[b * s.states * channels + state_at[n]] = r[n];
+                if (n0 + n < s.states) (s.grad_state + (k.b * s.states + n0 + n) * channels)[c.d] = r[n];
         }
+        k = next;
     }
+    __syncthreads();
     s_sum[0][w][lane] = make_float2(dD, dbias);
     __syncthreads();
     if (!c.active) return;
     float* sums = a.sums + slot * (s.states + 2) * channels;
 #pragma unroll
     for (int n = 0; n < kStates; ++n)
-        if (n0 + n < s.states) sums[state_at[n]] = dA[n];
+        if (n0 + n < s.states) sums[(n0 + n) * channels + c.d] = dA[n];
     if (w == 0) {
-        for (int k = 1; k < NW; ++k) dD += s_sum[0][k][lane].x, dbias += s_sum[0][k][lane].y;
+        for (int j = 1; j < NW; ++j) dD += s_sum[0][j][lane].x, dbias += s_sum[0][j][lane].y;
         sums[s.states * channels + c.d] = dD;
         sums[(s.states + 1) * channels + c.d] = dbias;
     }

@@ -36,7 +36,7 @@ from .. import _abi
 
 MAX_WIDTH = 8
 MAX_STATES = 32
-_BLOCK = 16   # ILX_SCAN_BLOCK
+_BLOCK = 8   # ILX_SCAN_BLOCK
 _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
@@ -66,9 +66,7 @@ class StateSpaceDesc(ctypes.Structure):
         ("last", c_void_p), ("saved", c_void_p), ("batch", c_int64), ("length", c_int64), ("channels", c_int32), ("states", c_int32),
         ("groups", c_int32), ("dtype", c_int32), ("bc_dtype", c_int32), ("softplus", c_int32),
         ("grad_out", c_void_p), ("grad_out_batch", c_int64), ("grad_out_time", c_int64), ("grad_last", c_void_p),
-        ("grad_x", c_void_p), ("grad_x_batch", c_int64), ("grad_x_time", c_int64),
-        ("grad_delta", c_void_p), ("grad_delta_batch", c_int64), ("grad_delta_time", c_int64),
-        ("grad_gate", c_void_p), ("grad_gate_batch", c_int64), ("grad_gate_time", c_int64),
+        ("grad_x", c_void_p), ("grad_delta", c_void_p), ("grad_gate", c_void_p), ("grad_batch", c_int64), ("grad_time", c_int64),
         ("grad_A", c_void_p), ("grad_B", c_void_p), ("grad_C", c_void_p), ("grad_D", c_void_p), ("grad_delta_bias", c_void_p),
         ("grad_state", c_void_p), ("workspace", c_void_p), ("workspace_floats", c_int64),
     ]
@@ -375,16 +373,14 @@ class _StateSpaceScan(torch.autograd.Function):
         grad_last = None if grad_last is None else grad_last.contiguous()
         rB, rC = _pair(B, C)
         d = _scan_desc(x, delta, A, rB, rC, D, gate, delta_bias, None, starts, lengths, ctx.softplus)
-        gx, gdelta, gA = torch.empty_like(x), torch.empty_like(delta), torch.empty_like(A)
+        gx, gA = torch.empty_like(x), torch.empty_like(A)
+        gdelta, ggate = torch.empty_like(gx), None if gate is None else torch.empty_like(gx)
         gB, gC = torch.empty(rB.shape, dtype=rB.dtype, device=x.device), torch.empty(rC.shape, dtype=rC.dtype, device=x.device)
-        gD, ggate, gbias = (None if t is None else torch.empty_like(t) for t in (D, gate, delta_bias))
+        gD, gbias = (None if t is None else torch.empty_like(t) for t in (D, delta_bias))
         gstate = torch.empty(x.shape[0], A.shape[1], x.shape[2], device=x.device) if ctx.has_state and ctx.needs_input_grad[8] else None
         d.saved = saved.data_ptr()
-        for name, t in (("grad_out", grad_out), ("grad_x", gx), ("grad_delta", gdelta), ("grad_gate", ggate)):
-            if t is not None:
-                setattr(d, name, t.data_ptr())
-                setattr(d, name + "_batch", t.stride(0))
-                setattr(d, name + "_time", t.stride(1))
+        d.grad_out, d.grad_out_batch, d.grad_out_time = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1)
+        d.grad_x, d.grad_delta, d.grad_gate, d.grad_batch, d.grad_time = gx.data_ptr(), gdelta.data_ptr(), _p(ggate), gx.stride(0), gx.stride(1)
         d.grad_last, d.grad_A, d.grad_B, d.grad_C = _p(grad_last), gA.data_ptr(), gB.data_ptr(), gC.data_ptr()
         d.grad_D, d.grad_delta_bias, d.grad_state = _p(gD), _p(gbias), _p(gstate)
         workspace = _scan_scratch(d, 1, x.device)  # noqa: F841
@@ -421,7 +417,7 @@ def state_space_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: t
     ``x``, ``delta``, ``gate`` (batch, length, channels); ``A`` (channels, N), N up to 32; ``B``, ``C`` (batch, length, groups, N)
     or (batch, length, N) shared by all channels, in x's type or float32; ``D``, ``delta_bias`` (channels).  ``state`` (batch,
     N, channels) is the state ahead of the first row (zeros if None); with ``return_state`` the result is ``(out, last)``.
-    Differentiable in every operand but ``starts`` and ``lengths``; between a forward and its backward pass one state in 16
+    Differentiable in every operand but ``starts`` and ``lengths``; between a forward and its backward pass one state in 8
     rows is kept."""
     _check_x(x, 3)
     batch, length, channels = x.shape
