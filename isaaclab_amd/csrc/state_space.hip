@@ -2,152 +2,282 @@
 //   h[n] <- exp(dt A[n]) h[n] + dt B[n] x,   y = sum_n C[n] h[n] + D x,   dt = softplus(delta + bias)
 // per channel, with B and C shared by the channels of a group.
 // A lane owns a channel and all its states, a wave 64 channels: the recurrence needs no exchange between lanes, a row's x,
-// delta, gate and out are one access of 64 neighbours each, and B and C come out of one register a row by broadcast.  Per state
-// and row that leaves a multiply, an exponential (a quarter of the rate), a multiply by B and two multiply-adds.  The next four
-// rows are on their way while four are worked on.
+// delta, gate and out are one access of 64 neighbours each, and B and C enter from lanes (state_space_dev.h).  Per state and row
+// that leaves a multiply, an exponential (a third to a quarter of the rate), a multiply, a quarter of a matrix instruction and a
+// multiply-add.  The next four rows, of this sequence or the wave's next, are on their way while four are worked on.
 // Where that makes too few waves (few sequences, long ones), a sequence is divided into parts: every part runs from a zero state
 // for what it adds to the state, a join passes the states through all parts (a part as a whole multiplies a state by
 // exp(A sum dt)), and every part runs again from the state that enters it.  That costs a second pass of exponentials and buys
 // up to 256 times the waves.
 #include "state_space_dev.h"
+#include "uniform_access.h"
 
 namespace ilx {
 
 constexpr int kScanRows = 4;    // rows whose inputs are in registers together; divides ILX_SCAN_BLOCK
 constexpr int kMostParts = 256;
 
-// One row's inputs as they are in memory.
-template <typename T, typename TB, int W> struct ScanRow {
-    T x, delta, gate;
-    TB B[W], C[W];
+enum { kHasGate = 1, kSoftplus = 2, kHasStarts = 4, kFull = 8 };   // kFull: as many states as the lane has registers
+
+// What stays in scalar registers through a wave's life; all else is read again where an item begins (arguments_again).
+template <typename T, typename TB> struct ScanStreams {
+    Stream<T> x, delta, gate;   // at the rows that are read next
+    Stream<TB> o, c;            // operand of `outer` and of `dot`
+    Stream<uint8_t> starts;
+    int flags;
+    int item, b, begin, end, t0;   // the item that is read, its rows that exist, the next row
+
+    template <bool REVERSE> __device__ __forceinline__ void open(int which, int group) {
+        const ArgsPtr a = arguments_again();
+        const int parts = static_cast<int>(a->parts), rows = static_cast<int>(a->part_rows);
+        item = which, b = item / parts, begin = (item - b * parts) * rows;
+        int len = static_cast<int>(a->s.length);
+        if (a->s.lengths) {
+            const int n = uni(a->s.lengths[b]);
+            len = n < 0 ? 0 : (n < len ? n : len);
+        }
+        end = begin + rows < len ? begin + rows : len;
+        t0 = REVERSE && begin < end ? begin + (end - 1 - begin) / kScanRows * kScanRows : begin;
+        if (REVERSE)
+            x.set(a->s.grad_out, b * a->s.grad_out_batch, t0, a->s.grad_out_time), o.set(a->s.C, b * a->s.C_batch + group * a->s.states, t0, a->s.C_time);
+        else
+            x.set(a->s.x, b * a->s.x_batch, t0, a->s.x_time), o.set(a->s.B, b * a->s.B_batch + group * a->s.states, t0, a->s.B_time);
+        delta.set(a->s.delta, b * a->s.delta_batch, t0, a->s.delta_time);
+        if (a->s.gate)
+            gate.set(a->s.gate, b * a->s.gate_batch, t0, a->s.gate_time);
+        else
+            gate = delta;   // (read and not used)
+        c.set(a->s.C, b * a->s.C_batch + group * a->s.states, t0, a->s.C_time);
+        starts.set(a->s.starts, b * a->s.starts_batch, t0, a->s.starts_time);
+    }
+    __device__ __forceinline__ int count() const { return end - t0 < kScanRows ? end - t0 : kScanRows; }
+    template <bool REVERSE> __device__ __forceinline__ void step() {
+        constexpr int n = REVERSE ? -kScanRows : kScanRows;
+        x.step(n), delta.step(n), gate.step(n), o.step(n), c.step(n), starts.step(n);
+        t0 += n;
+    }
 };
 
-template <typename T, typename TB, int S> struct ScanReader {
-    static constexpr int W = (S + 15) / 16;
-    const T *x, *delta, *gate;
-    const TB *B, *C;
-    int64_t x_time, delta_time, gate_time, B_time, C_time;
-    int d, n[W];
-    bool in[W];
+// The inputs of four rows, read while the four rows ahead of them are worked on.
+template <typename T, typename TB, int W, bool WITH_GATE, bool WITH_DOT> struct ScanRows {
+    T x[kScanRows], delta[kScanRows], gate[kScanRows];
+    TB o[W], c[kScanRows][W];
+    uint32_t starts;
 
-    __device__ __forceinline__ ScanReader(const ScanArgs& a, const ChannelLane& c, int64_t b, int lane, const void* px, int64_t px_batch, int64_t px_time) {
-        const ilx_state_space& s = a.s;
-        x = static_cast<const T*>(px) + b * px_batch, x_time = px_time;
-        delta = static_cast<const T*>(s.delta) + b * s.delta_batch, delta_time = s.delta_time;
-        gate = s.gate ? static_cast<const T*>(s.gate) + b * s.gate_batch : nullptr, gate_time = s.gate_time;
-        B = static_cast<const TB*>(s.B) + b * s.B_batch + c.group * s.states, B_time = s.B_time;
-        C = static_cast<const TB*>(s.C) + b * s.C_batch + c.group * s.states, C_time = s.C_time;
-        d = c.d;
+    // channel: the lane's channel, o_state, c_state: its states of the operands of `outer` and `dot`, all in bytes
+    __device__ __forceinline__ void read(const ScanStreams<T, TB>& k, uint32_t channel, const uint32_t (&o_state)[W], const uint32_t (&c_state)[W], int lane) {
+        const int count = k.count();
+        const auto bx = k.x.buffer(), bd = k.delta.buffer(), bz = k.gate.buffer(), bo = k.o.buffer(), bc = k.c.buffer();
 #pragma unroll
-        for (int k = 0; k < W; ++k) {
-            const int at = 16 * k + (lane & 15);
-            in[k] = at < s.states;
-            n[k] = in[k] ? at : s.states - 1;
+        for (int i = 0; i < kScanRows; ++i) {
+            const uint32_t r = i < count ? i : count - 1;
+            x[i] = lane_load<T>(bx, channel, r * k.x.time);
+            delta[i] = lane_load<T>(bd, channel, r * k.delta.time);
+            if (WITH_GATE) gate[i] = lane_load<T>(bz, channel, r * k.gate.time);
+            if (WITH_DOT) {
+#pragma unroll
+                for (int j = 0; j < W; ++j) c[i][j] = lane_load<TB>(bc, c_state[j], r * k.c.time);
+            }
+        }
+        const int at = lane >> 2 & 3;
+        const uint32_t row = (at < count ? at : count - 1) * k.o.time;
+#pragma unroll
+        for (int j = 0; j < W; ++j) o[j] = lane_load<TB>(bo, row + o_state[j], 0);
+        starts = 0;
+        if (k.flags & kHasStarts) {
+            bool on = false;
+            if (lane < count) on = k.starts.p[lane * k.starts.time] != 0;
+            starts = static_cast<uint32_t>(__ballot(on));
         }
     }
-    template <bool WITH_B, bool WITH_C, bool WITH_GATE> __device__ __forceinline__ void read(ScanRow<T, TB, W>& r, uint32_t t) const {
-        r.x = x[row_offset(t, x_time) + d];
-        r.delta = delta[row_offset(t, delta_time) + d];
-        if (WITH_GATE && gate) r.gate = gate[row_offset(t, gate_time) + d];
-#pragma unroll
-        for (int k = 0; k < W; ++k) {
-            if (WITH_B) r.B[k] = B[row_offset(t, B_time) + n[k]];
-            if (WITH_C) r.C[k] = C[row_offset(t, C_time) + n[k]];
-        }
-    }
-    __device__ __forceinline__ float state_lane(const TB (&v)[W], int k) const { return in[k] ? to_f32(v[k]) : 0.0f; }
 };
 
-// h <- exp(dt A) h + u B  for all states of the lane
-template <int S, int W> __device__ __forceinline__ void advance(float (&h)[S], const float (&A2)[S], const float (&B)[W], float dt, float u) {
-    static_for<S>([&](auto i) {
-        constexpr int n = i;
-        h[n] = __builtin_fmaf(__builtin_amdgcn_exp2f(dt * A2[n]), h[n], u * from_lane<(n & 15)>(B[n >> 4]));
+// A start: a branch of its own, taken rarely, and no selects on the way past it.
+template <int V> __device__ __forceinline__ void forget_if(bool start, f32x4 (&h)[V]) {
+    if (start) {
+        asm volatile("; an episode starts");
+#pragma unroll
+        for (int m = 0; m < V; ++m) h[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
+}
+
+// h <- exp(dt A) h + u B for all states of the lane; B from row ROW of the outer operand
+template <int ROW, int V, int W> __device__ __forceinline__ void advance(f32x4 (&h)[V], const f32x4 (&A2)[V], const float (&B)[W], float dt, float u) {
+    static_for<V>([&](auto i) {
+        constexpr int m = i;
+        f32x4 p;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) p[j] = __builtin_amdgcn_exp2f(dt * A2[m][j]) * h[m][j];
+        h[m] = outer<4 * (m & 3) + ROW>(B[m >> 2], u, p);
     });
 }
 
-template <int S, int W> __device__ __forceinline__ float dot(const float (&C)[W], const float (&h)[S], float y) {
+template <int V, int W> __device__ __forceinline__ float dot(const float (&C)[W], const f32x4 (&h)[V], float y) {
     float y1 = 0.0f;
-    if constexpr (S <= 16)
-        dot_states(y, y1, C[0], h);
-    else {
-        dot_sixteen<0>(y, y1, C[0], h);
-        dot_sixteen<16>(y, y1, C[1], h);
+    static_for<V>([&](auto i) {
+        constexpr int m = i;
+        if constexpr (m & 1)
+            dot_four<4 * (m & 3), m == 1>(y1, C[m >> 2], h[m]);
+        else
+            dot_four<4 * (m & 3), m == 0>(y, C[m >> 2], h[m]);
+    });
+    return V > 1 ? y + y1 : y;
+}
+
+// The lane's row of A times log2 e, zeros past the last state.
+template <int V> __device__ __forceinline__ void load_decays(const ScanArgs& a, int d, f32x4 (&A2)[V]) {
+    const float* A = a.s.A + static_cast<int64_t>(d) * a.s.states;
+    if (a.s.states == 4 * V && a.decays_aligned) {
+#pragma unroll
+        for (int m = 0; m < V; ++m) A2[m] = reinterpret_cast<const f32x4*>(A)[m] * kLog2e;
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4 * V; ++n) A2[n >> 2][n & 3] = n < a.s.states ? A[n] * kLog2e : 0.0f;
     }
-    return y + y1;
+}
+
+// The states of the lane's channel (its byte offset), `channels` apart.
+template <int V> __device__ __forceinline__ void load_state(const float* from, int states, int channels, uint32_t channel, f32x4 (&h)[V]) {
+#pragma unroll
+    for (int m = 0; m < V; ++m) h[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    if (!from) return;
+    const auto row = row_buffer(from);
+    const uint32_t step = static_cast<uint32_t>(channels) * 4;
+    if (states == 4 * V) {
+#pragma unroll
+        for (int n = 0; n < 4 * V; ++n) h[n >> 2][n & 3] = lane_load<float>(row, channel, n * step);
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4 * V; ++n)
+            if (n < states) h[n >> 2][n & 3] = lane_load<float>(row, channel, n * step);
+    }
+}
+template <int V> __device__ __forceinline__ void store_state(float* to, int states, int channels, uint32_t channel, const f32x4 (&h)[V]) {
+    const auto row = row_buffer(to);
+    const uint32_t step = static_cast<uint32_t>(channels) * 4;
+    if (states == 4 * V) {
+#pragma unroll
+        for (int n = 0; n < 4 * V; ++n) lane_store<float>(row, channel, n * step, h[n >> 2][n & 3]);
+    } else {
+#pragma unroll
+        for (int n = 0; n < 4 * V; ++n)
+            if (n < states) lane_store<float>(row, channel, n * step, h[n >> 2][n & 3]);
+    }
+}
+
+// Which states a lane holds of the operands of `outer` and `dot` (clamped to the last), and masks that zero what does not exist.
+template <typename TB, int W> struct SharedStates {
+    uint32_t o[W], c[W], o_mask[W], c_mask[W];   // o, c in bytes
+    __device__ __forceinline__ SharedStates(int lane, int states) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int p = 16 * j + 4 * (lane >> 4) + (lane & 3), q = 16 * j + (lane & 15);
+            o[j] = (p < states ? p : states - 1) * sizeof(TB), c[j] = (q < states ? q : states - 1) * sizeof(TB);
+            o_mask[j] = p < states ? ~0u : 0u, c_mask[j] = q < states ? ~0u : 0u;
+        }
+    }
+};
+
+template <int V> __device__ __forceinline__ int scan_flags(const ilx_state_space& s) {
+    return (s.gate ? kHasGate : 0) | (s.softplus ? kSoftplus : 0) | (s.starts ? kHasStarts : 0) | (s.states == 4 * V ? kFull : 0);
 }
 
 template <typename T, typename TB, int S>
 __global__ void __launch_bounds__(64) scan_forward_kernel(ScanArgs a) {
-    constexpr int W = (S + 15) / 16;
+    constexpr int V = S / 4, W = (S + 15) / 16;
     const int lane = threadIdx.x;
-    const uint32_t item = blockIdx.x / a.blocks, parts = static_cast<uint32_t>(a.parts);
-    const int64_t b = item / parts, part = item % parts;
     const ChannelLane c = channel_lane(a, blockIdx.x % a.blocks, lane);
-    const ilx_state_space& s = a.s;
-    const int64_t len = scan_length(s, b), channels = s.channels, begin = part * a.part_rows;
-    const int64_t limit = begin + a.part_rows < s.length ? begin + a.part_rows : s.length, end = limit < len ? limit : len;
-    float A2[S], h[S];
-    const float* enters = a.parts > 1 ? a.part_state + static_cast<int64_t>(item) * s.states * channels : s.state ? s.state + b * s.states * channels : nullptr;
-#pragma unroll
-    for (int n = 0; n < S; ++n) {
-        const bool in = n < s.states;
-        A2[n] = in ? s.A[static_cast<int64_t>(c.d) * s.states + n] * kLog2e : 0.0f;
-        h[n] = in && enters ? enters[n * channels + c.d] : 0.0f;
-    }
-    const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f, skip = s.D ? s.D[c.d] : 0.0f;
-    const ScanReader<T, TB, S> in(a, c, b, lane, s.x, s.x_batch, s.x_time);
-    T* po = static_cast<T*>(s.out) + b * s.out_batch + c.d;
-    ScanRow<T, TB, W> rows[kScanRows];
-    auto read = [&](int64_t t0) {
-#pragma unroll
-        for (int i = 0; i < kScanRows; ++i)
-            in.template read<true, true, true>(rows[i], static_cast<uint32_t>(t0 + i < end ? t0 + i : end - 1));
-    };
-    if (begin < end) read(begin);
-    for (int64_t t0 = begin; t0 < end; t0 += kScanRows) {
-        const int count = end - t0 < kScanRows ? static_cast<int>(end - t0) : kScanRows;
-        float x[kScanRows], dt[kScanRows], z[kScanRows], B[kScanRows][W], C[kScanRows][W];
-#pragma unroll
-        for (int i = 0; i < kScanRows; ++i) {
-            x[i] = to_f32(rows[i].x);
-            dt[i] = to_f32(rows[i].delta) + bias;
-            if (in.gate) z[i] = to_f32(rows[i].gate);
-#pragma unroll
-            for (int k = 0; k < W; ++k) B[i][k] = in.state_lane(rows[i].B, k), C[i][k] = in.state_lane(rows[i].C, k);
+    const uint32_t channel = c.d * sizeof(T), channel4 = c.d * 4;
+    const SharedStates<TB, W> shared(lane, a.s.states);
+    const int items = static_cast<int>(a.s.batch * a.parts), slots = static_cast<int>(a.slots);
+    f32x4 A2[V], h[V];
+    load_decays<V>(a, c.d, A2);
+    const float bias = a.s.delta_bias ? a.s.delta_bias[c.d] : 0.0f, skip = a.s.D ? a.s.D[c.d] : 0.0f;
+    ScanRows<T, TB, W, true, true> rows;
+    ScanStreams<T, TB> k;
+    k.flags = scan_flags<V>(a.s);
+    k.template open<false>(blockIdx.x / a.blocks, c.group);
+    if (k.begin < k.end) rows.read(k, channel, shared.o, shared.c, lane);
+    float* saved = nullptr;
+    while (k.item < items) {
+        // an item: what enters it, its rows, what leaves it
+        const int item = k.item, b = k.b, begin = k.begin, end = k.end;
+        Stream<T> out;
+        {
+            const ArgsPtr p = arguments_again();
+            const int64_t state = static_cast<int64_t>(p->s.states) * p->s.channels;
+            load_state<V>(p->parts > 1 ? p->part_state + item * state : p->s.state ? p->s.state + b * state : nullptr, p->s.states, p->s.channels, channel4, h);
+            out.set(p->s.out, b * p->s.out_batch, begin, p->s.out_time);
+            saved = p->s.saved ? p->s.saved + (b * p->saved_blocks + begin / ILX_SCAN_BLOCK) * state : nullptr;
         }
-        const uint64_t starts = start_bits(s, b, t0, count, lane);
-        if (t0 + kScanRows < end) read(t0 + kScanRows);
-        if (s.saved && t0 % ILX_SCAN_BLOCK == 0 && c.active) {
-            float* save = s.saved + (b * a.saved_blocks + t0 / ILX_SCAN_BLOCK) * s.states * channels + c.d;
+        for (int t0 = begin; t0 < end; t0 += kScanRows) {
+            const int count = end - t0 < kScanRows ? end - t0 : kScanRows;
+            float x[kScanRows], dt[kScanRows], z[kScanRows], B[W], C[kScanRows][W];
 #pragma unroll
-            for (int n = 0; n < S; ++n)
-                if (n < s.states) save[n * channels] = h[n];
-        }
-        if (s.softplus) {
+            for (int i = 0; i < kScanRows; ++i) {
+                x[i] = to_f32(rows.x[i]);
+                dt[i] = to_f32(rows.delta[i]) + bias;
+                z[i] = to_f32(rows.gate[i]);
 #pragma unroll
-            for (int i = 0; i < kScanRows; ++i) dt[i] = softplus_f(dt[i]);
-        }
+                for (int j = 0; j < W; ++j) C[i][j] = masked(to_f32(rows.c[i][j]), shared.c_mask[j]);
+            }
 #pragma unroll
-        for (int i = 0; i < kScanRows; ++i) {
-            if (i < count) {
-                if (starts >> i & 1) {
+            for (int j = 0; j < W; ++j) B[j] = masked(to_f32(rows.o[j]), shared.o_mask[j]);
+            const uint32_t starts = rows.starts;
+            if (t0 + kScanRows < end) {
+                k.template step<false>();
+                rows.read(k, channel, shared.o, shared.c, lane);
+            }
+            if (saved && t0 % ILX_SCAN_BLOCK == 0) {
+                const ArgsPtr p = arguments_again();
+                if (c.active) store_state<V>(saved, p->s.states, p->s.channels, channel4, h);
+                saved += static_cast<int64_t>(p->s.states) * p->s.channels;
+            }
+            if (k.flags & kSoftplus) {
 #pragma unroll
-                    for (int n = 0; n < S; ++n) h[n] = 0.0f;
+                for (int i = 0; i < kScanRows; ++i) dt[i] = softplus_f(dt[i]);
+            }
+            float y[kScanRows];
+            static_for<kScanRows>([&](auto r) {
+                constexpr int i = r;
+                if (i < count) {
+                    forget_if(starts >> i & 1, h);
+                    advance<i>(h, A2, B, dt[i], dt[i] * x[i]);
+                    y[i] = dot<V>(C[i], h, skip * x[i]);
                 }
-                advance(h, A2, B[i], dt[i], dt[i] * x[i]);
-                float y = dot<S>(C[i], h, skip * x[i]);
-                if (in.gate) y *= z[i] * sigmoid_fast(z[i]);
-                if (c.active) po[row_offset(static_cast<uint32_t>(t0 + i), s.out_time)] = from_f32<T>(y);
+            });
+            if (k.flags & kHasGate) {
+#pragma unroll
+                for (int i = 0; i < kScanRows; ++i) y[i] *= z[i] * sigmoid_fast(z[i]);
+            }
+            if (c.active) {
+#pragma unroll
+                for (int i = 0; i < kScanRows; ++i)
+                    if (i < count) lane_store<T>(out.buffer(), channel, i * out.time, from_f32<T>(y[i]));
+            }
+            out.step(kScanRows);
+        }
+        // the next item's first rows are on their way while this one is finished
+        const int next = item + slots;
+        k.item = next;
+        if (next < items) {
+            k.template open<false>(next, c.group);
+            if (k.begin < k.end) rows.read(k, channel, shared.o, shared.c, lane);
+        }
+        {
+            const ArgsPtr p = arguments_again();
+            const int length = static_cast<int>(p->s.length), part_rows = static_cast<int>(p->part_rows), limit = begin + part_rows < length ? begin + part_rows : length;
+            const int first = end > begin ? end : begin;
+            if (c.active && (first < limit || p->s.last)) {
+                out.set(p->s.out, b * p->s.out_batch, first, p->s.out_time);
+                for (int t = first; t < limit; ++t, out.step(1)) lane_store<T>(out.buffer(), channel, 0, from_f32<T>(0.0f));
+                if (p->s.last) {   // the part that ends the sequence
+                    const int len = p->s.lengths ? static_cast<int>(scan_length(a.s, b)) : length;
+                    if ((begin < len && len <= limit) || (len == 0 && begin == 0))
+                        store_state<V>(p->s.last + static_cast<int64_t>(b) * p->s.states * p->s.channels, p->s.states, p->s.channels, channel4, h);
+                }
             }
         }
-    }
-    if (!c.active) return;
-    for (int64_t t = begin > len ? begin : len; t < limit; ++t) po[t * s.out_time] = from_f32<T>(0.0f);
-    if (s.last && ((begin < len && len <= limit) || (len == 0 && part == 0))) {   // the part that ends the sequence
-#pragma unroll
-        for (int n = 0; n < S; ++n)
-            if (n < s.states) s.last[(b * s.states + n) * channels + c.d] = h[n];
     }
 }
 
@@ -155,78 +285,75 @@ __global__ void __launch_bounds__(64) scan_forward_kernel(ScanArgs a) {
 // state ahead of it, r <- a (r + dy C) from its last row to its first.
 template <typename T, typename TB, int S, bool REVERSE>
 __global__ void __launch_bounds__(64) scan_part_kernel(ScanArgs a) {
-    constexpr int W = (S + 15) / 16;
+    constexpr int V = S / 4, W = (S + 15) / 16;
     const int lane = threadIdx.x;
-    const uint32_t item = blockIdx.x / a.blocks, parts = static_cast<uint32_t>(a.parts);
-    const int64_t b = item / parts, part = item % parts;
     const ChannelLane c = channel_lane(a, blockIdx.x % a.blocks, lane);
-    const ilx_state_space& s = a.s;
-    const int64_t len = scan_length(s, b), channels = s.channels, begin = part * a.part_rows;
-    const int64_t limit = begin + a.part_rows < s.length ? begin + a.part_rows : s.length, end = limit < len ? limit : len;
-    float A2[S], h[S], sum = 0.0f;
+    const uint32_t channel = c.d * sizeof(T), channel4 = c.d * 4;
+    const SharedStates<TB, W> shared(lane, a.s.states);
+    f32x4 A2[V], h[V];
+    load_decays<V>(a, c.d, A2);
+#pragma unroll
+    for (int m = 0; m < V; ++m) h[m] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    float sum = 0.0f;
     bool any = false;
+    const float bias = a.s.delta_bias ? a.s.delta_bias[c.d] : 0.0f;
+    ScanRows<T, TB, W, REVERSE, false> rows;
+    ScanStreams<T, TB> k;
+    k.flags = scan_flags<V>(a.s);
+    k.template open<REVERSE>(blockIdx.x / a.blocks, c.group);
+    if (k.begin < k.end) {
+        rows.read(k, channel, shared.o, shared.c, lane);
+        for (;;) {
+            const int count = k.count();
+            float x[kScanRows], dt[kScanRows], M[W];
 #pragma unroll
-    for (int n = 0; n < S; ++n) {
-        A2[n] = n < s.states ? s.A[static_cast<int64_t>(c.d) * s.states + n] * kLog2e : 0.0f;
-        h[n] = 0.0f;
-    }
-    const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f;
-    const ScanReader<T, TB, S> in(a, c, b, lane, REVERSE ? s.grad_out : s.x, REVERSE ? s.grad_out_batch : s.x_batch, REVERSE ? s.grad_out_time : s.x_time);
-    ScanRow<T, TB, W> rows[kScanRows];
-    auto read = [&](int64_t t0) {
-#pragma unroll
-        for (int i = 0; i < kScanRows; ++i)
-            in.template read<!REVERSE, REVERSE, REVERSE>(rows[i], static_cast<uint32_t>(t0 + i < end ? t0 + i : end - 1));
-    };
-    const int64_t steps = begin < end ? (end - begin + kScanRows - 1) / kScanRows : 0;
-    if (steps > 0) read(begin + (REVERSE ? steps - 1 : 0) * kScanRows);
-    for (int64_t j = 0; j < steps; ++j) {
-        const int64_t t0 = begin + (REVERSE ? steps - 1 - j : j) * kScanRows;
-        const int count = end - t0 < kScanRows ? static_cast<int>(end - t0) : kScanRows;
-        float x[kScanRows], dt[kScanRows], z[kScanRows], M[kScanRows][W];
-#pragma unroll
-        for (int i = 0; i < kScanRows; ++i) {
-            x[i] = to_f32(rows[i].x);
-            dt[i] = to_f32(rows[i].delta) + bias;
-            if (REVERSE && in.gate) z[i] = to_f32(rows[i].gate);
-#pragma unroll
-            for (int k = 0; k < W; ++k) M[i][k] = in.state_lane(REVERSE ? rows[i].C : rows[i].B, k);
-        }
-        const uint64_t starts = start_bits(s, b, t0, count, lane);
-        any = any || starts != 0;
-        if (j + 1 < steps) read(REVERSE ? t0 - kScanRows : t0 + kScanRows);
-        if (s.softplus) {
-#pragma unroll
-            for (int i = 0; i < kScanRows; ++i) dt[i] = softplus_f(dt[i]);
-        }
-        if (REVERSE && in.gate) {
-#pragma unroll
-            for (int i = 0; i < kScanRows; ++i) x[i] *= z[i] * sigmoid_fast(z[i]);
-        }
-#pragma unroll
-        for (int k = 0; k < kScanRows; ++k) {
-            const int i = REVERSE ? kScanRows - 1 - k : k;
-            if (i < count) {
-                sum += dt[i];
-                if (REVERSE) {
-                    static_for<S>([&](auto m) {
-                        constexpr int n = m;
-                        h[n] = __builtin_amdgcn_exp2f(dt[i] * A2[n]) * (h[n] + x[i] * from_lane<(n & 15)>(M[i][n >> 4]));
-                    });
-                }
-                if (starts >> i & 1) {
-#pragma unroll
-                    for (int n = 0; n < S; ++n) h[n] = 0.0f;
-                }
-                if (!REVERSE) advance(h, A2, M[i], dt[i], dt[i] * x[i]);
+            for (int i = 0; i < kScanRows; ++i) {
+                x[i] = to_f32(rows.x[i]);
+                dt[i] = to_f32(rows.delta[i]) + bias;
             }
+            if (REVERSE && (k.flags & kHasGate)) {
+#pragma unroll
+                for (int i = 0; i < kScanRows; ++i) {
+                    const float z = to_f32(rows.gate[i]);
+                    x[i] *= z * sigmoid_fast(z);
+                }
+            }
+#pragma unroll
+            for (int j = 0; j < W; ++j) M[j] = masked(to_f32(rows.o[j]), shared.o_mask[j]);
+            const uint32_t starts = rows.starts;
+            any = any || starts != 0;
+            const bool more = REVERSE ? k.t0 > k.begin : k.t0 + kScanRows < k.end;
+            if (more) {
+                k.template step<REVERSE>();
+                rows.read(k, channel, shared.o, shared.c, lane);
+            }
+            if (k.flags & kSoftplus) {
+#pragma unroll
+                for (int i = 0; i < kScanRows; ++i) dt[i] = softplus_f(dt[i]);
+            }
+            static_for<kScanRows>([&](auto r) {
+                constexpr int i = REVERSE ? kScanRows - 1 - r : r;
+                if (i < count) {
+                    sum += dt[i];
+                    if constexpr (REVERSE) {
+                        static_for<V>([&](auto q) {
+                            constexpr int m = q;
+                            h[m] = outer<4 * (m & 3) + i>(M[m >> 2], x[i], h[m]);
+#pragma unroll
+                            for (int j = 0; j < 4; ++j) h[m][j] *= __builtin_amdgcn_exp2f(dt[i] * A2[m][j]);
+                        });
+                    }
+                    forget_if(starts >> i & 1, h);
+                    if constexpr (!REVERSE) advance<i>(h, A2, M, dt[i], dt[i] * x[i]);
+                }
+            });
+            if (!more) break;
         }
     }
     if (!c.active) return;
-#pragma unroll
-    for (int n = 0; n < S; ++n)
-        if (n < s.states) a.part_state[(static_cast<int64_t>(item) * s.states + n) * channels + c.d] = h[n];
-    a.part_decay[static_cast<int64_t>(item) * channels + c.d] = any ? __builtin_inff() : sum;
+    const ArgsPtr p = arguments_again();
+    store_state<V>(p->part_state + static_cast<int64_t>(k.item) * p->s.states * p->s.channels, p->s.states, p->s.channels, channel4, h);
+    p->part_decay[static_cast<int64_t>(k.item) * p->s.channels + c.d] = any ? __builtin_inff() : sum;
 }
 
 // Passes the states through the parts: part_state becomes what enters each part (backward: the gradient that enters it from
@@ -279,44 +406,39 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(ScanArgs a, int backwar
 // the state, read and written once.
 template <typename T, typename TB, int S>
 __global__ void __launch_bounds__(64) scan_step_kernel(ScanArgs a) {
-    constexpr int W = (S + 15) / 16;
+    constexpr int V = S / 4, W = (S + 15) / 16;
     const int lane = threadIdx.x;
     const ChannelLane c = channel_lane(a, blockIdx.x % a.blocks, lane);
+    const uint32_t channel = c.d * sizeof(T), channel4 = c.d * 4;
+    const SharedStates<TB, W> shared(lane, a.s.states);
     const ilx_state_space& s = a.s;
-    const int64_t channels = s.channels;
-    float A2[S];
-#pragma unroll
-    for (int n = 0; n < S; ++n) A2[n] = n < s.states ? s.A[static_cast<int64_t>(c.d) * s.states + n] * kLog2e : 0.0f;
+    f32x4 A2[V], h[V];
+    load_decays<V>(a, c.d, A2);
     const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f, skip = s.D ? s.D[c.d] : 0.0f;
+    const int64_t state_size = static_cast<int64_t>(s.states) * s.channels;
     for (int64_t b = blockIdx.x / a.blocks; b < s.batch; b += a.slots) {
-        float h[S], B[W], C[W];
-        float* state = s.last + b * s.states * channels + c.d;
+        float* state = s.last + b * state_size;
+        load_state<V>(state, s.states, s.channels, channel4, h);
+        float x = to_f32(lane_load<T>(row_buffer(static_cast<const T*>(s.x) + b * s.x_batch), channel, 0));
+        float dt = to_f32(lane_load<T>(row_buffer(static_cast<const T*>(s.delta) + b * s.delta_batch), channel, 0)) + bias, z = 0.0f;
+        if (s.gate) z = to_f32(lane_load<T>(row_buffer(static_cast<const T*>(s.gate) + b * s.gate_batch), channel, 0));
+        const TB* pB = static_cast<const TB*>(s.B) + b * s.B_batch + c.group * s.states;
+        const TB* pC = static_cast<const TB*>(s.C) + b * s.C_batch + c.group * s.states;
+        float B[W], C[W];
 #pragma unroll
-        for (int n = 0; n < S; ++n) h[n] = n < s.states ? state[n * channels] : 0.0f;
-        const ScanReader<T, TB, S> in(a, c, b, lane, s.x, s.x_batch, 0);
-        ScanRow<T, TB, W> row;
-        in.template read<true, true, true>(row, 0);
-        const bool start = s.starts && s.starts[b * s.starts_batch];
-#pragma unroll
-        for (int k = 0; k < W; ++k) B[k] = in.state_lane(row.B, k), C[k] = in.state_lane(row.C, k);
-        const float x = to_f32(row.x);
-        float dt = to_f32(row.delta) + bias;
+        for (int j = 0; j < W; ++j) {
+            B[j] = masked(to_f32(lane_load<TB>(row_buffer(pB), shared.o[j], 0)), shared.o_mask[j]);
+            C[j] = masked(to_f32(lane_load<TB>(row_buffer(pC), shared.c[j], 0)), shared.c_mask[j]);
+        }
+        const bool start = s.starts && uni(static_cast<int>(s.starts[b * s.starts_batch]));
         if (s.softplus) dt = softplus_f(dt);
-        if (start) {
-#pragma unroll
-            for (int n = 0; n < S; ++n) h[n] = 0.0f;
-        }
-        advance(h, A2, B, dt, dt * x);
-        float y = dot<S>(C, h, skip * x);
-        if (in.gate) {
-            const float z = to_f32(row.gate);
-            y *= z * sigmoid_fast(z);
-        }
+        forget_if(start, h);
+        advance<0>(h, A2, B, dt, dt * x);
+        float y = dot<V>(C, h, skip * x);
+        if (s.gate) y *= z * sigmoid_fast(z);
         if (!c.active) continue;
-#pragma unroll
-        for (int n = 0; n < S; ++n)
-            if (n < s.states) state[n * channels] = h[n];
-        static_cast<T*>(s.out)[b * s.out_batch + c.d] = from_f32<T>(y);
+        store_state<V>(state, s.states, s.channels, channel4, h);
+        lane_store<T>(row_buffer(static_cast<T*>(s.out) + b * s.out_batch), channel, 0, from_f32<T>(y));
     }
 }
 
@@ -326,16 +448,22 @@ int scan_check(const ilx_state_space& s, const char* name) {
     ILX_REQUIRE(s.channels % s.groups == 0, ILX_ESHAPE, "%s: %d channels do not split into %d groups", name, s.channels, s.groups);
     ILX_REQUIRE(s.states >= 1 && s.states <= ILX_SCAN_MAX_STATES, ILX_ESHAPE, "%s: %d states (1..%d supported)", name, s.states,
                 ILX_SCAN_MAX_STATES);
-    ILX_REQUIRE(s.channels <= INT32_MAX / ILX_SCAN_MAX_STATES - 64, ILX_ESHAPE, "%s: %d channels", name, s.channels);
+    ILX_REQUIRE(s.channels <= (1 << 24), ILX_ESHAPE, "%s: %d channels", name, s.channels);
     ILX_REQUIRE(s.dtype >= ILX_F32 && s.dtype <= ILX_F16, ILX_EINVAL, "%s: unknown type %d", name, s.dtype);
     ILX_REQUIRE(s.bc_dtype == ILX_F32 || s.bc_dtype == s.dtype, ILX_EINVAL, "%s: B and C of type %d beside activations of type %d", name,
                 s.bc_dtype, s.dtype);
     ILX_REQUIRE(s.batch <= INT32_MAX && s.length <= INT32_MAX - 64 && s.batch * (s.length + 1) < (int64_t{1} << 40), ILX_ESHAPE,
                 "%s: shape (%lld, %lld) too large", name, (long long)s.batch, (long long)s.length);
     if (s.length > 1)
-        for (const int64_t stride : {s.x_time, s.delta_time, s.gate_time, s.B_time, s.C_time, s.out_time, s.grad_out_time, s.grad_time})
-            ILX_REQUIRE(stride >= 0 && stride <= UINT32_MAX, ILX_ESHAPE, "%s: a time stride of %lld elements", name, (long long)stride);
+        for (const int64_t stride : {s.x_time, s.delta_time, s.gate_time, s.B_time, s.C_time, s.out_time, s.grad_out_time, s.grad_time, s.starts_time})
+            ILX_REQUIRE(stride >= 0 && stride < (int64_t{1} << 26), ILX_ESHAPE, "%s: a time stride of %lld elements", name, (long long)stride);
     return ILX_OK;
+}
+
+// Workgroups per block of channels: enough for four waves a SIMD, each with as many items as the next.
+void share_items(ScanArgs& a, int64_t items) {
+    const int64_t waves = 16 * device_cu_count(), most = waves / a.blocks > 0 ? waves / a.blocks : 1, each = (items + most - 1) / most;
+    a.slots = each > 0 ? (items + each - 1) / each : 1;
 }
 
 ScanArgs scan_args(const ilx_state_space& s) {
@@ -346,6 +474,8 @@ ScanArgs scan_args(const ilx_state_space& s) {
     a.blocks = s.groups * a.group_blocks;
     a.saved_blocks = (s.length + ILX_SCAN_BLOCK - 1) / ILX_SCAN_BLOCK;
     a.parts = 1, a.part_rows = s.length;
+    a.decays_aligned = aligned_to(s.A, 16);
+    share_items(a, s.batch);
     return a;
 }
 
@@ -364,6 +494,7 @@ int64_t divide_scan(ScanArgs& a, float* workspace) {
     if (a.parts == 1) return 0;
     const int64_t states = s.batch * a.parts * s.states * s.channels, decays = s.batch * a.parts * s.channels;
     a.part_state = workspace, a.part_decay = workspace + states;
+    share_items(a, s.batch * a.parts);
     return states + decays;
 }
 
@@ -376,7 +507,7 @@ namespace {
 enum ScanKind { kForward, kStep, kParts, kPartsBackward };
 
 template <typename T, typename TB, int S> void scan_launch(ScanKind kind, const ScanArgs& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(kind == kStep ? a.slots * a.blocks : a.s.batch * a.parts * a.blocks)), threads(64);
+    const dim3 grid(static_cast<unsigned>(kind == kStep || kind == kForward ? a.slots * a.blocks : a.s.batch * a.parts * a.blocks)), threads(64);
     switch (kind) {
         case kStep: ILX_LAUNCH((scan_step_kernel<T, TB, S>), grid, threads, 0, s, a); break;
         case kParts: ILX_LAUNCH((scan_part_kernel<T, TB, S, false>), grid, threads, 0, s, a); break;
@@ -423,7 +554,7 @@ extern "C" int ilx_state_space_forward(const ilx_state_space* scan, void* stream
     const int64_t needed = divide_scan(a, s.workspace);
     ILX_REQUIRE(needed == 0 || (s.workspace && s.workspace_floats >= needed), ILX_EINVAL,
                 "ilx_state_space_forward: workspace of %lld floats, %lld needed", (long long)s.workspace_floats, (long long)needed);
-    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX, ILX_ESHAPE, "ilx_state_space_forward: shape too large for one launch");
+    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX - 65536, ILX_ESHAPE, "ilx_state_space_forward: shape too large for one launch");
     if (a.parts > 1) launch_part_states(a, false, as_stream(stream));
     scan_dispatch(kForward, a, as_stream(stream));
     ILX_LAUNCH_CHECK("ilx_state_space_forward");
@@ -440,10 +571,8 @@ extern "C" int ilx_state_space_step(const ilx_state_space* scan, void* stream) {
     ILX_REQUIRE(s.x && s.delta && s.A && s.B && s.C && s.out && s.state, ILX_EINVAL, "ilx_state_space_step: NULL operand");
     ILX_REQUIRE(s.state == s.last, ILX_EINVAL, "ilx_state_space_step: the state is updated in place, last must be state");
     ILX_REQUIRE(!s.lengths && !s.saved, ILX_EINVAL, "ilx_state_space_step: lengths and saved must be NULL");
-    ScanArgs a = scan_args(s);
-    const int64_t most = 8192 / a.blocks > 0 ? 8192 / a.blocks : 1;
-    a.slots = s.batch < most ? s.batch : most;
-    ILX_REQUIRE(a.slots * a.blocks <= INT32_MAX, ILX_ESHAPE, "ilx_state_space_step: shape too large for one launch");
+    const ScanArgs a = scan_args(s);
+    ILX_REQUIRE(s.batch * a.blocks <= INT32_MAX - 65536, ILX_ESHAPE, "ilx_state_space_step: shape too large for one launch");
     scan_dispatch(kStep, a, as_stream(stream));
     ILX_LAUNCH_CHECK("ilx_state_space_step");
     return ILX_OK;

@@ -15,6 +15,23 @@ constexpr int kRows = ILX_SCAN_BLOCK;
 constexpr int kStates = 4;   // per wave
 constexpr float kLn2 = 0.693147180559945309417f;
 
+
+template <int L> __device__ __forceinline__ float from_lane(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + L, 0xf, 0xf, true));
+}
+template <int L> __device__ __forceinline__ void dot_four(float& y, float c, const float (&h)[4]) {
+    dot_four<L, true>(y, c, f32x4{h[0], h[1], h[2], h[3]});
+}
+template <int L> __device__ __forceinline__ void add_four(float (&r)[4], float c, float x) {
+    asm("s_nop 1\n"
+        "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+        : "+&v"(r[0]), "+&v"(r[1]), "+&v"(r[2]), "+&v"(r[3])
+        : "v"(c), "v"(x), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
+}
+
 template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
     const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true);
     return v + __builtin_bit_cast(float, o);

@@ -3,6 +3,7 @@
 #pragma once
 
 #include "sequence_dev.h"
+#include "uniform_access.h"
 
 #include <utility>
 
@@ -18,7 +19,8 @@ struct ScanArgs {
     int64_t parts, part_rows;
     float* part_state;   // (batch, parts, states, channels): what a part adds; after the join what enters it
     float* part_decay;   // (batch, parts, channels): sum of dt over a part, infinity if a start lies in it
-    int64_t slots;       // backward, step: workgroups per block of channels
+    int64_t slots;       // workgroups per block of channels
+    bool decays_aligned; // A on a 16-byte boundary
     float* sums;         // backward: (slots, states + 2, channels) partial sums of dA, dD and d delta_bias
     float* shared;       // backward: (group_blocks, batch, length, groups, 2 * padded states) partial sums of dB, dC
 };
@@ -48,6 +50,50 @@ __device__ __forceinline__ int64_t row_offset(uint32_t row, int64_t stride) {
     return static_cast<int64_t>(static_cast<uint64_t>(row) * static_cast<uint32_t>(stride));
 }
 
+// The kernel's arguments, read anew: a value that an item needs once must not hold scalar registers through all of its rows
+// (the compiler would keep all of them, and spill into vector registers, two to four cycles an access).
+typedef const __attribute__((address_space(4))) ScanArgs* ArgsPtr;
+__device__ __forceinline__ ArgsPtr arguments_again() {
+    auto p = __builtin_amdgcn_kernarg_segment_ptr();
+    asm volatile("" : "+s"(p));
+    return (ArgsPtr)p;
+}
+
+// Elements of a row that all lanes share, by buffer instructions: the row is a scalar base and a scalar offset, the lane's byte
+// offset one vector register that never changes, so an access costs no address arithmetic in the vector unit.
+template <typename T> __device__ __forceinline__ __amdgpu_buffer_rsrc_t row_buffer(const T* base) {
+    const uint64_t p = uni(reinterpret_cast<uint64_t>(base));
+    return __builtin_amdgcn_make_buffer_rsrc(reinterpret_cast<void*>(p), 0, 0xffffffff, 0x00027000);
+}
+template <typename T> __device__ __forceinline__ T lane_load(__amdgpu_buffer_rsrc_t row, uint32_t lane_bytes, uint32_t row_bytes) {
+    if constexpr (sizeof(T) == 4)
+        return __builtin_bit_cast(T, __builtin_amdgcn_raw_buffer_load_b32(row, lane_bytes, row_bytes, 0));
+    else
+        return __builtin_bit_cast(T, static_cast<uint16_t>(__builtin_amdgcn_raw_buffer_load_b16(row, lane_bytes, row_bytes, 0)));
+}
+template <typename T> __device__ __forceinline__ void lane_store(__amdgpu_buffer_rsrc_t row, uint32_t lane_bytes, uint32_t row_bytes, T v) {
+    if constexpr (sizeof(T) == 4)
+        __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, v), row, lane_bytes, row_bytes, 0);
+    else
+        __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), row, lane_bytes, row_bytes, 0);
+}
+
+// Rows of one sequence, from a moving first one.  Time strides are below 2^26 elements, so that the offset of one of the next 15
+// rows fits 32 bits.
+template <typename T> struct Stream {
+    const T* p;
+    uint32_t time;   // bytes
+    __device__ __forceinline__ void set(const void* base, int64_t sequence, int t0, int64_t stride) {
+        time = static_cast<uint32_t>(stride) * static_cast<uint32_t>(sizeof(T));
+        p = static_cast<const T*>(base) + sequence;
+        step(t0);
+    }
+    __device__ __forceinline__ void step(int rows) {
+        p = reinterpret_cast<const T*>(reinterpret_cast<uintptr_t>(p) + static_cast<int64_t>(rows) * static_cast<int64_t>(time));
+    }
+    __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer() const { return row_buffer(p); }
+};
+
 // Bit i: an episode begins at row t0 + i (i < count <= 64).
 __device__ __forceinline__ uint64_t start_bits(const ilx_state_space& s, int64_t b, int64_t t0, int count, int lane) {
     if (!s.starts) return 0;
@@ -61,69 +107,47 @@ template <typename F, int... I> __device__ __forceinline__ void static_for_(F f,
 }
 template <int N, typename F> __device__ __forceinline__ void static_for(F f) { static_for_(f, std::make_integer_sequence<int, N>{}); }
 
-// B and C of a row are the same for all channels of a wave.  They are held with state n in lane n of every 16 lanes, and an
-// instruction that multiplies by one of them takes it from that lane (a row broadcast in its operand): no instruction, scalar
-// register or LDS access of its own.
-template <int L> __device__ __forceinline__ float from_lane(float v) {
-    return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + L, 0xf, 0xf, true));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
+
+// B and C of a row are the same for all channels of a wave, so they are kept spread over lanes and enter the arithmetic from
+// there, without an instruction, scalar register or LDS access of their own:
+//  * h[0..3] += B[0..3] u  for all 64 channels is one 4 x 4 x 1 matrix instruction of 16 blocks: a lane's four results are its
+//    block's four values of the first operand times the lane's own second operand, and the first operand's block is the same
+//    for all blocks (or all of a row of 16 lanes).  One register holds 64 such values: 16 states of 4 rows.
+//  * y += sum_n C[n] h[n]  takes C[n] from lane n of every 16 lanes (a row broadcast in the multiply-add's operand).
+// Measured rates at full occupancy, in cycles a SIMD: multiply-add 2.6, with a broadcast operand 4.3, the matrix instruction 9.4 (for
+// four multiply-adds), exponential 8.2, a select 4.6, half a wave's exchange (permlane swap) 8.4.
+template <int BLOCK> __device__ __forceinline__ f32x4 outer(float values, float u, f32x4 h) {   // any 4 lanes' values for all lanes
+    return __builtin_amdgcn_mfma_f32_4x4x1f32(values, u, h, 4, BLOCK, 0);
 }
 
-// y0 + y1 += sum_n c[lane n] h[n] and r[n] += c[lane L + n] x.  The compiler does not give a fused multiply-add the
-// broadcast operand, hence the assembly; a broadcast may not read what one of the two instructions ahead wrote, hence s_nop.
-#define ILX_BCAST(n) " row_newbcast:" #n " row_mask:0xf bank_mask:0xf\n"
-__device__ __forceinline__ void dot_states(float& y0, float& y1, float c, const float (&h)[4]) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %2, %3" ILX_BCAST(0) "v_fmac_f32_dpp %1, %2, %4" ILX_BCAST(1)
-        "v_fmac_f32_dpp %0, %2, %5" ILX_BCAST(2) "v_fmac_f32_dpp %1, %2, %6" ILX_BCAST(3)
-        : "+&v"(y0), "+&v"(y1)
-        : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]));
+// y += sum of four states times lanes L .. L + 3 of c.  The compiler does not give a fused multiply-add the broadcast operand, hence
+// the assembly.  FIRST: a broadcast may not read what one of the two instructions ahead wrote, and a matrix instruction's result may
+// not be read within five; later ones follow it.
+template <int L, bool FIRST> __device__ __forceinline__ void dot_four(float& y, float c, f32x4 h) {
+    if constexpr (FIRST)
+        asm("s_nop 7\n"
+            "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+            "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+            "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+            "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+            : "+&v"(y)
+            : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
+    else
+        asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+            "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+            "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+            "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+            : "+&v"(y)
+            : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
 }
-__device__ __forceinline__ void dot_states(float& y0, float& y1, float c, const float (&h)[8]) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %2, %3" ILX_BCAST(0) "v_fmac_f32_dpp %1, %2, %4" ILX_BCAST(1)
-        "v_fmac_f32_dpp %0, %2, %5" ILX_BCAST(2) "v_fmac_f32_dpp %1, %2, %6" ILX_BCAST(3)
-        "v_fmac_f32_dpp %0, %2, %7" ILX_BCAST(4) "v_fmac_f32_dpp %1, %2, %8" ILX_BCAST(5)
-        "v_fmac_f32_dpp %0, %2, %9" ILX_BCAST(6) "v_fmac_f32_dpp %1, %2, %10" ILX_BCAST(7)
-        : "+&v"(y0), "+&v"(y1)
-        : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "v"(h[4]), "v"(h[5]), "v"(h[6]), "v"(h[7]));
-}
-template <int O, int S> __device__ __forceinline__ void dot_sixteen(float& y0, float& y1, float c, const float (&h)[S]) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %2, %3" ILX_BCAST(0) "v_fmac_f32_dpp %1, %2, %4" ILX_BCAST(1)
-        "v_fmac_f32_dpp %0, %2, %5" ILX_BCAST(2) "v_fmac_f32_dpp %1, %2, %6" ILX_BCAST(3)
-        "v_fmac_f32_dpp %0, %2, %7" ILX_BCAST(4) "v_fmac_f32_dpp %1, %2, %8" ILX_BCAST(5)
-        "v_fmac_f32_dpp %0, %2, %9" ILX_BCAST(6) "v_fmac_f32_dpp %1, %2, %10" ILX_BCAST(7)
-        "v_fmac_f32_dpp %0, %2, %11" ILX_BCAST(8) "v_fmac_f32_dpp %1, %2, %12" ILX_BCAST(9)
-        "v_fmac_f32_dpp %0, %2, %13" ILX_BCAST(10) "v_fmac_f32_dpp %1, %2, %14" ILX_BCAST(11)
-        "v_fmac_f32_dpp %0, %2, %15" ILX_BCAST(12) "v_fmac_f32_dpp %1, %2, %16" ILX_BCAST(13)
-        "v_fmac_f32_dpp %0, %2, %17" ILX_BCAST(14) "v_fmac_f32_dpp %1, %2, %18" ILX_BCAST(15)
-        : "+&v"(y0), "+&v"(y1)
-        : "v"(c), "v"(h[O + 0]), "v"(h[O + 1]), "v"(h[O + 2]), "v"(h[O + 3]), "v"(h[O + 4]), "v"(h[O + 5]), "v"(h[O + 6]), "v"(h[O + 7]),
-          "v"(h[O + 8]), "v"(h[O + 9]), "v"(h[O + 10]), "v"(h[O + 11]), "v"(h[O + 12]), "v"(h[O + 13]), "v"(h[O + 14]), "v"(h[O + 15]));
-}
-__device__ __forceinline__ void dot_states(float& y0, float& y1, float c, const float (&h)[16]) { dot_sixteen<0>(y0, y1, c, h); }
-// four states from lane L on
-template <int L> __device__ __forceinline__ void dot_four(float& y, float c, const float (&h)[4]) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-        : "+&v"(y)
-        : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
-}
-template <int L> __device__ __forceinline__ void add_four(float (&r)[4], float c, float x) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-        : "+&v"(r[0]), "+&v"(r[1]), "+&v"(r[2]), "+&v"(r[3])
-        : "v"(c), "v"(x), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
-}
+
+// v where the state exists, else 0, without a select
+__device__ __forceinline__ float masked(float v, uint32_t mask) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & mask); }
 
 int scan_check(const ilx_state_space& s, const char* name);
 ScanArgs scan_args(const ilx_state_space& s);
+void share_items(ScanArgs& a, int64_t items);
 // parts of a sequence, and the floats their states and decays take
 int64_t divide_scan(ScanArgs& a, float* workspace);
 void launch_part_states(const ScanArgs& a, bool backward, hipStream_t stream);
