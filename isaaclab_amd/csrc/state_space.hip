@@ -16,6 +16,10 @@ namespace ilx {
 
 constexpr int kScanRows = 4;    // rows whose inputs are in registers together; divides ILX_SCAN_BLOCK
 constexpr int kMostParts = 256;
+constexpr int kScanWaves = 4;   // to a workgroup: independent, but a workgroup puts one on each SIMD of its CU (single waves end up
+                                // unevenly: two thirds of the waves that fit were resident on average)
+
+__device__ __forceinline__ int wave_unit() { return uni(static_cast<int>(blockIdx.x * kScanWaves + (threadIdx.x >> 6))); }
 
 enum { kHasGate = 1, kSoftplus = 2, kHasStarts = 4, kFull = 8 };   // kFull: as many states as the lane has registers
 
@@ -114,18 +118,18 @@ template <int ROW, int V, int W> __device__ __forceinline__ void advance(f32x4 (
 
 template <int V, int W> __device__ __forceinline__ float dot(const float (&C)[W], const f32x4 (&h)[V], float y) {
     float y1 = 0.0f;
-    static_for<V>([&](auto i) {
-        constexpr int m = i;
-        if constexpr (m & 1)
-            dot_four<4 * (m & 3), m == 1>(y1, C[m >> 2], h[m]);
-        else
-            dot_four<4 * (m & 3), m == 0>(y, C[m >> 2], h[m]);
-    });
-    return V > 1 ? y + y1 : y;
+    if constexpr (V == 1)
+        dot_states(y, y1, C[0], h[0]);
+    else if constexpr (V == 2)
+        dot_states(y, y1, C[0], h[0], h[1]);
+    else
+        dot_states(y, y1, C[0], h[0], h[1], h[2], h[3]);
+    if constexpr (V == 8) dot_states(y, y1, C[1], h[4], h[5], h[6], h[7]);
+    return y + y1;
 }
 
 // The lane's row of A times log2 e, zeros past the last state.
-template <int V> __device__ __forceinline__ void load_decays(const ScanArgs& a, int d, f32x4 (&A2)[V]) {
+template <int V> __device__ __forceinline__ void load_decays(const StateSpaceArgs& a, int d, f32x4 (&A2)[V]) {
     const float* A = a.s.A + static_cast<int64_t>(d) * a.s.states;
     if (a.s.states == 4 * V && a.decays_aligned) {
 #pragma unroll
@@ -183,10 +187,11 @@ template <int V> __device__ __forceinline__ int scan_flags(const ilx_state_space
 }
 
 template <typename T, typename TB, int S>
-__global__ void __launch_bounds__(64) scan_forward_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(64 * kScanWaves) scan_forward_kernel(StateSpaceArgs a) {
     constexpr int V = S / 4, W = (S + 15) / 16;
-    const int lane = threadIdx.x;
-    const ChannelLane c = channel_lane(a, blockIdx.x % a.blocks, lane);
+    const int lane = threadIdx.x & 63, unit = wave_unit();
+    if (unit >= a.units) return;
+    const ChannelLane c = channel_lane(a, unit % a.blocks, lane);
     const uint32_t channel = c.d * sizeof(T), channel4 = c.d * 4;
     const SharedStates<TB, W> shared(lane, a.s.states);
     const int items = static_cast<int>(a.s.batch * a.parts), slots = static_cast<int>(a.slots);
@@ -196,7 +201,7 @@ __global__ void __launch_bounds__(64) scan_forward_kernel(ScanArgs a) {
     ScanRows<T, TB, W, true, true> rows;
     ScanStreams<T, TB> k;
     k.flags = scan_flags<V>(a.s);
-    k.template open<false>(blockIdx.x / a.blocks, c.group);
+    k.template open<false>(unit / a.blocks, c.group);
     if (k.begin < k.end) rows.read(k, channel, shared.o, shared.c, lane);
     float* saved = nullptr;
     while (k.item < items) {
@@ -284,10 +289,11 @@ __global__ void __launch_bounds__(64) scan_forward_kernel(ScanArgs a) {
 // What a part of a sequence adds to the state, from zeros: forward the state behind it, backward (REVERSE) the gradient of the
 // state ahead of it, r <- a (r + dy C) from its last row to its first.
 template <typename T, typename TB, int S, bool REVERSE>
-__global__ void __launch_bounds__(64) scan_part_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(64 * kScanWaves) scan_part_kernel(StateSpaceArgs a) {
     constexpr int V = S / 4, W = (S + 15) / 16;
-    const int lane = threadIdx.x;
-    const ChannelLane c = channel_lane(a, blockIdx.x % a.blocks, lane);
+    const int lane = threadIdx.x & 63, unit = wave_unit();
+    if (unit >= a.units) return;
+    const ChannelLane c = channel_lane(a, unit % a.blocks, lane);
     const uint32_t channel = c.d * sizeof(T), channel4 = c.d * 4;
     const SharedStates<TB, W> shared(lane, a.s.states);
     f32x4 A2[V], h[V];
@@ -300,7 +306,7 @@ __global__ void __launch_bounds__(64) scan_part_kernel(ScanArgs a) {
     ScanRows<T, TB, W, REVERSE, false> rows;
     ScanStreams<T, TB> k;
     k.flags = scan_flags<V>(a.s);
-    k.template open<REVERSE>(blockIdx.x / a.blocks, c.group);
+    k.template open<REVERSE>(unit / a.blocks, c.group);
     if (k.begin < k.end) {
         rows.read(k, channel, shared.o, shared.c, lane);
         for (;;) {
@@ -359,7 +365,7 @@ __global__ void __launch_bounds__(64) scan_part_kernel(ScanArgs a) {
 // Passes the states through the parts: part_state becomes what enters each part (backward: the gradient that enters it from
 // the part behind).  64 states of a sequence to a workgroup, a sixteenth of the parts to each of its waves: a wave joins its own
 // parts, the waves' joins meet in LDS, and each wave passes what enters it through its parts again, out of registers.
-__global__ void __launch_bounds__(1024) scan_join_kernel(ScanArgs a, int backward, const float* first) {
+__global__ void __launch_bounds__(1024) scan_join_kernel(StateSpaceArgs a, int backward, const float* first) {
     constexpr int kWaves = 16, kPer = kMostParts / kWaves;
     __shared__ float s_decay[kWaves][64], s_state[kWaves][64];
     const ilx_state_space& s = a.s;
@@ -405,10 +411,11 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(ScanArgs a, int backwar
 // One row per sequence: the recurrence above with sequences in the place of rows, so that A stays in registers.  Bound by
 // the state, read and written once.
 template <typename T, typename TB, int S>
-__global__ void __launch_bounds__(64) scan_step_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(64 * kScanWaves) scan_step_kernel(StateSpaceArgs a) {
     constexpr int V = S / 4, W = (S + 15) / 16;
-    const int lane = threadIdx.x;
-    const ChannelLane c = channel_lane(a, blockIdx.x % a.blocks, lane);
+    const int lane = threadIdx.x & 63, unit = wave_unit();
+    if (unit >= a.units) return;
+    const ChannelLane c = channel_lane(a, unit % a.blocks, lane);
     const uint32_t channel = c.d * sizeof(T), channel4 = c.d * 4;
     const SharedStates<TB, W> shared(lane, a.s.states);
     const ilx_state_space& s = a.s;
@@ -416,7 +423,7 @@ __global__ void __launch_bounds__(64) scan_step_kernel(ScanArgs a) {
     load_decays<V>(a, c.d, A2);
     const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f, skip = s.D ? s.D[c.d] : 0.0f;
     const int64_t state_size = static_cast<int64_t>(s.states) * s.channels;
-    for (int64_t b = blockIdx.x / a.blocks; b < s.batch; b += a.slots) {
+    for (int64_t b = unit / a.blocks; b < s.batch; b += a.slots) {
         float* state = s.last + b * state_size;
         load_state<V>(state, s.states, s.channels, channel4, h);
         float x = to_f32(lane_load<T>(row_buffer(static_cast<const T*>(s.x) + b * s.x_batch), channel, 0));
@@ -461,13 +468,13 @@ int scan_check(const ilx_state_space& s, const char* name) {
 }
 
 // Workgroups per block of channels: enough for four waves a SIMD, each with as many items as the next.
-void share_items(ScanArgs& a, int64_t items) {
+void share_items(StateSpaceArgs& a, int64_t items) {
     const int64_t waves = 16 * device_cu_count(), most = waves / a.blocks > 0 ? waves / a.blocks : 1, each = (items + most - 1) / most;
     a.slots = each > 0 ? (items + each - 1) / each : 1;
 }
 
-ScanArgs scan_args(const ilx_state_space& s) {
-    ScanArgs a{};
+StateSpaceArgs scan_args(const ilx_state_space& s) {
+    StateSpaceArgs a{};
     a.s = s;
     a.group_channels = s.channels / s.groups;
     a.group_blocks = (a.group_channels + 63) / 64;
@@ -481,7 +488,7 @@ ScanArgs scan_args(const ilx_state_space& s) {
 
 // Two waves per SIMD hide a row's latency well enough that a second pass does not pay; below that a sequence is divided towards
 // four per SIMD, in parts of at least 32 rows (a part's cost ahead of its first row is that of about eight).
-int64_t divide_scan(ScanArgs& a, float* workspace) {
+int64_t divide_scan(StateSpaceArgs& a, float* workspace) {
     const ilx_state_space& s = a.s;
     const int64_t waves = s.batch * a.blocks, full = 4 * device_cu_count();   // one per SIMD
     if (waves == 0 || waves >= 2 * full || s.length < 64) return 0;
@@ -506,8 +513,9 @@ namespace {
 
 enum ScanKind { kForward, kStep, kParts, kPartsBackward };
 
-template <typename T, typename TB, int S> void scan_launch(ScanKind kind, const ScanArgs& a, hipStream_t s) {
-    const dim3 grid(static_cast<unsigned>(kind == kStep || kind == kForward ? a.slots * a.blocks : a.s.batch * a.parts * a.blocks)), threads(64);
+template <typename T, typename TB, int S> void scan_launch(ScanKind kind, StateSpaceArgs a, hipStream_t s) {
+    a.units = static_cast<int>((kind == kStep || kind == kForward ? a.slots : a.s.batch * a.parts) * a.blocks);
+    const dim3 grid(blocks_for(a.units, kScanWaves)), threads(64 * kScanWaves);
     switch (kind) {
         case kStep: ILX_LAUNCH((scan_step_kernel<T, TB, S>), grid, threads, 0, s, a); break;
         case kParts: ILX_LAUNCH((scan_part_kernel<T, TB, S, false>), grid, threads, 0, s, a); break;
@@ -516,7 +524,7 @@ template <typename T, typename TB, int S> void scan_launch(ScanKind kind, const 
     }
 }
 
-template <typename T, typename TB> void scan_states(ScanKind kind, const ScanArgs& a, hipStream_t s) {
+template <typename T, typename TB> void scan_states(ScanKind kind, const StateSpaceArgs& a, hipStream_t s) {
     const int n = a.s.states;
     if (n <= 4) return scan_launch<T, TB, 4>(kind, a, s);
     if (n <= 8) return scan_launch<T, TB, 8>(kind, a, s);
@@ -524,7 +532,7 @@ template <typename T, typename TB> void scan_states(ScanKind kind, const ScanArg
     scan_launch<T, TB, 32>(kind, a, s);
 }
 
-void scan_dispatch(ScanKind kind, const ScanArgs& a, hipStream_t s) {
+void scan_dispatch(ScanKind kind, const StateSpaceArgs& a, hipStream_t s) {
     const bool wide = a.s.bc_dtype == ILX_F32;
     switch (a.s.dtype) {
         case ILX_F32: return scan_states<float, float>(kind, a, s);
@@ -535,7 +543,7 @@ void scan_dispatch(ScanKind kind, const ScanArgs& a, hipStream_t s) {
 
 }  // namespace
 
-void ilx::launch_part_states(const ScanArgs& a, bool backward, hipStream_t s) {
+void ilx::launch_part_states(const StateSpaceArgs& a, bool backward, hipStream_t s) {
     scan_dispatch(backward ? kPartsBackward : kParts, a, s);
     const int64_t column_blocks = (static_cast<int64_t>(a.s.states) * a.s.channels + 63) / 64;
     ILX_LAUNCH(scan_join_kernel, dim3(static_cast<unsigned>(a.s.batch * column_blocks)), dim3(1024), 0, s, a, backward ? 1 : 0,
@@ -550,7 +558,7 @@ extern "C" int ilx_state_space_forward(const ilx_state_space* scan, void* stream
     if (s.batch == 0) return ILX_OK;
     ILX_REQUIRE(s.A && (s.length == 0 || (s.x && s.delta && s.B && s.C && s.out)), ILX_EINVAL, "ilx_state_space_forward: NULL operand");
     ILX_REQUIRE(!s.last || s.last != s.state, ILX_EINVAL, "ilx_state_space_forward: last and state are the same buffer");
-    ScanArgs a = scan_args(s);
+    StateSpaceArgs a = scan_args(s);
     const int64_t needed = divide_scan(a, s.workspace);
     ILX_REQUIRE(needed == 0 || (s.workspace && s.workspace_floats >= needed), ILX_EINVAL,
                 "ilx_state_space_forward: workspace of %lld floats, %lld needed", (long long)s.workspace_floats, (long long)needed);
@@ -571,7 +579,7 @@ extern "C" int ilx_state_space_step(const ilx_state_space* scan, void* stream) {
     ILX_REQUIRE(s.x && s.delta && s.A && s.B && s.C && s.out && s.state, ILX_EINVAL, "ilx_state_space_step: NULL operand");
     ILX_REQUIRE(s.state == s.last, ILX_EINVAL, "ilx_state_space_step: the state is updated in place, last must be state");
     ILX_REQUIRE(!s.lengths && !s.saved, ILX_EINVAL, "ilx_state_space_step: lengths and saved must be NULL");
-    const ScanArgs a = scan_args(s);
+    const StateSpaceArgs a = scan_args(s);
     ILX_REQUIRE(s.batch * a.blocks <= INT32_MAX - 65536, ILX_ESHAPE, "ilx_state_space_step: shape too large for one launch");
     scan_dispatch(kStep, a, as_stream(stream));
     ILX_LAUNCH_CHECK("ilx_state_space_step");

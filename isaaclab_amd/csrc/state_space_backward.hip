@@ -20,7 +20,13 @@ template <int L> __device__ __forceinline__ float from_lane(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + L, 0xf, 0xf, true));
 }
 template <int L> __device__ __forceinline__ void dot_four(float& y, float c, const float (&h)[4]) {
-    dot_four<L, true>(y, c, f32x4{h[0], h[1], h[2], h[3]});
+    asm("s_nop 1\n"
+        "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+        "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+        : "+&v"(y)
+        : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
 }
 template <int L> __device__ __forceinline__ void add_four(float (&r)[4], float c, float x) {
     asm("s_nop 1\n"
@@ -66,7 +72,7 @@ struct ScanBlock {
 };
 
 template <typename T, typename TB, int NW>
-__global__ void __launch_bounds__(64 * NW, 3) scan_backward_kernel(ScanArgs a) {
+__global__ void __launch_bounds__(64 * NW, 3) scan_backward_kernel(StateSpaceArgs a) {
     constexpr int E = kRows / NW;   // rows a wave prepares and finishes per block
     __shared__ float2 s_step[2][kRows][64];       // dt and dt x, of this block and the one before
     __shared__ float s_dy[2][kRows][64];
@@ -296,7 +302,7 @@ __global__ void __launch_bounds__(64 * NW, 3) scan_backward_kernel(ScanArgs a) {
 }
 
 // dB and dC: the sums of the blocks of channels of a group, in order; rows past a sequence's end are zeros.
-template <typename TB> __global__ void __launch_bounds__(256) scan_shared_sums_kernel(ScanArgs a, int padded) {
+template <typename TB> __global__ void __launch_bounds__(256) scan_shared_sums_kernel(StateSpaceArgs a, int padded) {
     const ilx_state_space& s = a.s;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, rows = s.batch * s.length * s.groups;
     if (i >= rows * s.states) return;
@@ -322,8 +328,8 @@ namespace {
 
 int waves_for(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : 8; }
 
-ScanArgs backward_args(const ilx_state_space& s, int64_t* floats) {
-    ScanArgs a = scan_args(s);
+StateSpaceArgs backward_args(const ilx_state_space& s, int64_t* floats) {
+    StateSpaceArgs a = scan_args(s);
     const int64_t part_floats = divide_scan(a, s.workspace);
     const int64_t most = 2048 / a.blocks > 0 ? 2048 / a.blocks : 1, items = s.batch * a.parts;
     a.slots = items < most ? items : most;
@@ -335,11 +341,11 @@ ScanArgs backward_args(const ilx_state_space& s, int64_t* floats) {
     return a;
 }
 
-template <typename T, typename TB, int NW> void backward_launch(const ScanArgs& a, hipStream_t s) {
+template <typename T, typename TB, int NW> void backward_launch(const StateSpaceArgs& a, hipStream_t s) {
     ILX_LAUNCH((scan_backward_kernel<T, TB, NW>), dim3(static_cast<unsigned>(a.slots * a.blocks)), dim3(64 * NW), 0, s, a);
 }
 
-template <typename T, typename TB> void backward_states(const ScanArgs& a, hipStream_t s) {
+template <typename T, typename TB> void backward_states(const StateSpaceArgs& a, hipStream_t s) {
     const int waves = waves_for(a.s.states);
     switch (waves) {
         case 1: backward_launch<T, TB, 1>(a, s); break;
@@ -360,7 +366,7 @@ extern "C" int ilx_state_space_workspace(const ilx_state_space* scan, int backwa
     if (backward) {
         backward_args(*scan, floats);
     } else {
-        ScanArgs a = scan_args(*scan);
+        StateSpaceArgs a = scan_args(*scan);
         *floats = divide_scan(a, nullptr);
     }
     return ILX_OK;
@@ -376,7 +382,7 @@ extern "C" int ilx_state_space_backward(const ilx_state_space* scan, void* strea
                 ILX_EINVAL, "ilx_state_space_backward: NULL operand");
     ILX_REQUIRE(!some || (s.gate != nullptr) == (s.grad_gate != nullptr), ILX_EINVAL, "ilx_state_space_backward: gate and grad_gate come together");
     int64_t needed = 0;
-    const ScanArgs a = backward_args(s, &needed);
+    const StateSpaceArgs a = backward_args(s, &needed);
     ILX_REQUIRE(s.workspace_floats >= needed && (s.workspace || needed == 0), ILX_EINVAL,
                 "ilx_state_space_backward: workspace of %lld floats, %lld needed", (long long)s.workspace_floats, (long long)needed);
     ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX && s.batch * s.length * s.groups * s.states / 256 < INT32_MAX, ILX_ESHAPE,

@@ -9,7 +9,8 @@
 
 namespace ilx {
 
-struct ScanArgs {
+// (One name, one layout in the whole library: ilx::launch is instantiated by the type and its instances are merged between files.)
+struct StateSpaceArgs {
     ilx_state_space s;
     int group_channels;    // channels / groups
     int group_blocks;      // blocks of 64 channels per group
@@ -20,6 +21,7 @@ struct ScanArgs {
     float* part_state;   // (batch, parts, states, channels): what a part adds; after the join what enters it
     float* part_decay;   // (batch, parts, channels): sum of dt over a part, infinity if a start lies in it
     int64_t slots;       // workgroups per block of channels
+    int units;           // waves of a launch whose waves are independent
     bool decays_aligned; // A on a 16-byte boundary
     float* sums;         // backward: (slots, states + 2, channels) partial sums of dA, dD and d delta_bias
     float* shared;       // backward: (group_blocks, batch, length, groups, 2 * padded states) partial sums of dB, dC
@@ -30,7 +32,7 @@ struct ChannelLane {
     int group, d;
     bool active;
 };
-__device__ __forceinline__ ChannelLane channel_lane(const ScanArgs& a, int block, int lane) {
+__device__ __forceinline__ ChannelLane channel_lane(const StateSpaceArgs& a, int block, int lane) {
     ChannelLane c;
     c.group = block / a.group_blocks;
     const int within = (block - c.group * a.group_blocks) * 64 + lane;
@@ -52,7 +54,7 @@ __device__ __forceinline__ int64_t row_offset(uint32_t row, int64_t stride) {
 
 // The kernel's arguments, read anew: a value that an item needs once must not hold scalar registers through all of its rows
 // (the compiler would keep all of them, and spill into vector registers, two to four cycles an access).
-typedef const __attribute__((address_space(4))) ScanArgs* ArgsPtr;
+typedef const __attribute__((address_space(4))) StateSpaceArgs* ArgsPtr;
 __device__ __forceinline__ ArgsPtr arguments_again() {
     auto p = __builtin_amdgcn_kernarg_segment_ptr();
     asm volatile("" : "+s"(p));
@@ -121,35 +123,50 @@ template <int BLOCK> __device__ __forceinline__ f32x4 outer(float values, float 
     return __builtin_amdgcn_mfma_f32_4x4x1f32(values, u, h, 4, BLOCK, 0);
 }
 
-// y += sum of four states times lanes L .. L + 3 of c.  The compiler does not give a fused multiply-add the broadcast operand, hence
-// the assembly.  FIRST: a broadcast may not read what one of the two instructions ahead wrote, and a matrix instruction's result may
-// not be read within five; later ones follow it.
-template <int L, bool FIRST> __device__ __forceinline__ void dot_four(float& y, float c, f32x4 h) {
-    if constexpr (FIRST)
-        asm("s_nop 7\n"
-            "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-            "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-            "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-            "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-            : "+&v"(y)
-            : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
-    else
-        asm("v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-            "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-            "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-            "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-            : "+&v"(y)
-            : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
+// y0 + y1 += sum of the states times lanes 0 .. of c.  The compiler does not give a fused multiply-add the broadcast operand, hence
+// the assembly; a broadcast may not read what one of the two instructions ahead wrote, and a matrix instruction's result may not be
+// read within five, hence the wait ahead of each block.
+#define ILX_BCAST(n) " row_newbcast:" #n " row_mask:0xf bank_mask:0xf\n"
+#define ILX_WAIT "s_nop 7\n"
+__device__ __forceinline__ void dot_states(float& y0, float& y1, float c, const f32x4& a) {
+    asm(ILX_WAIT
+        "v_fmac_f32_dpp %0, %2, %3" ILX_BCAST(0) "v_fmac_f32_dpp %1, %2, %4" ILX_BCAST(1)
+        "v_fmac_f32_dpp %0, %2, %5" ILX_BCAST(2) "v_fmac_f32_dpp %1, %2, %6" ILX_BCAST(3)
+        : "+&v"(y0), "+&v"(y1)
+        : "v"(c), "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]));
+}
+__device__ __forceinline__ void dot_states(float& y0, float& y1, float c, const f32x4& a, const f32x4& b) {
+    asm(ILX_WAIT
+        "v_fmac_f32_dpp %0, %2, %3" ILX_BCAST(0) "v_fmac_f32_dpp %1, %2, %4" ILX_BCAST(1)
+        "v_fmac_f32_dpp %0, %2, %5" ILX_BCAST(2) "v_fmac_f32_dpp %1, %2, %6" ILX_BCAST(3)
+        "v_fmac_f32_dpp %0, %2, %7" ILX_BCAST(4) "v_fmac_f32_dpp %1, %2, %8" ILX_BCAST(5)
+        "v_fmac_f32_dpp %0, %2, %9" ILX_BCAST(6) "v_fmac_f32_dpp %1, %2, %10" ILX_BCAST(7)
+        : "+&v"(y0), "+&v"(y1)
+        : "v"(c), "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]));
+}
+__device__ __forceinline__ void dot_states(float& y0, float& y1, float c, const f32x4& a, const f32x4& b, const f32x4& d, const f32x4& e) {
+    asm(ILX_WAIT
+        "v_fmac_f32_dpp %0, %2, %3" ILX_BCAST(0) "v_fmac_f32_dpp %1, %2, %4" ILX_BCAST(1)
+        "v_fmac_f32_dpp %0, %2, %5" ILX_BCAST(2) "v_fmac_f32_dpp %1, %2, %6" ILX_BCAST(3)
+        "v_fmac_f32_dpp %0, %2, %7" ILX_BCAST(4) "v_fmac_f32_dpp %1, %2, %8" ILX_BCAST(5)
+        "v_fmac_f32_dpp %0, %2, %9" ILX_BCAST(6) "v_fmac_f32_dpp %1, %2, %10" ILX_BCAST(7)
+        "v_fmac_f32_dpp %0, %2, %11" ILX_BCAST(8) "v_fmac_f32_dpp %1, %2, %12" ILX_BCAST(9)
+        "v_fmac_f32_dpp %0, %2, %13" ILX_BCAST(10) "v_fmac_f32_dpp %1, %2, %14" ILX_BCAST(11)
+        "v_fmac_f32_dpp %0, %2, %15" ILX_BCAST(12) "v_fmac_f32_dpp %1, %2, %16" ILX_BCAST(13)
+        "v_fmac_f32_dpp %0, %2, %17" ILX_BCAST(14) "v_fmac_f32_dpp %1, %2, %18" ILX_BCAST(15)
+        : "+&v"(y0), "+&v"(y1)
+        : "v"(c), "v"(a[0]), "v"(a[1]), "v"(a[2]), "v"(a[3]), "v"(b[0]), "v"(b[1]), "v"(b[2]), "v"(b[3]), "v"(d[0]), "v"(d[1]), "v"(d[2]), "v"(d[3]),
+          "v"(e[0]), "v"(e[1]), "v"(e[2]), "v"(e[3]));
 }
 
 // v where the state exists, else 0, without a select
 __device__ __forceinline__ float masked(float v, uint32_t mask) { return __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, v) & mask); }
 
 int scan_check(const ilx_state_space& s, const char* name);
-ScanArgs scan_args(const ilx_state_space& s);
-void share_items(ScanArgs& a, int64_t items);
+StateSpaceArgs scan_args(const ilx_state_space& s);
+void share_items(StateSpaceArgs& a, int64_t items);
 // parts of a sequence, and the floats their states and decays take
-int64_t divide_scan(ScanArgs& a, float* workspace);
-void launch_part_states(const ScanArgs& a, bool backward, hipStream_t stream);
+int64_t divide_scan(StateSpaceArgs& a, float* workspace);
+void launch_part_states(const StateSpaceArgs& a, bool backward, hipStream_t stream);
 
 }  // namespace ilx
