@@ -21,22 +21,18 @@ __device__ __forceinline__ float rcp_fast(float x) { return __builtin_amdgcn_rcp
 
 __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.0f + exp_fast(-x)); }
 
-// log(1 + e^x) = max(x, 0) + log1p(e^-|x|), the second term as 2 artanh(e / (2 + e)) with e in (0, 1]: its argument is at
-// most 1/3, so the series in odd powers up to the 15th is short by less than 2^-26 of the value at every x (a logarithm of
-// 1 + e would lose e's last bits, which for a step size of 1e-4 are all it has).
+// log(1 + e^x) = max(x, 0) + log1p(e^-|x|), the second term as 2 artanh(s), s = e / (2 + e) with e in (0, 1] (a logarithm of 1 + e
+// would lose e's last bits, which for a step size of 1e-4 are all it has).  s is at most 1/3; the polynomial in s^2 is the one of degree
+// 4 with the least largest relative error on [0, 1/9], 2^-27.9.  In float32 the result is off by at most 5 units of 2^-24.
 __device__ __forceinline__ float softplus_f(float x) {
     const float e = exp_fast(-__builtin_fabsf(x));
     const float s = e * rcp_fast(2.0f + e), q = s * s;
-    float p = 1.0f / 15;
-    p = __builtin_fmaf(p, q, 1.0f / 13);
-    p = __builtin_fmaf(p, q, 1.0f / 11);
-    p = __builtin_fmaf(p, q, 1.0f / 9);
-    p = __builtin_fmaf(p, q, 1.0f / 7);
-    p = __builtin_fmaf(p, q, 1.0f / 5);
-    p = __builtin_fmaf(p, q, 1.0f / 3);
-    p = p * q;
-    const float l = 2.0f * __builtin_fmaf(p, s, s);
-    return x != x ? x : __builtin_fmaxf(x, 0.0f) + l;
+    float p = 0.281783342f;
+    p = __builtin_fmaf(p, q, 0.279606014f);
+    p = __builtin_fmaf(p, q, 0.400249094f);
+    p = __builtin_fmaf(p, q, 0.66666317f);
+    p = __builtin_fmaf(p, q, 2.0f);
+    return __builtin_fmaf(p, s, __builtin_fmaxf(x, 0.0f));   // (a NaN comes through e)
 }
 
 // V neighbouring channels of one row, as one load or store.

@@ -470,7 +470,7 @@ int scan_check(const ilx_state_space& s, const char* name) {
 // Workgroups per block of channels: enough for four waves a SIMD, each with as many items as the next.
 void share_items(StateSpaceArgs& a, int64_t items) {
     const int64_t waves = 16 * device_cu_count(), most = waves / a.blocks > 0 ? waves / a.blocks : 1, each = (items + most - 1) / most;
-    a.slots = each > 0 ? (items + each - 1) / each : 1;
+    a.slots = each > 0 ? (items + each - 1) / each : 0;
 }
 
 StateSpaceArgs scan_args(const ilx_state_space& s) {

@@ -1,303 +1,378 @@
 // Backward pass of the selective state space recurrence.  With dy the gradient of y (before the gate) and r_t that of h_t,
-//   r_t[n] = dy_t C_t[n] + a_{t+1}[n] r_{t+1}[n],   a_t = exp(dt_t A) (0 at a start),   p_t = a_t h_{t-1},
-//   dB_t[n] = sum_d r dt x,   dC_t[n] = sum_d dy h,   dA[n] = sum_t r p dt,   dx = D dy + dt sum_n r B,
-//   d dt = x sum_n r B + sum_n r p A,   d delta = d dt sigmoid(delta + bias).
+//   r_t[n] = dy_t C_t[n] + a_{t+1}[n] r_{t+1}[n],   a_t = exp(dt_t A) (0 at a start),   q_t = a_t r_t h_{t-1},
+//   dB_t[n] = sum_d r dt x,   dC_t[n] = sum_d dy h,   dA[n] = sum_t q dt,   dx = D dy + dt sum_n r B,
+//   d dt = x sum_n r B + sum_n q A,   d delta = d dt sigmoid(delta + bias).
 // The states are not kept by the forward pass (they are `states` times the inputs); it saves one in ILX_SCAN_BLOCK rows, and a
-// workgroup recomputes a block's forward from there, then walks it backwards.  A workgroup has 64 channels, a lane each, and a
-// wave for every four states, so a lane holds a and p of a whole block in registers (2 x 8 x 4); what is summed over the
-// states (sum r B, sum r p A, y) meets in LDS once per block, and what is summed over the channels (dB, dC) is added across the
-// lanes by a halving exchange: eight values become one register in 8 + 4 + 2 lanes' worth of instructions, not 8 x 6.
+// wave recomputes a block's forward from there, a and h of all its rows in registers, then walks it backwards.
+// A wave holds 16 channels times four quarters of the states: lane l has channel l % 16 and S states from S (l / 16) on.  So
+// everything a row needs stays inside the wave:
+//  * a row's dt, dt x and dy are made once, by the quarter of lanes whose turn the row is, and reach the others through LDS
+//    without a barrier; the same lanes finish the row (dx, d delta, d gate);
+//  * sums over the states (sum r B, sum q A, y) are added over the four quarters for four rows together, by exchanges that leave
+//    each quarter its own row: three exchanges for four sums;
+//  * sums over the channels (dB, dC) are first halved twice inside 16 lanes, each step leaving half of the lanes one value and
+//    half another (twelve adds for eight values, where a plain tree takes 32); what is left, 16 numbers of a workgroup's four waves
+//    (64 channels) to a result, is added from LDS behind the block's one barrier.
 #include "state_space_dev.h"
 
 namespace ilx {
 
 constexpr int kRows = ILX_SCAN_BLOCK;
-constexpr int kStates = 4;   // per wave
+constexpr int kWaves = 4;
+constexpr int kChannels = 16;   // per wave
 constexpr float kLn2 = 0.693147180559945309417f;
+static_assert(kRows == 8, "two sets of four rows");
 
+__device__ __forceinline__ uint32_t bits(float v) { return __builtin_bit_cast(uint32_t, v); }
+__device__ __forceinline__ float number(uint32_t v) { return __builtin_bit_cast(float, v); }
 
+// Lanes below 32 get a folded onto itself, lanes from 32 on b; the same between neighbouring 16 lanes.
+__device__ __forceinline__ float fold32(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane32_swap(bits(a), bits(b), false, false);
+    return number(r[0]) + number(r[1]);
+}
+__device__ __forceinline__ float fold16(float a, float b) {
+    const auto r = __builtin_amdgcn_permlane16_swap(bits(a), bits(b), false, false);
+    return number(r[0]) + number(r[1]);
+}
+// Four rows' sums over the four quarters of the lanes: quarter g gets row g's.
+__device__ __forceinline__ float fold_rows(const float (&v)[4]) { return fold16(fold32(v[0], v[2]), fold32(v[1], v[3])); }
+
+// Inside 16 lanes: lanes 0-7 get a folded onto itself, lanes 8-15 b; inside 8 lanes: 0-3 a, 4-7 b.
+__device__ __forceinline__ float fold8(float a, float b) {
+    float r;
+    asm("s_nop 1\n"
+        "v_add_f32_dpp %0, %1, %1 row_ror:8 row_mask:0xf bank_mask:0x3\n"
+        "v_add_f32_dpp %0, %2, %2 row_ror:8 row_mask:0xf bank_mask:0xc\n"
+        : "=&v"(r)
+        : "v"(a), "v"(b));
+    return r;
+}
+__device__ __forceinline__ float fold4(float a, float b) {
+    float r;
+    asm("s_nop 1\n"
+        "v_add_f32_dpp %0, %1, %1 row_half_mirror row_mask:0xf bank_mask:0x5\n"
+        "v_add_f32_dpp %0, %2, %2 row_half_mirror row_mask:0xf bank_mask:0xa\n"
+        : "=&v"(r)
+        : "v"(a), "v"(b));
+    return r;
+}
+// Of 2 S values per lane: register k, lanes 4 b .. 4 b + 3 of every 16 hold parts of value 4 k + order(b).
+__device__ __forceinline__ constexpr int bank_of(int value) { return (value & 1) * 2 + (value >> 1 & 1); }
+template <int N, int R> __device__ __forceinline__ void halve_twice(const float (&v)[N], float (&out)[R]) {
+    if constexpr (N == 2) {
+        const float t = fold8(v[0], v[1]);
+        out[0] = fold4(t, t);
+    } else {
+#pragma unroll
+        for (int k = 0; k < R; ++k) out[k] = fold4(fold8(v[4 * k], v[4 * k + 1]), fold8(v[4 * k + 2], v[4 * k + 3]));
+    }
+}
+
+// Operands out of lanes: row Q of four, the quarter's own states (state_space_dev.h).
 template <int L> __device__ __forceinline__ float from_lane(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, v), 0x150 + L, 0xf, 0xf, true));
 }
-template <int L> __device__ __forceinline__ void dot_four(float& y, float c, const float (&h)[4]) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-        : "+&v"(y)
-        : "v"(c), "v"(h[0]), "v"(h[1]), "v"(h[2]), "v"(h[3]), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
+// h += values u
+template <int Q, int S, int O> __device__ __forceinline__ void add_outer(float (&h)[S], const float (&values)[O], float u) {
+    if constexpr (S >= 4) {
+#pragma unroll
+        for (int m = 0; m < O; ++m) {
+            f32x4 c = {h[4 * m], h[4 * m + 1], h[4 * m + 2], h[4 * m + 3]};
+            c = __builtin_amdgcn_mfma_f32_4x4x1f32(values[m], u, c, 2, Q, 0);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) h[4 * m + j] = c[j];
+        }
+    } else {
+        static_for<S>([&](auto j) { h[j] = __builtin_fmaf(from_lane<4 * Q + j>(values[0]), u, h[j]); });
+    }
 }
-template <int L> __device__ __forceinline__ void add_four(float (&r)[4], float c, float x) {
-    asm("s_nop 1\n"
-        "v_fmac_f32_dpp %0, %4, %5 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %1, %4, %5 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %2, %4, %5 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
-        "v_fmac_f32_dpp %3, %4, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
-        : "+&v"(r[0]), "+&v"(r[1]), "+&v"(r[2]), "+&v"(r[3])
-        : "v"(c), "v"(x), "n"(L), "n"(L + 1), "n"(L + 2), "n"(L + 3));
-}
-
-template <int CTRL> __device__ __forceinline__ float dpp_add(float v) {
-    const int o = __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xf, 0xf, true);
-    return v + __builtin_bit_cast(float, o);
-}
-
-// {a.lower half, b.lower half} + {a.upper half, b.upper half}: in the lower 32 lanes a folded onto itself, in the upper b.
-__device__ __forceinline__ float fold32(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane32_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
-    return __builtin_bit_cast(float, static_cast<unsigned>(r[0])) + __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
-}
-// the same between the rows of 16 lanes: even rows keep a, odd rows b
-__device__ __forceinline__ float fold16(float a, float b) {
-    const auto r = __builtin_amdgcn_permlane16_swap(__builtin_bit_cast(unsigned, a), __builtin_bit_cast(unsigned, b), false, false);
-    return __builtin_bit_cast(float, static_cast<unsigned>(r[0])) + __builtin_bit_cast(float, static_cast<unsigned>(r[1]));
-}
-
-// The sums over the 64 lanes of eight values: lane l gets the one numbered bit 5 of l + 2 * bit 4 + 4 * bit 3.
-__device__ __forceinline__ float sum_lanes(const float (&v)[8], int lane) {
-    const float a = fold16(fold32(v[0], v[1]), fold32(v[2], v[3]));
-    const float b = fold16(fold32(v[4], v[5]), fold32(v[6], v[7]));
-    const float a8 = dpp_add<0x128>(a), b8 = dpp_add<0x128>(b);   // row_ror:8
-    float s = lane & 8 ? b8 : a8;
-    s = dpp_add<0x141>(s);   // row_half_mirror: lane i and 7 - i
-    s = dpp_add<0x4e>(s);    // quad_perm 2,3,0,1
-    return dpp_add<0xb1>(s); // quad_perm 1,0,3,2
+// sum of values h over the lane's states
+template <int Q, int S, int O> __device__ __forceinline__ float dot_quarter(const float (&values)[O], const float (&h)[S]) {
+    float y = 0.0f;
+    if constexpr (S < 4) {
+        static_for<S>([&](auto j) { y = __builtin_fmaf(from_lane<4 * Q + j>(values[0]), h[j], y); });
+    } else {
+#pragma unroll
+        for (int m = 0; m < O; ++m)
+            asm(ILX_WAIT
+                "v_fmac_f32_dpp %0, %1, %2 row_newbcast:%6 row_mask:0xf bank_mask:0xf\n"
+                "v_fmac_f32_dpp %0, %1, %3 row_newbcast:%7 row_mask:0xf bank_mask:0xf\n"
+                "v_fmac_f32_dpp %0, %1, %4 row_newbcast:%8 row_mask:0xf bank_mask:0xf\n"
+                "v_fmac_f32_dpp %0, %1, %5 row_newbcast:%9 row_mask:0xf bank_mask:0xf\n"
+                "s_nop 1\n"   // (an exchange between lanes may not read it sooner)
+                : "+&v"(y)
+                : "v"(values[m]), "v"(h[4 * m]), "v"(h[4 * m + 1]), "v"(h[4 * m + 2]), "v"(h[4 * m + 3]), "n"(4 * Q), "n"(4 * Q + 1), "n"(4 * Q + 2),
+                  "n"(4 * Q + 3));
+    }
+    return y;
 }
 
 // A block of rows of one part of a sequence.
 struct ScanBlock {
-    int64_t item, b, begin, end, t0;   // begin .. end: the part's rows that exist
+    int item, b, begin, end, t0;   // begin .. end: the part's rows that exist
     int count;
 };
 
-template <typename T, typename TB, int NW>
-__global__ void __launch_bounds__(64 * NW, 3) scan_backward_kernel(StateSpaceArgs a) {
-    constexpr int E = kRows / NW;   // rows a wave prepares and finishes per block
-    __shared__ float2 s_step[2][kRows][64];       // dt and dt x, of this block and the one before
-    __shared__ float s_dy[2][kRows][64];
-    __shared__ float2 s_sum[NW][kRows][64];       // sum r B and sum r p A log2 e over the wave's states
-    __shared__ float s_y[NW][kRows][64];
-    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), n0 = w * kStates;
-    const int block = blockIdx.x % a.blocks;
-    const int64_t slot = blockIdx.x / a.blocks;
-    const ChannelLane c = channel_lane(a, block, lane);
-    const int group_block = block - c.group * a.group_blocks;
+template <typename T, typename TB, int S>
+__global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_kernel(StateSpaceArgs a) {
+    constexpr int O = (S + 3) / 4, R = S / 2 > 0 ? S / 2 : 1;
+    __shared__ float4 s_row[kWaves][kRows][kChannels];   // dt, dt x, dy
+    __shared__ float s_part[2][kWaves][R][kRows][64];    // halved sums of this block and the one before
+    const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
+    const int block = blockIdx.x % a.blocks, slot = blockIdx.x / a.blocks;
+    const int group = block / a.group_blocks, group_block = block - group * a.group_blocks;
+    const int within = group_block * 64 + w * kChannels + (lane & 15);
+    const bool active = within < a.group_channels;
+    const int d = group * a.group_channels + (active ? within : a.group_channels - 1);
     const ilx_state_space& s = a.s;
-    const int64_t channels = s.channels, items = s.batch * a.parts;
-    float A2[kStates], dA[kStates];   // A2 = A log2 e
+    const int states = s.states, channels = s.channels, items = static_cast<int>(s.batch * a.parts);
+    const bool gated = s.gate != nullptr;
+    float A2[S], dA[S];   // A2 = A log2 e
 #pragma unroll
-    for (int n = 0; n < kStates; ++n) {
-        const bool in = n0 + n < s.states;
-        A2[n] = in ? s.A[static_cast<int64_t>(c.d) * s.states + n0 + n] * kLog2e : 0.0f;
-        dA[n] = 0.0f;
+    for (int j = 0; j < S; ++j) {
+        const int n = S * quarter + j;
+        A2[j] = n < states ? s.A[static_cast<int64_t>(d) * states + n] * kLog2e : 0.0f;
+        dA[j] = 0.0f;
     }
-    const float bias = s.delta_bias ? s.delta_bias[c.d] : 0.0f, skip = s.D ? s.D[c.d] : 0.0f;
+    const float bias = s.delta_bias ? s.delta_bias[d] : 0.0f, skip = s.D ? s.D[d] : 0.0f;
     float dD = 0.0f, dbias = 0.0f;
-    const int value = (lane >> 5 & 1) + 2 * (lane >> 4 & 1) + 4 * (lane >> 3 & 1);   // what sum_lanes leaves here
-    const int shared_column = (value >> 2) * (NW * kStates) + n0 + (value & 3);
-    // B and C of four rows and the wave's four states in every 16 lanes
-    const int bc_row = lane >> 2 & 3, bc_state = n0 + (lane & 3);
-    const bool bc_in = bc_state < s.states;
-    const int bc_at = bc_in ? bc_state : s.states - 1;
-    const uint32_t parts = static_cast<uint32_t>(a.parts);
+    // where the lane's values are: its channel, its quarter's states (clamped to the last), its element of the operands
+    const uint32_t channel = static_cast<uint32_t>(d) * sizeof(T);
+    uint32_t state_at[S];
+#pragma unroll
+    for (int j = 0; j < S; ++j) state_at[j] = (static_cast<uint32_t>(S * quarter + j < states ? S * quarter + j : states - 1) * channels + d) * 4;
+    uint32_t operand_at[O], operand_mask[O];
+#pragma unroll
+    for (int m = 0; m < O; ++m) {
+        const int i = 4 * m + (lane & 3), n = S * quarter + (i < S ? i : S - 1);
+        operand_at[m] = (n < states ? n : states - 1) * sizeof(TB);
+        operand_mask[m] = i < S && n < states ? ~0u : 0u;
+    }
 
     // the last block of an item, with count 0 if the item has no rows
-    auto item_end = [&](int64_t item) {
+    auto item_end = [&](int item) {
+        const ArgsPtr p = arguments_again();
+        const int parts = static_cast<int>(p->parts), part_rows = static_cast<int>(p->part_rows);
         ScanBlock k;
-        k.item = item, k.b = static_cast<uint32_t>(item) / parts, k.begin = static_cast<uint32_t>(item) % parts * a.part_rows;
-        const int64_t len = scan_length(s, k.b);
-        k.end = k.begin + a.part_rows < len ? k.begin + a.part_rows : len;
+        k.item = item, k.b = item / parts, k.begin = (item - k.b * parts) * part_rows;
+        int len = static_cast<int>(p->s.length);
+        if (p->s.lengths) {
+            const int n = uni(p->s.lengths[k.b]);
+            len = n < 0 ? 0 : (n < len ? n : len);
+        }
+        k.end = k.begin + part_rows < len ? k.begin + part_rows : len;
         k.t0 = k.begin < k.end ? k.begin + (k.end - k.begin - 1) / kRows * kRows : k.begin;
-        k.count = k.begin < k.end ? static_cast<int>(k.end - k.t0) : 0;
+        k.count = k.begin < k.end ? k.end - k.t0 : 0;
         return k;
     };
     // a block's inputs, read while the block ahead of it in this order is worked on
-    T in_d[E], in_x[E], in_g[E], in_z[E];
-    TB in_B[kRows / 4], in_C[kRows / 4];
-    float in_h[kStates];
-    uint64_t in_starts = 0;
+    T in_d[2], in_x[2], in_g[2], in_z[2];
+    TB in_B[2][O], in_C[2][O];
+    float in_h[S];
+    uint32_t in_starts = 0;
     auto read = [&](const ScanBlock& k) {
-        const T* px = static_cast<const T*>(s.x) + k.b * s.x_batch;
-        const T* pd = static_cast<const T*>(s.delta) + k.b * s.delta_batch;
-        const T* pz = static_cast<const T*>(s.gate) + k.b * s.gate_batch;
-        const T* pg = static_cast<const T*>(s.grad_out) + k.b * s.grad_out_batch;
-        const TB* pB = static_cast<const TB*>(s.B) + k.b * s.B_batch + c.group * s.states;
-        const TB* pC = static_cast<const TB*>(s.C) + k.b * s.C_batch + c.group * s.states;
+        const ArgsPtr p = arguments_again();
+        Stream<T> x, delta, gate, grad;
+        Stream<TB> B, C;
+        x.set(p->s.x, k.b * p->s.x_batch, k.t0, p->s.x_time);
+        delta.set(p->s.delta, k.b * p->s.delta_batch, k.t0, p->s.delta_time);
+        grad.set(p->s.grad_out, k.b * p->s.grad_out_batch, k.t0, p->s.grad_out_time);
+        B.set(p->s.B, k.b * p->s.B_batch + group * p->s.states, k.t0, p->s.B_time);
+        C.set(p->s.C, k.b * p->s.C_batch + group * p->s.states, k.t0, p->s.C_time);
+        if (p->s.gate)
+            gate.set(p->s.gate, k.b * p->s.gate_batch, k.t0, p->s.gate_time);
+        else
+            gate = grad;   // (read and not used)
 #pragma unroll
-        for (int e = 0; e < E; ++e) {
-            const int i = e * NW + w;
-            const uint32_t t = static_cast<uint32_t>(k.t0 + (i < k.count ? i : k.count - 1));
-            in_d[e] = (pd + row_offset(t, s.delta_time))[c.d];
-            in_x[e] = (px + row_offset(t, s.x_time))[c.d];
-            in_g[e] = (pg + row_offset(t, s.grad_out_time))[c.d];
-            if (s.gate) in_z[e] = (pz + row_offset(t, s.gate_time))[c.d];
+        for (int e = 0; e < 2; ++e) {
+            const uint32_t row = 4 * e + quarter < k.count ? 4 * e + quarter : k.count - 1;
+            in_d[e] = lane_load<T>(delta.buffer(), row * delta.time + channel, 0);
+            in_x[e] = lane_load<T>(x.buffer(), row * x.time + channel, 0);
+            in_g[e] = lane_load<T>(grad.buffer(), row * grad.time + channel, 0);
+            in_z[e] = lane_load<T>(gate.buffer(), row * gate.time + channel, 0);
+            const int q = 4 * e + (lane >> 2 & 3);
+            const uint32_t operand_row = q < k.count ? q : k.count - 1;
+#pragma unroll
+            for (int m = 0; m < O; ++m) {
+                in_B[e][m] = lane_load<TB>(B.buffer(), operand_row * B.time + operand_at[m], 0);
+                in_C[e][m] = lane_load<TB>(C.buffer(), operand_row * C.time + operand_at[m], 0);
+            }
         }
+        const auto save = row_buffer(p->s.saved + (k.b * p->saved_blocks + k.t0 / kRows) * (static_cast<int64_t>(p->s.states) * p->s.channels));
 #pragma unroll
-        for (int j = 0; j < kRows / 4; ++j) {
-            const int i = 4 * j + bc_row;
-            const uint32_t t = static_cast<uint32_t>(k.t0 + (i < k.count ? i : k.count - 1));
-            in_B[j] = pB[row_offset(t, s.B_time) + bc_at];
-            in_C[j] = pC[row_offset(t, s.C_time) + bc_at];
+        for (int j = 0; j < S; ++j) in_h[j] = lane_load<float>(save, state_at[j], 0);
+        in_starts = 0;
+        if (p->s.starts) {
+            const uint8_t* from = p->s.starts + k.b * p->s.starts_batch + k.t0 * p->s.starts_time;
+            bool on = false;
+            if (lane < k.count) on = from[lane * p->s.starts_time] != 0;
+            in_starts = static_cast<uint32_t>(__ballot(on));
         }
-        const float* save = s.saved + (k.b * a.saved_blocks + k.t0 / kRows) * s.states * channels;
-#pragma unroll
-        for (int n = 0; n < kStates; ++n) in_h[n] = (save + (n0 + n < s.states ? n0 + n : s.states - 1) * channels)[c.d];
-        in_starts = start_bits(s, k.b, k.t0, k.count, lane);
     };
 
     ScanBlock k = item_end(slot);
     if (k.count > 0) read(k);
-    float r[kStates];
+    float r[S];
     bool fresh = true;
     int buffer = 0;
     while (k.item < items) {
         if (fresh) {   // the item's last block: what enters the part from behind, and zeros for the rows that do not exist
-            const float* enters = a.parts > 1 ? a.part_state + k.item * s.states * channels : s.grad_last ? s.grad_last + k.b * s.states * channels : nullptr;
+            const ArgsPtr p = arguments_again();
+            const int64_t size = static_cast<int64_t>(p->s.states) * p->s.channels;
+            const float* enters = p->parts > 1 ? p->part_state + k.item * size : p->s.grad_last ? p->s.grad_last + k.b * size : nullptr;
 #pragma unroll
-            for (int n = 0; n < kStates; ++n) r[n] = enters && c.active && n0 + n < s.states ? (enters + (n0 + n) * channels)[c.d] : 0.0f;
-            const int64_t limit = k.begin + a.part_rows < s.length ? k.begin + a.part_rows : s.length;
-            for (int64_t t = (k.end > k.begin ? k.end : k.begin) + w; t < limit; t += NW) {
-                const int64_t at = k.b * s.grad_batch + t * s.grad_time + c.d;
-                if (!c.active) break;
-                static_cast<T*>(s.grad_x)[at] = from_f32<T>(0.0f);
-                static_cast<T*>(s.grad_delta)[at] = from_f32<T>(0.0f);
-                if (s.gate) static_cast<T*>(s.grad_gate)[at] = from_f32<T>(0.0f);
+            for (int j = 0; j < S; ++j) r[j] = 0.0f;
+            if (enters) {
+                const auto from = row_buffer(enters);
+#pragma unroll
+                for (int j = 0; j < S; ++j) r[j] = active && S * quarter + j < states ? lane_load<float>(from, state_at[j], 0) : 0.0f;
+            }
+            const int length = static_cast<int>(p->s.length), part_rows = static_cast<int>(p->part_rows), limit = k.begin + part_rows < length ? k.begin + part_rows : length;
+            for (int t = (k.end > k.begin ? k.end : k.begin) + quarter; t < limit; t += 4) {
+                const int64_t at = k.b * p->s.grad_batch + t * p->s.grad_time + d;
+                if (!active) break;
+                static_cast<T*>(p->s.grad_x)[at] = from_f32<T>(0.0f);
+                static_cast<T*>(p->s.grad_delta)[at] = from_f32<T>(0.0f);
+                if (gated) static_cast<T*>(p->s.grad_gate)[at] = from_f32<T>(0.0f);
             }
         }
         ScanBlock next = k;
         if (k.t0 > k.begin) {
             next.t0 = k.t0 - kRows, next.count = kRows;
-        } else if (k.item + a.slots < items) {
-            next = item_end(k.item + a.slots);
+        } else if (k.item + static_cast<int>(a.slots) < items) {
+            next = item_end(k.item + static_cast<int>(a.slots));
         } else {
             next.item = items, next.count = 0;
         }
         if (k.count > 0) {
             // rows past the end act as rows that leave the state alone: dt = x = dy = 0
-            float slope[E], dgate[E], x[E];
+            float slope[2], dgate[2], x[2], dt[2], dy[2];
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = e * NW + w;
-                const bool in = i < k.count && c.active;
+            for (int e = 0; e < 2; ++e) {
+                const bool in = 4 * e + quarter < k.count && active;
                 const float raw = to_f32(in_d[e]) + bias, g = to_f32(in_g[e]);
                 x[e] = in ? to_f32(in_x[e]) : 0.0f;
-                float dy = g;
-                dgate[e] = 0.0f;
-                if (s.gate) {
+                dy[e] = g, dgate[e] = 0.0f, slope[e] = 1.0f, dt[e] = raw;
+                if (gated) {
                     const float z = to_f32(in_z[e]), sig = sigmoid_fast(z);
-                    dy = g * z * sig;
+                    dy[e] = g * z * sig;
                     dgate[e] = g * sig * __builtin_fmaf(z, 1.0f - sig, 1.0f);
                 }
-                slope[e] = s.softplus ? sigmoid_fast(raw) : 1.0f;
-                const float dt = in ? (s.softplus ? softplus_f(raw) : raw) : 0.0f;
-                s_step[buffer][i][lane] = make_float2(dt, dt * x[e]);
-                s_dy[buffer][i][lane] = in ? dy : 0.0f;
+                if (s.softplus) slope[e] = sigmoid_fast(raw), dt[e] = softplus_f(raw);
+                dy[e] = in ? dy[e] : 0.0f, dt[e] = in ? dt[e] : 0.0f;
+                s_row[w][4 * e + quarter][lane & 15] = make_float4(dt[e], dt[e] * x[e], dy[e], 0.0f);
             }
-            float B[kRows / 4], C[kRows / 4], h0[kStates], decay[kRows][kStates], h[kRows][kStates];
+            float B[2][O], C[2][O], h0[S], decay[kRows][S], h[kRows][S];
 #pragma unroll
-            for (int j = 0; j < kRows / 4; ++j) B[j] = bc_in ? to_f32(in_B[j]) : 0.0f, C[j] = bc_in ? to_f32(in_C[j]) : 0.0f;
+            for (int e = 0; e < 2; ++e)
 #pragma unroll
-            for (int n = 0; n < kStates; ++n) h0[n] = n0 + n < s.states ? in_h[n] : 0.0f;
-            const uint64_t starts = in_starts;
-            __syncthreads();
+                for (int m = 0; m < O; ++m) B[e][m] = masked(to_f32(in_B[e][m]), operand_mask[m]), C[e][m] = masked(to_f32(in_C[e][m]), operand_mask[m]);
+#pragma unroll
+            for (int j = 0; j < S; ++j) h0[j] = in_h[j];
+            const uint32_t starts = in_starts;
             if (next.count > 0) read(next);
-            float kept = 0.0f;
+            float y[2], rb[2], ra[2];
             auto walk = [&](auto with_starts) {
+                float four[4], four_a[4];
                 static_for<kRows>([&](auto row) {
                     constexpr int i = row;
-                    __builtin_amdgcn_sched_barrier(0);
-                    const float2 v = s_step[buffer][i][lane];
+                    const float4 v = s_row[w][i][lane & 15];
                     const bool start = decltype(with_starts)::value && (starts >> i & 1);
-                    static_for<kStates>([&](auto state) {
-                        constexpr int n = state;
-                        const float before = i == 0 ? h0[n] : h[i == 0 ? 0 : i - 1][n];
-                        const float e = __builtin_amdgcn_exp2f(v.x * A2[n]);
-                        decay[i][n] = start ? 0.0f : e;
-                        h[i][n] = __builtin_fmaf(decay[i][n], start ? 0.0f : before, v.y * from_lane<4 * (i & 3) + n>(B[i >> 2]));
-                    });
-                    float y = 0.0f;
-                    dot_four<4 * (i & 3)>(y, C[i >> 2], h[i]);
-                    s_y[w][i][lane] = y;
+#pragma unroll
+                    for (int j = 0; j < S; ++j) {
+                        const float before = i == 0 ? h0[j] : h[i == 0 ? 0 : i - 1][j], e = __builtin_amdgcn_exp2f(v.x * A2[j]);
+                        decay[i][j] = start ? 0.0f : e;
+                        h[i][j] = decay[i][j] * (start ? 0.0f : before);
+                    }
+                    add_outer<(i & 3)>(h[i], B[i >> 2], v.y);
+                    four[i & 3] = dot_quarter<(i & 3)>(C[i >> 2], h[i]);
+                    if constexpr ((i & 3) == 3) y[i >> 2] = fold_rows(four);
                 });
-                uint64_t starts_again = starts;   // (kept apart: the compiler would hold what the two walks share in registers)
+                uint32_t starts_again = starts;   // (kept apart: the compiler would hold what the two walks share in registers)
                 asm volatile("" : "+s"(starts_again) : : "memory");
                 static_for<kRows>([&](auto row) {
                     constexpr int i = kRows - 1 - row;
-                    __builtin_amdgcn_sched_barrier(0);
-                    const float2 u = s_step[buffer][i][lane];
-                    const float dy = s_dy[buffer][i][lane];
+                    const float4 u = s_row[w][i][lane & 15];
                     const bool start = decltype(with_starts)::value && (starts_again >> i & 1);
-                    float v[2 * kStates], rb = 0.0f, ra = 0.0f;
-                    add_four<4 * (i & 3)>(r, C[i >> 2], dy);
-                    dot_four<4 * (i & 3)>(rb, B[i >> 2], r);
-                    static_for<kStates>([&](auto state) {
-                        constexpr int n = state;
-                        v[n] = r[n] * u.y;
-                        v[kStates + n] = dy * h[i][n];
-                        r[n] = start ? 0.0f : r[n] * decay[i][n];
-                        const float q = r[n] * (start ? 0.0f : i == 0 ? h0[n] : h[i == 0 ? 0 : i - 1][n]);
-                        ra = __builtin_fmaf(q, A2[n], ra);
-                        dA[n] = __builtin_fmaf(q, u.x, dA[n]);
-                    });
-                    s_sum[w][i][lane] = make_float2(rb, ra);
-                    const float sum = sum_lanes(v, lane);
-                    kept = (lane & 7) == i ? sum : kept;
+                    float v[2 * S], sums[R];
+                    add_outer<(i & 3)>(r, C[i >> 2], u.z);
+                    four[i & 3] = dot_quarter<(i & 3)>(B[i >> 2], r);
+                    four_a[i & 3] = 0.0f;
+#pragma unroll
+                    for (int j = 0; j < S; ++j) {
+                        v[j] = r[j] * u.y;
+                        v[S + j] = u.z * h[i][j];
+                        r[j] = start ? 0.0f : r[j] * decay[i][j];
+                        const float q = r[j] * (start ? 0.0f : i == 0 ? h0[j] : h[i == 0 ? 0 : i - 1][j]);
+                        four_a[i & 3] = __builtin_fmaf(q, A2[j], four_a[i & 3]);
+                        dA[j] = __builtin_fmaf(q, u.x, dA[j]);
+                    }
+                    halve_twice(v, sums);
+#pragma unroll
+                    for (int m = 0; m < R; ++m) s_part[buffer][w][m][i][lane] = sums[m];
+                    if constexpr ((i & 3) == 0) rb[i >> 2] = fold_rows(four), ra[i >> 2] = fold_rows(four_a);
                 });
             };
             if (starts)
                 walk(std::true_type{});
             else
                 walk(std::false_type{});
-            if ((lane & 7) < k.count) {
-                const int64_t at = ((group_block * s.batch + k.b) * s.length + k.t0 + (lane & 7)) * s.groups + c.group;
-                a.shared[at * (2 * NW * kStates) + shared_column] = kept;
-            }
-            __syncthreads();
+            {
+                const ArgsPtr p = arguments_again();
+                const uint32_t time = static_cast<uint32_t>(p->s.grad_time) * sizeof(T);
+                const int64_t at = k.b * p->s.grad_batch + static_cast<int64_t>(k.t0) * p->s.grad_time;
 #pragma unroll
-            for (int e = 0; e < E; ++e) {
-                const int i = e * NW + w;
-                if (i < k.count && c.active) {
-                    float rb = 0.0f, ra = 0.0f, y = 0.0f;
-#pragma unroll
-                    for (int j = 0; j < NW; ++j) {
-                        const float2 v = s_sum[j][i][lane];
-                        rb += v.x, ra += v.y;
-                        y += s_y[j][i][lane];
+                for (int e = 0; e < 2; ++e) {
+                    const int i = 4 * e + quarter;
+                    if (i < k.count && active) {
+                        const float draw = __builtin_fmaf(x[e], rb[e], ra[e] * kLn2) * slope[e];
+                        const uint32_t to = i * time + channel;
+                        lane_store<T>(row_buffer(static_cast<T*>(p->s.grad_x) + at), to, 0, from_f32<T>(__builtin_fmaf(dt[e], rb[e], skip * dy[e])));
+                        lane_store<T>(row_buffer(static_cast<T*>(p->s.grad_delta) + at), to, 0, from_f32<T>(draw));
+                        if (gated) lane_store<T>(row_buffer(static_cast<T*>(p->s.grad_gate) + at), to, 0, from_f32<T>(dgate[e] * __builtin_fmaf(skip, x[e], y[e])));
+                        dD = __builtin_fmaf(dy[e], x[e], dD);
+                        dbias += draw;
                     }
-                    const float dt = s_step[buffer][i][lane].x, dy = s_dy[buffer][i][lane], draw = __builtin_fmaf(x[e], rb, ra * kLn2) * slope[e];
-                    const int64_t at = k.b * s.grad_batch + row_offset(static_cast<uint32_t>(k.t0 + i), s.grad_time);
-                    (static_cast<T*>(s.grad_x) + at)[c.d] = from_f32<T>(__builtin_fmaf(dt, rb, skip * dy));
-                    (static_cast<T*>(s.grad_delta) + at)[c.d] = from_f32<T>(draw);
-                    if (s.gate) (static_cast<T*>(s.grad_gate) + at)[c.d] = from_f32<T>(dgate[e] * __builtin_fmaf(skip, x[e], y));
-                    dD = __builtin_fmaf(dy, x[e], dD);
-                    dbias += draw;
                 }
             }
-            buffer ^= 1;   // (the next block's rows go where nobody still reads; its sums are written behind a barrier)
+            __syncthreads();
+            // dB and dC of the block's rows over the workgroup's channels
+            float* to = a.shared + ((static_cast<int64_t>(group_block) * s.batch + k.b) * s.length + k.t0) * s.groups * (8 * S);
+            for (int o = threadIdx.x; o < k.count * 8 * S; o += 64 * kWaves) {
+                const int i = o / (8 * S), value = o - i * (8 * S), n = value % (4 * S), v = value / (4 * S) * S + n % S;
+                const int at = 16 * (n / S) + 4 * bank_of(v & 3);
+                float sum = 0.0f;
+#pragma unroll
+                for (int m = 0; m < kWaves; ++m) {
+                    const float4 q = *reinterpret_cast<const float4*>(&s_part[buffer][m][v >> 2][i][at]);
+                    sum += (q.x + q.y) + (q.z + q.w);
+                }
+                to[(static_cast<int64_t>(i) * s.groups + group) * (8 * S) + value] = sum;
+            }
+            buffer ^= 1;   // (this one is written again behind the next block's barrier)
         } else if (next.count > 0) {
             read(next);
         }
         fresh = next.item != k.item;
-        if (fresh && k.begin == 0 && s.grad_state && c.active) {
+        if (fresh && k.begin == 0 && s.grad_state && active) {
 #pragma unroll
-            for (int n = 0; n < kStates; ++n)
-                if (n0 + n < s.states) (s.grad_state + (k.b * s.states + n0 + n) * channels)[c.d] = r[n];
+            for (int j = 0; j < S; ++j)
+                if (S * quarter + j < states) s.grad_state[k.b * static_cast<int64_t>(states) * channels + (state_at[j] >> 2)] = r[j];
         }
         k = next;
     }
-    __syncthreads();
-    s_sum[0][w][lane] = make_float2(dD, dbias);
-    __syncthreads();
-    if (!c.active) return;
-    float* sums = a.sums + slot * (s.states + 2) * channels;
+    // the workgroup's part of the parameters' gradients
+    dD = fold32(dD, dD), dbias = fold32(dbias, dbias);
+    dD = fold16(dD, dD), dbias = fold16(dbias, dbias);
+    if (!active) return;
+    float* sums = a.sums + static_cast<int64_t>(slot) * (states + 2) * channels;
 #pragma unroll
-    for (int n = 0; n < kStates; ++n)
-        if (n0 + n < s.states) sums[(n0 + n) * channels + c.d] = dA[n];
-    if (w == 0) {
-        for (int j = 1; j < NW; ++j) dD += s_sum[0][j][lane].x, dbias += s_sum[0][j][lane].y;
-        sums[s.states * channels + c.d] = dD;
-        sums[(s.states + 1) * channels + c.d] = dbias;
+    for (int j = 0; j < S; ++j)
+        if (S * quarter + j < states) sums[state_at[j] >> 2] = dA[j];
+    if (quarter == 0) {
+        sums[static_cast<int64_t>(states) * channels + d] = dD;
+        sums[static_cast<int64_t>(states + 1) * channels + d] = dbias;
     }
 }
 
@@ -326,35 +401,34 @@ using namespace ilx;
 
 namespace {
 
-int waves_for(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : 8; }
+int lane_states(int states) { return states <= 4 ? 1 : states <= 8 ? 2 : states <= 16 ? 4 : 8; }
 
 StateSpaceArgs backward_args(const ilx_state_space& s, int64_t* floats) {
     StateSpaceArgs a = scan_args(s);
     const int64_t part_floats = divide_scan(a, s.workspace);
-    const int64_t most = 2048 / a.blocks > 0 ? 2048 / a.blocks : 1, items = s.batch * a.parts;
-    a.slots = items < most ? items : most;
+    // two workgroups in turn where three are resident, each with as many sequences as the next
+    const int64_t items = s.batch * a.parts, wanted = 6 * device_cu_count(), most = wanted / a.blocks > 0 ? wanted / a.blocks : 1;
+    const int64_t each = (items + most - 1) / most;
+    a.slots = each > 0 ? (items + each - 1) / each : 0;
     const int64_t sums = a.slots * (s.states + 2) * s.channels;
-    const int64_t shared = a.group_blocks * s.batch * s.length * s.groups * 2 * waves_for(s.states) * kStates;
+    const int64_t shared = a.group_blocks * s.batch * s.length * s.groups * 8 * lane_states(s.states);
     a.sums = s.workspace + part_floats;
     a.shared = a.sums + sums;
     *floats = part_floats + sums + shared;
     return a;
 }
 
-template <typename T, typename TB, int NW> void backward_launch(const StateSpaceArgs& a, hipStream_t s) {
-    ILX_LAUNCH((scan_backward_kernel<T, TB, NW>), dim3(static_cast<unsigned>(a.slots * a.blocks)), dim3(64 * NW), 0, s, a);
-}
-
 template <typename T, typename TB> void backward_states(const StateSpaceArgs& a, hipStream_t s) {
-    const int waves = waves_for(a.s.states);
-    switch (waves) {
-        case 1: backward_launch<T, TB, 1>(a, s); break;
-        case 2: backward_launch<T, TB, 2>(a, s); break;
-        case 4: backward_launch<T, TB, 4>(a, s); break;
-        default: backward_launch<T, TB, 8>(a, s); break;
+    const dim3 grid(static_cast<unsigned>(a.slots * a.blocks)), threads(64 * kWaves);
+    const int each = lane_states(a.s.states);
+    switch (each) {
+        case 1: ILX_LAUNCH((scan_backward_kernel<T, TB, 1>), grid, threads, 0, s, a); break;
+        case 2: ILX_LAUNCH((scan_backward_kernel<T, TB, 2>), grid, threads, 0, s, a); break;
+        case 4: ILX_LAUNCH((scan_backward_kernel<T, TB, 4>), grid, threads, 0, s, a); break;
+        default: ILX_LAUNCH((scan_backward_kernel<T, TB, 8>), grid, threads, 0, s, a); break;
     }
     const int64_t values = a.s.batch * a.s.length * a.s.groups * a.s.states;
-    if (values > 0) ILX_LAUNCH((scan_shared_sums_kernel<TB>), dim3(blocks_for(values)), dim3(256), 0, s, a, waves * kStates);
+    if (values > 0) ILX_LAUNCH((scan_shared_sums_kernel<TB>), dim3(blocks_for(values)), dim3(256), 0, s, a, 4 * each);
 }
 
 }  // namespace
@@ -385,7 +459,7 @@ extern "C" int ilx_state_space_backward(const ilx_state_space* scan, void* strea
     const StateSpaceArgs a = backward_args(s, &needed);
     ILX_REQUIRE(s.workspace_floats >= needed && (s.workspace || needed == 0), ILX_EINVAL,
                 "ilx_state_space_backward: workspace of %lld floats, %lld needed", (long long)s.workspace_floats, (long long)needed);
-    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX && s.batch * s.length * s.groups * s.states / 256 < INT32_MAX, ILX_ESHAPE,
+    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX - 65536 && s.batch * s.length * s.groups * s.states / 256 < INT32_MAX, ILX_ESHAPE,
                 "ilx_state_space_backward: shape too large for one launch");
     hipStream_t st = as_stream(stream);
     if (s.batch > 0) {
