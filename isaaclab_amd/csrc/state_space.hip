@@ -66,7 +66,7 @@ template <typename T, typename TB> struct ScanStreams {
 template <typename T, typename TB, int W, bool WITH_GATE, bool WITH_DOT> struct ScanRows {
     T x[kScanRows], delta[kScanRows], gate[kScanRows];
     TB o[W], c[kScanRows][W];
-    uint32_t starts;
+    uint8_t start;   // of row `lane`
 
     // channel: the lane's channel, o_state, c_state: its states of the operands of `outer` and `dot`, all in bytes
     __device__ __forceinline__ void read(const ScanStreams<T, TB>& k, uint32_t channel, const uint32_t (&o_state)[W], const uint32_t (&c_state)[W], int lane) {
@@ -87,13 +87,10 @@ template <typename T, typename TB, int W, bool WITH_GATE, bool WITH_DOT> struct 
         const uint32_t row = (at < count ? at : count - 1) * k.o.time;
 #pragma unroll
         for (int j = 0; j < W; ++j) o[j] = lane_load<TB>(bo, row + o_state[j], 0);
-        starts = 0;
-        if (k.flags & kHasStarts) {
-            bool on = false;
-            if (lane < count) on = k.starts.p[lane * k.starts.time] != 0;
-            starts = static_cast<uint32_t>(__ballot(on));
-        }
+        start = 0;
+        if ((k.flags & kHasStarts) && lane < count) start = k.starts.p[lane * k.starts.time];
     }
+    __device__ __forceinline__ uint32_t starts() const { return static_cast<uint32_t>(__ballot(start != 0)); }   // a bit a row
 };
 
 // A start: a branch of its own, taken rarely, and no selects on the way past it.
@@ -228,7 +225,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_forward_kernel(StateSpac
             }
 #pragma unroll
             for (int j = 0; j < W; ++j) B[j] = masked(to_f32(rows.o[j]), shared.o_mask[j]);
-            const uint32_t starts = rows.starts;
+            const uint32_t starts = rows.starts();
             if (t0 + kScanRows < end) {
                 k.template step<false>();
                 rows.read(k, channel, shared.o, shared.c, lane);
@@ -326,7 +323,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_part_kernel(StateSpaceAr
             }
 #pragma unroll
             for (int j = 0; j < W; ++j) M[j] = masked(to_f32(rows.o[j]), shared.o_mask[j]);
-            const uint32_t starts = rows.starts;
+            const uint32_t starts = rows.starts();
             any = any || starts != 0;
             const bool more = REVERSE ? k.t0 > k.begin : k.t0 + kScanRows < k.end;
             if (more) {

@@ -108,6 +108,14 @@ template <int Q, int S, int O> __device__ __forceinline__ float dot_quarter(cons
     return y;
 }
 
+// The state ahead of row I of a block.
+template <int I, int S> __device__ __forceinline__ float before(const float (&h0)[S], const float (&h)[kRows][S], int j) {
+    if constexpr (I == 0)
+        return h0[j];
+    else
+        return h[I - 1][j];
+}
+
 // A block of rows of one part of a sequence.
 struct ScanBlock {
     int item, b, begin, end, t0;   // begin .. end: the part's rows that exist
@@ -170,7 +178,7 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
     T in_d[2], in_x[2], in_g[2], in_z[2];
     TB in_B[2][O], in_C[2][O];
     float in_h[S];
-    uint32_t in_starts = 0;
+    uint8_t in_start = 0;   // of row `lane` of the block
     auto read = [&](const ScanBlock& k) {
         const ArgsPtr p = arguments_again();
         Stream<T> x, delta, gate, grad;
@@ -202,13 +210,8 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
         const auto save = row_buffer(p->s.saved + (k.b * p->saved_blocks + k.t0 / kRows) * (static_cast<int64_t>(p->s.states) * p->s.channels));
 #pragma unroll
         for (int j = 0; j < S; ++j) in_h[j] = lane_load<float>(save, state_at[j], 0);
-        in_starts = 0;
-        if (p->s.starts) {
-            const uint8_t* from = p->s.starts + k.b * p->s.starts_batch + k.t0 * p->s.starts_time;
-            bool on = false;
-            if (lane < k.count) on = from[lane * p->s.starts_time] != 0;
-            in_starts = static_cast<uint32_t>(__ballot(on));
-        }
+        in_start = 0;
+        if (p->s.starts && lane < k.count) in_start = (p->s.starts + k.b * p->s.starts_batch + k.t0 * p->s.starts_time)[lane * p->s.starts_time];
     };
 
     ScanBlock k = item_end(slot);
@@ -270,7 +273,7 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
                 for (int m = 0; m < O; ++m) B[e][m] = masked(to_f32(in_B[e][m]), operand_mask[m]), C[e][m] = masked(to_f32(in_C[e][m]), operand_mask[m]);
 #pragma unroll
             for (int j = 0; j < S; ++j) h0[j] = in_h[j];
-            const uint32_t starts = in_starts;
+            const uint32_t starts = static_cast<uint32_t>(__ballot(in_start != 0));
             if (next.count > 0) read(next);
             float y[2], rb[2], ra[2];
             auto walk = [&](auto with_starts) {
@@ -279,11 +282,14 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
                     constexpr int i = row;
                     const float4 v = s_row[w][i][lane & 15];
                     const bool start = decltype(with_starts)::value && (starts >> i & 1);
-#pragma unroll
-                    for (int j = 0; j < S; ++j) {
-                        const float before = i == 0 ? h0[j] : h[i == 0 ? 0 : i - 1][j], e = __builtin_amdgcn_exp2f(v.x * A2[j]);
-                        decay[i][j] = start ? 0.0f : e;
-                        h[i][j] = decay[i][j] * (start ? 0.0f : before);
+                    if (start) {
+                        asm volatile("; an episode starts");   // (a branch, not selects: nearly no row takes it)
+                        static_for<S>([&](auto j) { decay[i][j] = 0.0f, h[i][j] = 0.0f; });
+                    } else {
+                        static_for<S>([&](auto j) {
+                            decay[i][j] = __builtin_amdgcn_exp2f(v.x * A2[j]);
+                            h[i][j] = decay[i][j] * before<i>(h0, h, j);
+                        });
                     }
                     add_outer<(i & 3)>(h[i], B[i >> 2], v.y);
                     four[i & 3] = dot_quarter<(i & 3)>(C[i >> 2], h[i]);
@@ -303,10 +309,17 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
                     for (int j = 0; j < S; ++j) {
                         v[j] = r[j] * u.y;
                         v[S + j] = u.z * h[i][j];
-                        r[j] = start ? 0.0f : r[j] * decay[i][j];
-                        const float q = r[j] * (start ? 0.0f : i == 0 ? h0[j] : h[i == 0 ? 0 : i - 1][j]);
-                        four_a[i & 3] = __builtin_fmaf(q, A2[j], four_a[i & 3]);
-                        dA[j] = __builtin_fmaf(q, u.x, dA[j]);
+                    }
+                    if (start) {
+                        asm volatile("; an episode starts");
+                        static_for<S>([&](auto j) { r[j] = 0.0f; });
+                    } else {
+                        static_for<S>([&](auto j) {
+                            r[j] *= decay[i][j];
+                            const float q = r[j] * before<i>(h0, h, j);
+                            four_a[i & 3] = __builtin_fmaf(q, A2[j], four_a[i & 3]);
+                            dA[j] = __builtin_fmaf(q, u.x, dA[j]);
+                        });
                     }
                     halve_twice(v, sums);
 #pragma unroll
