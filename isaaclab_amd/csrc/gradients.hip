@@ -1,6 +1,6 @@
 // Global norm of many gradient tensors, and their scaling in place.
 // Two launches: every workgroup reduces its share of the elements to one number, then every workgroup of the second launch
-// adds all these numbers in the same order (there are at most 1 024) and scales its share.  Bound by memory: two reads and one
+// adds all these numbers in the same order (there are at most 2 048) and scales its share.  Bound by memory: two reads and one
 // write of every element, the second read left out where nothing is to scale.  Squares are added in 64 bits, so a gradient
 // of 1e30 has a norm and small gradients beside large ones count; the adds hide behind the loads.
 // The tensors' pointers and sizes travel as kernel arguments, kTensors of them to a launch: no table in device memory that
@@ -12,15 +12,17 @@
 
 namespace ilx {
 
-constexpr int kTensors = 96;              // per launch
-constexpr int64_t kChunk = 16384;         // elements: one share of a tensor
-constexpr int kMostPartials = 1024;
+constexpr int kTensors = 200;             // per launch: what fits the 4 KB of a kernel's arguments
+constexpr uint32_t kChunk = 16384;        // elements: one share of a tensor
+constexpr int64_t kMostElements = int64_t{1} << 30;   // of an entry; a larger tensor takes several
+constexpr int kMostPartials = 2048;
+constexpr int kPacks = 8;                 // 16-byte reads that a thread has in flight
 
 struct TensorTable {
     void* data[kTensors];
-    int64_t size[kTensors];
-    int32_t first_chunk[kTensors + 1];    // chunks ahead of tensor i
-    int32_t dtype[kTensors];
+    uint32_t size[kTensors];
+    int32_t first_chunk[kTensors + 1];    // chunks ahead of entry i
+    uint8_t dtype[kTensors];
     int32_t count;
 };
 
@@ -32,9 +34,10 @@ struct NormArgs {
     float max_norm;
     float* norm;
 };
+static_assert(sizeof(NormArgs) <= 4096 - 256, "kernel arguments");
 
 __device__ __forceinline__ int find_tensor(const TensorTable& t, int chunk) {
-    int lo = 0, hi = t.count - 1;   // the last tensor whose first chunk is not past `chunk`
+    int lo = 0, hi = t.count - 1;   // the last entry whose first chunk is not past `chunk`
     while (lo < hi) {
         const int mid = (lo + hi + 1) >> 1;
         if (t.first_chunk[mid] <= chunk)
@@ -46,24 +49,33 @@ __device__ __forceinline__ int find_tensor(const TensorTable& t, int chunk) {
 }
 
 // Calls f(value) for the elements of a chunk that fall to this thread, and with STORE writes back what it returns.
-template <bool STORE, typename T, typename F> __device__ __forceinline__ void each_element(T* p, int64_t n, F f) {
-    constexpr int V = 16 / sizeof(T);
-    int64_t head = 0;   // elements ahead of the first 16-byte boundary
-    const unsigned off = static_cast<unsigned>(reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T);
-    if (off) head = V - off < n ? V - off : n;
-    const int64_t packs = (n - head) / V, tail = head + packs * V;
-    if (static_cast<int64_t>(threadIdx.x) < head) {
+template <bool STORE, typename T, typename F> __device__ __forceinline__ void each_element(T* p, uint32_t n, F f) {
+    constexpr uint32_t V = 16 / sizeof(T);
+    const uint32_t off = static_cast<uint32_t>(reinterpret_cast<uintptr_t>(p) & 15) / sizeof(T);
+    const uint32_t head = off == 0 ? 0 : (V - off < n ? V - off : n);   // elements ahead of the first 16-byte boundary
+    const uint32_t packs = (n - head) / V, tail = head + packs * V;
+    if (threadIdx.x < head) {
         const float y = f(to_f32(p[threadIdx.x]));
         if (STORE) p[threadIdx.x] = from_f32<T>(y);
     }
-    for (int64_t i = threadIdx.x; i < packs; i += blockDim.x) {
-        float v[V];
-        load_channels<V>(p + head + i * V, v);
+    Pack<T, V>* q = reinterpret_cast<Pack<T, V>*>(p + head);
+    for (uint32_t i = threadIdx.x; i < packs; i += kPacks * 256) {
+        Pack<T, V> v[kPacks];
 #pragma unroll
-        for (int k = 0; k < V; ++k) v[k] = f(v[k]);
-        if (STORE) store_channels<V>(p + head + i * V, v);
+        for (int k = 0; k < kPacks; ++k) v[k] = q[i + k * 256 < packs ? i + k * 256 : i];
+#pragma unroll
+        for (int k = 0; k < kPacks; ++k) {
+            if (i + k * 256 < packs) {
+#pragma unroll
+                for (uint32_t e = 0; e < V; ++e) {
+                    const float y = f(to_f32(v[k].v[e]));
+                    if (STORE) v[k].v[e] = from_f32<T>(y);
+                }
+                if (STORE) q[i + k * 256] = v[k];
+            }
+        }
     }
-    const int64_t at = tail + threadIdx.x;
+    const uint32_t at = tail + threadIdx.x;
     if (at < n) {
         const float y = f(to_f32(p[at]));
         if (STORE) p[at] = from_f32<T>(y);
@@ -72,8 +84,8 @@ template <bool STORE, typename T, typename F> __device__ __forceinline__ void ea
 
 template <bool STORE, typename F> __device__ __forceinline__ void each_in_chunk(const TensorTable& t, int chunk, F f) {
     const int i = find_tensor(t, chunk);
-    const int64_t at = static_cast<int64_t>(chunk - t.first_chunk[i]) * kChunk;
-    const int64_t n = t.size[i] - at < kChunk ? t.size[i] - at : kChunk;
+    const uint32_t at = static_cast<uint32_t>(chunk - t.first_chunk[i]) * kChunk, left = t.size[i] - at;
+    const uint32_t n = left < kChunk ? left : kChunk;
     switch (t.dtype[i]) {
         case ILX_F32: each_element<STORE>(static_cast<float*>(t.data[i]) + at, n, f); break;
         case ILX_BF16: each_element<STORE>(static_cast<bf16_t*>(t.data[i]) + at, n, f); break;
@@ -131,21 +143,33 @@ using namespace ilx;
 
 namespace {
 
-constexpr int kMostTables = kMostPartials / 4;
+constexpr int kMostTables = kMostPartials / 16;
 
 size_t element_size(int dtype) { return dtype == ILX_F32 ? 4 : 2; }
 int64_t chunks_of(int64_t n) { return (n + kChunk - 1) / kChunk; }
+int64_t entries_of(int64_t n) { return (n + kMostElements - 1) / kMostElements; }
 
-// The tensors from number `next` on that fit one table, empty ones left out; returns the number behind the last.
-int fill_table(TensorTable& t, void* const* data, const int64_t* sizes, const int32_t* dtypes, int count, int next) {
+// Where a walk over the tensors' entries is: entry `part` of tensor `which`.
+struct Walk {
+    int which = 0;
+    int64_t part = 0;
+};
+
+// The next entries that fit one table, empty tensors left out.
+void fill_table(TensorTable& t, void* const* data, const int64_t* sizes, const int32_t* dtypes, int count, Walk& w) {
     t.count = 0, t.first_chunk[0] = 0;
-    for (; next < count && t.count < kTensors; ++next) {
-        if (sizes[next] == 0) continue;
-        t.data[t.count] = data[next], t.size[t.count] = sizes[next], t.dtype[t.count] = dtypes[next];
-        t.first_chunk[t.count + 1] = t.first_chunk[t.count] + static_cast<int32_t>(chunks_of(sizes[next]));
-        ++t.count;
+    while (w.which < count && t.count < kTensors) {
+        const int64_t begin = w.part * kMostElements, left = sizes[w.which] - begin;
+        if (left <= 0) {
+            ++w.which, w.part = 0;
+            continue;
+        }
+        const int64_t n = left < kMostElements ? left : kMostElements;
+        t.data[t.count] = static_cast<char*>(data[w.which]) + begin * element_size(dtypes[w.which]);
+        t.size[t.count] = static_cast<uint32_t>(n), t.dtype[t.count] = static_cast<uint8_t>(dtypes[w.which]);
+        t.first_chunk[t.count + 1] = t.first_chunk[t.count] + static_cast<int32_t>(chunks_of(n));
+        ++t.count, ++w.part;
     }
-    return next;
 }
 
 // Two tensors that share memory would be scaled twice, in no order.
@@ -188,19 +212,19 @@ extern "C" int ilx_gradient_norm(void* const* tensors_host, const int64_t* sizes
     ILX_REQUIRE(!clip || max_norm >= 0.0f, ILX_EINVAL, "ilx_gradient_norm: max_norm %g is negative or not a number", static_cast<double>(max_norm));
     ILX_REQUIRE(workspace && workspace_floats >= 2 * kMostPartials && aligned_to(workspace, 8), ILX_EINVAL,
                 "ilx_gradient_norm: workspace of %lld floats, %d needed, 8-byte aligned", (long long)workspace_floats, 2 * kMostPartials);
-    int64_t chunks_all = 0;
+    int64_t entries = 0;
     int used = 0;   // tensors with elements
     for (int i = 0; i < count; ++i) {
         ILX_REQUIRE(sizes_host[i] >= 0 && (tensors_host[i] || sizes_host[i] == 0), ILX_EINVAL, "ilx_gradient_norm: tensor %d is NULL or of negative size", i);
         ILX_REQUIRE(dtypes_host[i] >= ILX_F32 && dtypes_host[i] <= ILX_F16, ILX_EINVAL, "ilx_gradient_norm: tensor %d has unknown type %d", i,
                     dtypes_host[i]);
         ILX_REQUIRE(aligned_to(tensors_host[i], element_size(dtypes_host[i])), ILX_EINVAL, "ilx_gradient_norm: tensor %d is not aligned to its type", i);
-        chunks_all += chunks_of(sizes_host[i]);
+        entries += entries_of(sizes_host[i]);
         used += sizes_host[i] > 0;
     }
-    ILX_REQUIRE(chunks_all < INT32_MAX, ILX_ESHAPE, "ilx_gradient_norm: too many elements");
-    const int tables = used > 0 ? (used + kTensors - 1) / kTensors : 1;
-    ILX_REQUIRE(tables <= kMostTables, ILX_ESHAPE, "ilx_gradient_norm: %d tensors (at most %d)", used, kTensors * kMostTables);
+    ILX_REQUIRE(entries <= kTensors * kMostTables, ILX_ESHAPE, "ilx_gradient_norm: %d tensors, %lld pieces of 2^30 elements (at most %d)", used,
+                (long long)entries, kTensors * kMostTables);
+    const int tables = entries > 0 ? static_cast<int>((entries + kTensors - 1) / kTensors) : 1;
     if (clip) {
         const int rc = check_apart(tensors_host, sizes_host, dtypes_host, count, used);
         if (rc != ILX_OK) return rc;
@@ -213,8 +237,9 @@ extern "C" int ilx_gradient_norm(void* const* tensors_host, const int64_t* sizes
     a.maximum = norm_kind, a.max_norm = clip ? max_norm : 3.402823466e+38f;
     hipStream_t s = as_stream(stream);
     int at = 0;
-    for (int k = 0, next = 0; k < tables; ++k) {
-        next = fill_table(a.t, tensors_host, sizes_host, dtypes_host, count, next);
+    Walk walk;
+    for (int k = 0; k < tables; ++k) {
+        fill_table(a.t, tensors_host, sizes_host, dtypes_host, count, walk);
         const int chunks = a.t.first_chunk[a.t.count];
         a.partial0 = at, a.partials_here = chunks < 1 ? 1 : (chunks < most ? chunks : most);
         at += a.partials_here;
@@ -225,10 +250,11 @@ extern "C" int ilx_gradient_norm(void* const* tensors_host, const int64_t* sizes
         a.t.count = 0, a.t.first_chunk[0] = 0;
         ILX_LAUNCH(gradient_scale_kernel, dim3(1), dim3(256), 0, s, a);
     } else {
-        for (int k = 0, next = 0; k < tables; ++k) {
-            next = fill_table(a.t, tensors_host, sizes_host, dtypes_host, count, next);
+        walk = Walk();
+        for (int k = 0; k < tables; ++k) {
+            if (tables > 1) fill_table(a.t, tensors_host, sizes_host, dtypes_host, count, walk);   // (else it is filled)
             const int chunks = a.t.first_chunk[a.t.count];
-            ILX_LAUNCH(gradient_scale_kernel, dim3(chunks < 1 ? 1 : (chunks < 2048 ? chunks : 2048)), dim3(256), 0, s, a);
+            ILX_LAUNCH(gradient_scale_kernel, dim3(chunks < 1 ? 1 : (chunks < 4096 ? chunks : 4096)), dim3(256), 0, s, a);
             a.norm = nullptr;
         }
     }

@@ -35,8 +35,8 @@ __device__ __forceinline__ float softplus_f(float x) {
     return __builtin_fmaf(p, s, __builtin_fmaxf(x, 0.0f));   // (a NaN comes through e)
 }
 
-// V neighbouring channels of one row, as one load or store.
-template <typename T, int V> struct alignas(sizeof(T) * V) Pack { T v[V]; };
+// V neighbouring channels of one row, as one load or store of up to 16 bytes.
+template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack { T v[V]; };
 
 template <int V, typename T> __device__ __forceinline__ void load_channels(const T* p, float (&v)[V]) {
     const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(p);
@@ -52,10 +52,10 @@ template <int V, typename T> __device__ __forceinline__ void store_channels(T* p
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
-// The end of a parameter's gradient: `count` rows of (n0 + 1 + 1) x channels partial sums, one row per workgroup that kept
+// The end of a parameter's gradient: `count` rows of (n0 + extra) x channels partial sums, one row per workgroup that kept
 // some, are added in a fixed order, in 64 bits.  Value k of channel d goes to out0[d, k] for k < n0, then out1[d], out2[d];
 // outputs that are NULL are left out.
-void launch_parameter_sums(const float* partial, int64_t count, int32_t channels, int32_t n0, float* out0, float* out1, float* out2,
+void launch_parameter_sums(const float* partial, int64_t count, int32_t channels, int32_t n0, int32_t extra, float* out0, float* out1, float* out2,
                            hipStream_t stream);
 
 }  // namespace ilx

@@ -9,6 +9,7 @@
 namespace ilx {
 
 constexpr int kConvThreads = 256;
+constexpr int kConvRows = 4;
 
 struct ConvArgs {
     ilx_short_conv c;
@@ -88,6 +89,30 @@ template <int W, int V> __device__ __forceinline__ void forget(float (&win)[W][V
         for (int v = 0; v < V; ++v) win[k][v] = 0.0f;
 }
 
+// The next kConvRows rows of x (and of the output's gradient) and their start flags, read while the rows ahead are worked on.
+template <typename T, int V, bool GRAD> struct ConvRows {
+    Pack<T, V> x[kConvRows], g[kConvRows];
+    uint8_t start[kConvRows];
+
+    __device__ __forceinline__ void read(const ConvArgs& a, int d0, int64_t b, int64_t t, int64_t end) {
+        const T* px = static_cast<const T*>(a.c.x) + b * a.c.x_batch + d0;
+        const T* pg = static_cast<const T*>(a.c.grad_out) + b * a.c.grad_out_batch + d0;
+        const uint8_t* ps = a.c.starts + b * a.c.starts_batch;
+#pragma unroll
+        for (int i = 0; i < kConvRows; ++i) {
+            const int64_t r = t + i < end ? t + i : end - 1;
+            x[i] = *reinterpret_cast<const Pack<T, V>*>(px + r * a.c.x_time);
+            if (GRAD) g[i] = *reinterpret_cast<const Pack<T, V>*>(pg + r * a.c.grad_out_time);
+            start[i] = 0;
+            if (a.c.starts) start[i] = ps[r * a.c.starts_time];
+        }
+    }
+};
+template <int V, typename T> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&v)[V]) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = to_f32(p.v[k]);
+}
+
 template <typename T, int W, int V>
 __global__ void __launch_bounds__(kConvThreads) short_conv_forward_kernel(ConvArgs a) {
     const int cx = threadIdx.x & ((1 << a.cx_log2) - 1), row = threadIdx.x >> a.cx_log2;
@@ -101,20 +126,28 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_forward_kernel(ConvAr
     T* out = static_cast<T*>(a.c.out) + b * a.c.out_batch + d0;
     if (t0 < len || t0 == 0) {
         float w[W][V], bias[V], win[W][V];
+        ConvRows<T, V, false> rows;
+        if (t0 < te) rows.read(a, d0, b, t0, te);
         load_weights<W, V>(a, d0, w, bias);
         load_window<T, W, V>(a, d0, b, t0, win);
-        const T* x = static_cast<const T*>(a.c.x) + b * a.c.x_batch + d0;
-        for (int64_t t = t0; t < te; ++t) {
-            if (a.c.starts && a.c.starts[b * a.c.starts_batch + t * a.c.starts_time]) forget<W, V>(win);
-            load_channels<V>(x + t * a.c.x_time, win[W - 1]);
-            float p[V];
-            filter<W, V>(w, bias, win, p);
-            if (a.c.silu) {
+        for (int64_t t = t0; t < te; t += kConvRows) {
+            const ConvRows<T, V, false> now = rows;
+            if (t + kConvRows < te) rows.read(a, d0, b, t + kConvRows, te);
 #pragma unroll
-                for (int v = 0; v < V; ++v) p[v] *= sigmoid_fast(p[v]);
+            for (int i = 0; i < kConvRows; ++i) {
+                if (t + i < te) {
+                    if (now.start[i]) forget<W, V>(win);
+                    unpack<V>(now.x[i], win[W - 1]);
+                    float p[V];
+                    filter<W, V>(w, bias, win, p);
+                    if (a.c.silu) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) p[v] *= sigmoid_fast(p[v]);
+                    }
+                    store_channels<V>(out + (t + i) * a.c.out_time, p);
+                    shift<W, V>(win);
+                }
             }
-            store_channels<V>(out + t * a.c.out_time, p);
-            shift<W, V>(win);
         }
         if (a.c.last && (len == 0 || (te == len && t0 < len))) {   // the segment that ends the sequence
 #pragma unroll
@@ -150,8 +183,6 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvA
         const int64_t b = item / a.segments, t0 = (item - b * a.segments) * a.segment;
         const int64_t t1 = t0 + a.segment < a.c.length ? t0 + a.segment : a.c.length;
         const int64_t len = sequence_length(a.c.lengths, b, a.c.length);
-        const T* x = static_cast<const T*>(a.c.x) + b * a.c.x_batch + d0;
-        const T* dy = static_cast<const T*>(a.c.grad_out) + b * a.c.grad_out_batch + d0;
         T* dx = static_cast<T*>(a.c.grad_x) + b * a.c.grad_x_batch + d0;
         auto emit = [&](int64_t t, const float (&g)[V]) {
             if (t >= t0) {
@@ -171,46 +202,57 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvA
                 for (int v = 0; v < V; ++v) acc[j][v] = 0.0f;
             }
             const int64_t te = t1 + W - 1 < len ? t1 + W - 1 : len;
-            for (int64_t t = t0; t < te; ++t) {
-                if (a.c.starts && a.c.starts[b * a.c.starts_batch + t * a.c.starts_time]) {
-                    forget<W, V>(win);
+            ConvRows<T, V, true> rows;
+            if (t0 < te) rows.read(a, d0, b, t0, te);
+            for (int64_t first = t0; first < te; first += kConvRows) {
+                const ConvRows<T, V, true> now = rows;
+                if (first + kConvRows < te) rows.read(a, d0, b, first + kConvRows, te);
 #pragma unroll
-                    for (int j = 1; j < W; ++j) open[j] = false;
-                }
-                load_channels<V>(x + t * a.c.x_time, win[W - 1]);
-                float g[V], p[V];
-                load_channels<V>(dy + t * a.c.grad_out_time, g);
-                filter<W, V>(w, bias, win, p);
-                if (a.c.silu) {
+                for (int r = 0; r < kConvRows; ++r) {
+                    const int64_t t = first + r;
+                    if (t >= te) break;
+                    if (now.start[r]) {
+                        forget<W, V>(win);
 #pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        const float s = sigmoid_fast(p[v]);
-                        g[v] *= s * __builtin_fmaf(p[v], 1.0f - s, 1.0f);
+                        for (int j = 1; j < W; ++j) open[j] = false;
                     }
-                }
+                    unpack<V>(now.x[r], win[W - 1]);
+                    float g[V], p[V];
+                    unpack<V>(now.g[r], g);
+                    filter<W, V>(w, bias, win, p);
+                    if (a.c.silu) {
 #pragma unroll
-                for (int j = 0; j < W; ++j)
-#pragma unroll
-                    for (int v = 0; v < V; ++v) acc[j][v] = open[j] ? __builtin_fmaf(w[W - 1 - j][v], g[v], acc[j][v]) : acc[j][v];
-                if (t < t1) {
-#pragma unroll
-                    for (int v = 0; v < V; ++v) {
-                        db[v] += g[v];
-#pragma unroll
-                        for (int k = 0; k < W; ++k) dw[k][v] = __builtin_fmaf(g[v], win[k][v], dw[k][v]);
+                        for (int v = 0; v < V; ++v) {
+                            const float s = sigmoid_fast(p[v]);
+                            g[v] *= s * __builtin_fmaf(p[v], 1.0f - s, 1.0f);
+                        }
                     }
+#pragma unroll
+                    for (int j = 0; j < W; ++j)
+                        if (open[j]) {
+#pragma unroll
+                            for (int v = 0; v < V; ++v) acc[j][v] = __builtin_fmaf(w[W - 1 - j][v], g[v], acc[j][v]);
+                        }
+                    if (t < t1) {
+#pragma unroll
+                        for (int v = 0; v < V; ++v) {
+                            db[v] += g[v];
+#pragma unroll
+                            for (int k = 0; k < W; ++k) dw[k][v] = __builtin_fmaf(g[v], win[k][v], dw[k][v]);
+                        }
+                    }
+                    emit(t - (W - 1), acc[W - 1]);
+                    shift<W, V>(win);
+#pragma unroll
+                    for (int j = W - 1; j > 0; --j) {
+                        open[j] = open[j - 1];
+#pragma unroll
+                        for (int v = 0; v < V; ++v) acc[j][v] = acc[j - 1][v];
+                    }
+                    open[0] = true;
+#pragma unroll
+                    for (int v = 0; v < V; ++v) acc[0][v] = 0.0f;
                 }
-                emit(t - (W - 1), acc[W - 1]);
-                shift<W, V>(win);
-#pragma unroll
-                for (int j = W - 1; j > 0; --j) {
-                    open[j] = open[j - 1];
-#pragma unroll
-                    for (int v = 0; v < V; ++v) acc[j][v] = acc[j - 1][v];
-                }
-                open[0] = true;
-#pragma unroll
-                for (int v = 0; v < V; ++v) acc[0][v] = 0.0f;
             }
             if (te == len) {   // rows whose last readers are the carried-out state
 #pragma unroll
@@ -276,22 +318,29 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvArgs 
     for (int k = 0; k < W - 1; ++k) store_channels<V>(last + k * static_cast<int64_t>(a.c.channels), win[k + 1]);
 }
 
-// out0[d, k] = sum over the partial rows of value (k, d): 64 columns per workgroup, sixteen threads to a column.
+// out0[d, k] = sum over the partial rows of value (k, d): 32 columns to a workgroup, 32 threads to a column, eight rows of a thread in
+// flight.
 __global__ void __launch_bounds__(1024) parameter_sums_kernel(const float* partial, int64_t count, int channels, int n0, int columns,
                                                               float* out0, float* out1, float* out2) {
-    __shared__ double sums[16][64];
-    const int lane = threadIdx.x & 63, part = threadIdx.x >> 6;
-    const int64_t col = static_cast<int64_t>(blockIdx.x) * 64 + lane;
+    __shared__ double sums[32][33];
+    const int lane = threadIdx.x & 31, part = threadIdx.x >> 5;
+    const int col = static_cast<int>(blockIdx.x) * 32 + lane;
     double s = 0.0;
     if (col < columns)
-        for (int64_t r = part; r < count; r += 16) s += static_cast<double>(partial[r * columns + col]);
+        for (int64_t r = part; r < count; r += 8 * 32) {
+            float v[8];
+#pragma unroll
+            for (int k = 0; k < 8; ++k) v[k] = r + 32 * k < count ? partial[(r + 32 * k) * columns + col] : 0.0f;
+#pragma unroll
+            for (int k = 0; k < 8; ++k) s += static_cast<double>(v[k]);
+        }
     sums[part][lane] = s;
     __syncthreads();
     if (part != 0 || col >= columns) return;
     s = 0.0;
 #pragma unroll
-    for (int k = 0; k < 16; ++k) s += sums[k][lane];
-    const int k = static_cast<int>(col / channels), d = static_cast<int>(col - static_cast<int64_t>(k) * channels);
+    for (int k = 0; k < 32; ++k) s += sums[k][lane];
+    const int k = col / channels, d = col - k * channels;
     if (k < n0)
         out0[static_cast<int64_t>(d) * n0 + k] = static_cast<float>(s);
     else if (k == n0) {
@@ -300,10 +349,10 @@ __global__ void __launch_bounds__(1024) parameter_sums_kernel(const float* parti
         out2[d] = static_cast<float>(s);
 }
 
-void launch_parameter_sums(const float* partial, int64_t count, int32_t channels, int32_t n0, float* out0, float* out1, float* out2,
+void launch_parameter_sums(const float* partial, int64_t count, int32_t channels, int32_t n0, int32_t extra, float* out0, float* out1, float* out2,
                            hipStream_t stream) {
-    const int columns = channels * (n0 + 1 + (out2 ? 1 : 0));
-    ILX_LAUNCH(parameter_sums_kernel, dim3(blocks_for(columns, 64)), dim3(1024), 0, stream, partial, count, static_cast<int>(channels),
+    const int columns = channels * (n0 + extra);
+    ILX_LAUNCH(parameter_sums_kernel, dim3(blocks_for(columns, 32)), dim3(1024), 0, stream, partial, count, static_cast<int>(channels),
                static_cast<int>(n0), columns, out0, out1, out2);
 }
 
@@ -322,7 +371,7 @@ bool conv_rows_aligned(const void* p, int64_t batch, int64_t time, int64_t batch
 
 int conv_vector(const ilx_short_conv& c, bool backward) {
     const size_t item = conv_item_bytes(c.dtype);
-    const int v = 4;
+    const int v = !backward && item == 2 ? 8 : 4;   // 16 bytes; backward keeps five rows of values a channel, four channels fit
     const auto rows = [&](const void* p, int64_t sb, int64_t st) { return conv_rows_aligned(p, sb, st, c.batch, c.length, item, v); };
     bool ok = c.channels % v == 0 && rows(c.x, c.x_batch, c.x_time) && rows(c.out, c.out_batch, c.out_time) && aligned_to(c.state, 16) &&
               aligned_to(c.last, 16);
@@ -339,7 +388,9 @@ ConvArgs conv_args(const ilx_short_conv& c, int v, bool backward) {
     a.cx_log2 = 0;
     while (a.cx_log2 < 6 && (1 << a.cx_log2) < a.groups) ++a.cx_log2;
     a.channel_blocks = (a.groups + (1 << a.cx_log2) - 1) >> a.cx_log2;
-    a.segment = 32;
+    // A long segment reads few rows twice; it is halved while there are too few threads for two waves a SIMD.
+    a.segment = 64;
+    while (a.segment > 8 && c.batch * ((c.length + a.segment - 1) / a.segment) * a.groups < 512 * device_cu_count()) a.segment /= 2;
     a.segments = c.length > 0 ? (c.length + a.segment - 1) / a.segment : 1;
     a.items = c.batch * a.segments;
     const int rows = kConvThreads >> a.cx_log2;
@@ -370,7 +421,7 @@ template <typename T, int W, int V> void conv_launch(ConvKind kind, const ConvAr
         ILX_LAUNCH((short_conv_step_kernel<T, W, V>), dim3(blocks_for(a.items, kConvThreads)), dim3(threads), 0, s, a);
     } else if (kind == kForward) {
         ILX_LAUNCH((short_conv_forward_kernel<T, W, V>), dim3(static_cast<unsigned>(a.slots * a.channel_blocks)), dim3(threads), 0, s, a);
-    } else {
+    } else if constexpr (V <= 4) {
         ILX_LAUNCH((short_conv_backward_kernel<T, W, V>), dim3(static_cast<unsigned>(a.slots * a.channel_blocks)), dim3(threads),
                    static_cast<unsigned>(kConvThreads * (W + 1) * V * sizeof(float)), s, a);
     }
@@ -390,6 +441,9 @@ template <typename T, int V> void conv_width(ConvKind kind, const ConvArgs& a, h
 }
 
 template <typename T> void conv_vector_width(ConvKind kind, const ConvArgs& a, int v, hipStream_t s) {
+    if constexpr (sizeof(T) == 2) {
+        if (v == 8) return conv_width<T, 8>(kind, a, s);
+    }
     if (v == 4)
         conv_width<T, 4>(kind, a, s);
     else
@@ -445,7 +499,7 @@ extern "C" int ilx_short_conv_backward(const ilx_short_conv* conv, void* stream)
                 (long long)(a.slots * (c.width + 1) * c.channels));
     hipStream_t s = as_stream(stream);
     if (c.batch > 0) conv_dispatch(kBackward, a, v, s);
-    launch_parameter_sums(c.workspace, a.slots, c.channels, c.width, c.grad_weight, c.grad_bias, nullptr, s);
+    launch_parameter_sums(c.workspace, a.slots, c.channels, c.width, 1, c.grad_weight, c.grad_bias, nullptr, s);
     ILX_LAUNCH_CHECK("ilx_short_conv_backward");
     return ILX_OK;
 }

@@ -484,7 +484,7 @@ extern "C" int ilx_state_space_backward(const ilx_state_space* scan, void* strea
             default: wide ? backward_states<f16_t, float>(a, st) : backward_states<f16_t, f16_t>(a, st); break;
         }
     }
-    launch_parameter_sums(a.sums, a.slots, s.channels, s.states, s.grad_A, s.grad_D, s.grad_delta_bias, st);
+    launch_parameter_sums(a.sums, a.slots, s.channels, s.states, 2, s.grad_A, s.grad_D, s.grad_delta_bias, st);
     ILX_LAUNCH_CHECK("ilx_state_space_backward");
     return ILX_OK;
 }

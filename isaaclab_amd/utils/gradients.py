@@ -1,7 +1,7 @@
 """Global gradient norm and clipping on ``ilx_gradient_norm`` (include/isaaclab_amd_sequence.h): the end of a training step.
 
 No counterpart in the reference, whose RL libraries call torch.  All tensors, of any mix of float32, bfloat16 and float16, are
-reduced in one launch per 96 tensors and scaled in place in another; nothing is read back to the host.  Squares are added
+reduced in one launch per 200 tensors and scaled in place in another; nothing is read back to the host.  Squares are added
 in 64 bits in a fixed order, so the norm neither overflows nor depends on scheduling: replicas with equal gradients clip
 alike.
 """
@@ -19,7 +19,7 @@ from .. import _abi
 from .sequence import _DTYPES, _written
 
 _norm = _abi._sig("ilx_gradient_norm", _abi.P, _abi.P, _abi.P, c_int32, c_int32, c_int32, c_float, _abi.P, _abi.P, c_int64, _abi.P)
-_WORKSPACE = 2048   # floats, what ilx_gradient_norm_workspace says for any list
+_WORKSPACE = 4096   # floats, what ilx_gradient_norm_workspace says for any list
 
 
 def _is_dense(t: torch.Tensor) -> bool:
@@ -38,17 +38,16 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
     device = tensors[0].device
     if device.type != "cuda":
         raise _abi.IlxError("isaaclab_amd kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
-    pointers, sizes, dtypes = array("q"), array("q"), array("i")
-    for i, g in enumerate(tensors):
-        if g.device != device:
-            raise ValueError(f"gradient {i} is on {g.device}, the first on {device}")
-        if g.dtype not in _DTYPES:
-            raise ValueError(f"gradient {i} is {g.dtype}: float32, bfloat16 or float16 expected")
-        if g.layout != torch.strided or not _is_dense(g):
-            raise ValueError(f"gradient {i} is not dense: strides {g.stride() if g.layout == torch.strided else g.layout} of shape {tuple(g.shape)}")
-        pointers.append(g.data_ptr())
-        sizes.append(g.numel())
-        dtypes.append(_DTYPES[g.dtype])
+    kinds = [_DTYPES.get(g.dtype, -1) for g in tensors]
+    if min(kinds) < 0 or not all(g.is_contiguous() for g in tensors) or any(g.device != device for g in tensors):
+        for i, g in enumerate(tensors):
+            if g.device != device:
+                raise ValueError(f"gradient {i} is on {g.device}, the first on {device}")
+            if g.dtype not in _DTYPES:
+                raise ValueError(f"gradient {i} is {g.dtype}: float32, bfloat16 or float16 expected")
+            if g.layout != torch.strided or not _is_dense(g):
+                raise ValueError(f"gradient {i} is not dense: strides {g.stride() if g.layout == torch.strided else g.layout} of shape {tuple(g.shape)}")
+    pointers, sizes, dtypes = array("q", [g.data_ptr() for g in tensors]), array("q", [g.numel() for g in tensors]), array("i", kinds)
     norm = _abi.keep(torch.empty((), device=device))
     workspace = _abi.keep(torch.empty(_WORKSPACE, device=device))
 
@@ -63,8 +62,7 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
             status = launch()
     _abi.check(status, "ilx_gradient_norm")
     if clip:
-        for g in tensors:
-            _written(g)
+        _written(tensors)
     return norm
 
 

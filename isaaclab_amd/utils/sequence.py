@@ -187,10 +187,11 @@ def _check_out(out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
     return out
 
 
-def _written(t: torch.Tensor):
-    """Autograd sees the in-place update: a backward pass that needs the value from before it fails loudly."""
-    if not t.is_inference():
-        torch.autograd.graph.increment_version(t)
+def _written(tensors):
+    """Autograd sees the in-place update: a backward pass that needs a value from before it fails loudly."""
+    tensors = [t for t in tensors if not t.is_inference()]
+    if tensors:
+        torch.autograd.graph.increment_version(tensors)
 
 
 # ---- short convolution ----------------------------------------------------------------------------------------------
@@ -292,7 +293,7 @@ def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.T
         starts_batch=starts.stride(0) if starts is not None else 0, out=out.data_ptr(), out_batch=out.stride(0), last=state.data_ptr(),
         batch=batch, length=1, channels=channels, width=weight.shape[1], dtype=_DTYPES[x.dtype], silu=silu)
     _launch(_conv_step, desc, "ilx_short_conv_step", x.device)
-    _written(state)
+    _written((state,))
     return out
 
 
@@ -456,5 +457,5 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
         out=out.data_ptr(), out_batch=out.stride(0), last=state.data_ptr(), batch=batch, length=1, channels=channels, states=A.shape[1],
         groups=B.shape[1], dtype=_DTYPES[x.dtype], bc_dtype=_DTYPES[B.dtype], softplus=int(bool(softplus)))
     _launch(_scan_step, desc, "ilx_state_space_step", x.device)
-    _written(state)
+    _written((state,))
     return out

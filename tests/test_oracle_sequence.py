@@ -109,7 +109,7 @@ def test_state_space_refusals():
 
 
 def test_gradient_norm_refusals():
-    def call(pointers, sizes, dtypes, kind=0, clip=1, max_norm=1.0, norm=FAKE, workspace=FAKE, floats=2048, count=None):
+    def call(pointers, sizes, dtypes, kind=0, clip=1, max_norm=1.0, norm=FAKE, workspace=FAKE, floats=4096, count=None):
         n = len(pointers)
         return G._norm((ctypes.c_void_p * n)(*pointers), (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(*dtypes), n if count is None else count, kind,
                        clip, max_norm, norm, workspace, floats, None)
