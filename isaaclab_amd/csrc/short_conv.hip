@@ -9,7 +9,7 @@
 namespace ilx {
 
 constexpr int kConvThreads = 256;
-constexpr int kConvRows = 4;
+constexpr int kConvRows = 2;   // read ahead; 4: a recording of 16384 x 1024 in bfloat16 takes 42 us for 36, 8 (V = 4): 38, and spills in the backward pass (89 us for 66)
 
 struct ConvArgs {
     ilx_short_conv c;

@@ -8,6 +8,7 @@ alike.
 
 from __future__ import annotations
 
+import contextlib
 import math
 from array import array
 from collections.abc import Iterable
@@ -16,7 +17,7 @@ from ctypes import c_float, c_int32, c_int64
 import torch
 
 from .. import _abi
-from .sequence import _DTYPES, _written
+from .sequence import _DTYPES, _current_device, _written
 
 _norm = _abi._sig("ilx_gradient_norm", _abi.P, _abi.P, _abi.P, c_int32, c_int32, c_int32, c_float, _abi.P, _abi.P, c_int64, _abi.P)
 _WORKSPACE = 4096   # floats, what ilx_gradient_norm_workspace says for any list
@@ -35,31 +36,25 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
     tensors = [g for g in gradients if g is not None]
     if not tensors:
         raise ValueError("no gradients")
-    device = tensors[0].device
-    if device.type != "cuda":
+    first = tensors[0]
+    if not first.is_cuda:
         raise _abi.IlxError("isaaclab_amd kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
+    index = first.get_device()
     kinds = [_DTYPES.get(g.dtype, -1) for g in tensors]
-    if min(kinds) < 0 or not all(g.is_contiguous() for g in tensors) or any(g.device != device for g in tensors):
+    if min(kinds) < 0 or not all([g.is_contiguous() and g.get_device() == index for g in tensors]):
         for i, g in enumerate(tensors):
-            if g.device != device:
-                raise ValueError(f"gradient {i} is on {g.device}, the first on {device}")
+            if g.get_device() != index:
+                raise ValueError(f"gradient {i} is on {g.device}, the first on {first.device}")
             if g.dtype not in _DTYPES:
                 raise ValueError(f"gradient {i} is {g.dtype}: float32, bfloat16 or float16 expected")
             if g.layout != torch.strided or not _is_dense(g):
                 raise ValueError(f"gradient {i} is not dense: strides {g.stride() if g.layout == torch.strided else g.layout} of shape {tuple(g.shape)}")
     pointers, sizes, dtypes = array("q", [g.data_ptr() for g in tensors]), array("q", [g.numel() for g in tensors]), array("i", kinds)
-    norm = _abi.keep(torch.empty((), device=device))
-    workspace = _abi.keep(torch.empty(_WORKSPACE, device=device))
-
-    def launch():
-        return _norm(pointers.buffer_info()[0], sizes.buffer_info()[0], dtypes.buffer_info()[0], len(tensors), int(norm_type == math.inf), int(clip),
-                     max_norm, norm.data_ptr(), workspace.data_ptr(), _WORKSPACE, _abi.stream())
-
-    if device.index == torch.cuda.current_device():
-        status = launch()
-    else:
-        with torch.cuda.device(device):
-            status = launch()
+    norm = _abi.keep(torch.empty((), device=first.device))
+    workspace = _abi.keep(torch.empty(_WORKSPACE, device=first.device))
+    with contextlib.nullcontext() if index == _current_device() else torch.cuda.device(index):
+        status = _norm(pointers.buffer_info()[0], sizes.buffer_info()[0], dtypes.buffer_info()[0], len(tensors), int(norm_type == math.inf),
+                       int(clip), max_norm, norm.data_ptr(), workspace.data_ptr(), _WORKSPACE, _abi.stream())
     _abi.check(status, "ilx_gradient_norm")
     if clip:
         _written(tensors)

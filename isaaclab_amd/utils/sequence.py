@@ -83,12 +83,15 @@ _scan_backward = _abi._sig("ilx_state_space_backward", _P, _P)
 _scan_step = _abi._sig("ilx_state_space_step", _P, _P)
 
 
-def _launch(fn, desc, what: str, device: torch.device):
+_current_device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)   # (without the lazy-initialisation check)
+
+
+def _launch(fn, desc, what: str, index: int):
     """One call on the tensors' device and its current stream."""
-    if device.index == torch.cuda.current_device():
+    if index == _current_device():
         _abi.check(fn(ctypes.byref(desc), _abi.stream()), what)
     else:
-        with torch.cuda.device(device):
+        with torch.cuda.device(index):
             _abi.check(fn(ctypes.byref(desc), _abi.stream()), what)
 
 
@@ -103,30 +106,34 @@ def _copy(t: torch.Tensor, name: str, **how) -> torch.Tensor:
     return t.to(**how).contiguous()
 
 
-def _check_activation(t: torch.Tensor, name: str, shape: tuple, like: torch.Tensor) -> torch.Tensor:
+def _on(t: torch.Tensor, name: str, index: int):
+    if t.get_device() != index:
+        raise ValueError(f"{name} is on {t.device}, the activations on cuda:{index}")
+
+
+def _check_activation(t: torch.Tensor, name: str, like: torch.Tensor, index: int) -> torch.Tensor:
     """``t`` with unit channel stride (copied only if it has another)."""
-    if tuple(t.shape) != shape:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if t.dtype != like.dtype:
+    if t.shape != like.shape:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(like.shape)}")
+    if t.dtype is not like.dtype:
         raise ValueError(f"{name} is {t.dtype} beside {like.dtype} activations")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, the activations on {like.device}")
+    _on(t, name, index)
     return t if t.stride(-1) == 1 or t.shape[-1] == 1 else _copy(t, name)
 
 
-def _check_parameter(t: torch.Tensor | None, name: str, shape: tuple, device) -> torch.Tensor | None:
+def _check_parameter(t: torch.Tensor | None, name: str, shape: tuple, index: int) -> torch.Tensor | None:
     if t is None:
         return None
-    if tuple(t.shape) != shape:
+    if t.shape != shape:
         raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {shape}")
-    if t.dtype != torch.float32:
+    if t.dtype is not torch.float32:
         raise ValueError(f"{name} is {t.dtype}: parameters and states are float32")
-    if t.device != device:
-        raise ValueError(f"{name} is on {t.device}, the activations on {device}")
+    _on(t, name, index)
     return t if t.is_contiguous() else _copy(t, name)
 
 
-def _check_x(x: torch.Tensor, dims: int):
+def _check_x(x: torch.Tensor, dims: int) -> tuple[torch.Tensor, int]:
+    """x with unit channel stride, and its device."""
     if not x.is_cuda:
         raise _abi.IlxError("isaaclab_amd kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
     if x.dim() != dims:
@@ -135,44 +142,50 @@ def _check_x(x: torch.Tensor, dims: int):
         raise ValueError(f"activations are float32, bfloat16 or float16, got {x.dtype}")
     if x.shape[-1] == 0:
         raise ValueError("x has no channels")
+    return (x if x.stride(-1) == 1 or x.shape[-1] == 1 else _copy(x, "x")), x.get_device()
 
 
-def _check_starts(starts: torch.Tensor | None, shape: tuple, device) -> torch.Tensor | None:
-    if starts is None:
-        return None
-    if tuple(starts.shape) != shape or starts.dtype not in (torch.bool, torch.uint8):
-        raise ValueError(f"starts is {starts.dtype} {tuple(starts.shape)}, expected bool {shape}")
-    if starts.device != device:
-        raise ValueError(f"starts is on {starts.device}, the activations on {device}")
+def _check_starts(starts: torch.Tensor | None, shape: tuple, index: int) -> torch.Tensor | None:
+    if starts is not None:
+        if starts.shape != shape or starts.dtype not in (torch.bool, torch.uint8):
+            raise ValueError(f"starts is {starts.dtype} {tuple(starts.shape)}, expected bool {shape}")
+        _on(starts, "starts", index)
     return starts
 
 
-def _check_lengths(lengths: torch.Tensor | None, batch: int, device) -> torch.Tensor | None:
+def _check_lengths(lengths: torch.Tensor | None, batch: int, index: int) -> torch.Tensor | None:
     if lengths is None:
         return None
-    if tuple(lengths.shape) != (batch,) or lengths.dtype not in (torch.int32, torch.int64):
+    if lengths.shape != (batch,) or lengths.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"lengths is {lengths.dtype} {tuple(lengths.shape)}, expected int32 or int64 {(batch,)}")
-    if lengths.device != device:
-        raise ValueError(f"lengths is on {lengths.device}, the activations on {device}")
-    return lengths if lengths.dtype == torch.int32 and lengths.is_contiguous() else _copy(lengths, "lengths", dtype=torch.int32)
+    _on(lengths, "lengths", index)
+    return lengths if lengths.dtype is torch.int32 and lengths.is_contiguous() else _copy(lengths, "lengths", dtype=torch.int32)
 
 
-def _check_state(state: torch.Tensor, shape: tuple, x: torch.Tensor):
+def _check_state(state: torch.Tensor, shape: tuple, index: int):
     """A state that is updated in place: it cannot be a copy."""
     if not isinstance(state, torch.Tensor):
         raise ValueError("a step needs its carried state (zeros for a new sequence)")
     if not state.is_contiguous():
         raise ValueError("state is updated in place and must be contiguous")
-    _check_parameter(state, "state", shape, x.device)
+    _check_parameter(state, "state", shape, index)
 
 
-def _no_gradients(what: str, *tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+def _wants_gradients(tensors) -> bool:
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                return True
+    return False
+
+
+def _no_gradients(what: str, tensors):
+    if _wants_gradients(tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or use the form over sequences")
 
 
-def _needs_gradients(*tensors) -> bool:
-    if not torch.is_grad_enabled() or not any(t is not None and t.requires_grad for t in tensors):
+def _needs_gradients(tensors) -> bool:
+    if not _wants_gradients(tensors):
         return False
     if _abi.recording():
         raise _abi.IlxError("a call that needs gradients cannot be recorded in a command list (its backward pass runs on another thread)")
@@ -181,10 +194,23 @@ def _needs_gradients(*tensors) -> bool:
 
 def _check_out(out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
     if out is None:
-        return _abi.keep(torch.empty_like(x))
-    if out.shape != x.shape or out.dtype != x.dtype or out.device != x.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
+        return _empty_like(x)
+    if out.shape != x.shape or out.dtype is not x.dtype or out.device != x.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
         raise ValueError(f"out must be like x ({tuple(x.shape)}, {x.dtype}) with unit channel stride")
     return out
+
+
+def _empty_like(x: torch.Tensor) -> torch.Tensor:
+    """Dense, in x's order of batch and time; where x is a view whose rows overlap (a sliding window), in the plain order."""
+    out = torch.empty_like(x)
+    return out if out.stride(-1) == 1 or out.shape[-1] == 1 else torch.empty(x.shape, dtype=x.dtype, device=x.device)
+
+
+def _keep(*tensors):
+    """What a recorded call reads or writes stays alive with its list."""
+    if _abi.recording():
+        for t in tensors:
+            _abi.keep(t)
 
 
 def _written(tensors):
@@ -192,6 +218,11 @@ def _written(tensors):
     tensors = [t for t in tensors if not t.is_inference()]
     if tensors:
         torch.autograd.graph.increment_version(tensors)
+
+
+def _moved(desc, **pointers) -> bool:
+    """Whether a saved tensor came back from another place than the forward pass saw it (hooks may pack saved tensors)."""
+    return any(getattr(desc, name) != _p(t) for name, t in pointers.items())
 
 
 # ---- short convolution ----------------------------------------------------------------------------------------------
@@ -203,19 +234,23 @@ def _silu(activation) -> int:
 
 def _conv_desc(x, weight, bias, state, starts, lengths, silu) -> ShortConvDesc:
     batch, length, channels = x.shape
+    x_batch, x_time, _ = x.stride()
+    starts_batch, starts_time = starts.stride() if starts is not None else (0, 0)
+    # (in the order of the fields)
     return ShortConvDesc(
-        x=x.data_ptr(), x_batch=x.stride(0), x_time=x.stride(1), weight=weight.data_ptr(), bias=_p(bias), state=_p(state), starts=_p(starts),
-        starts_batch=starts.stride(0) if starts is not None else 0, starts_time=starts.stride(1) if starts is not None else 0,
-        lengths=_p(lengths), batch=batch, length=length, channels=channels, width=weight.shape[1], dtype=_DTYPES[x.dtype], silu=silu)
+        x.data_ptr(), x_batch, x_time, weight.data_ptr(), _p(bias), _p(state), _p(starts), starts_batch, starts_time, _p(lengths),
+        None, 0, 0, None, batch, length, channels, weight.shape[1], _DTYPES[x.dtype], silu)
 
 
 def _conv_call(x, weight, bias, state, starts, lengths, silu, want_last):
     desc = _conv_desc(x, weight, bias, state, starts, lengths, silu)
-    out = _abi.keep(torch.empty_like(x))
-    last = _abi.keep(torch.empty(x.shape[0], weight.shape[1] - 1, x.shape[2], device=x.device)) if want_last else None
-    desc.out, desc.out_batch, desc.out_time, desc.last = out.data_ptr(), out.stride(0), out.stride(1), _p(last)
-    _launch(_conv_forward, desc, "ilx_short_conv_forward", x.device)
-    return out, last
+    out = _empty_like(x)
+    last = torch.empty(x.shape[0], weight.shape[1] - 1, x.shape[2], device=x.device) if want_last else None
+    _keep(out, last)
+    desc.out, desc.last = out.data_ptr(), _p(last)
+    desc.out_batch, desc.out_time, _ = out.stride()
+    _launch(_conv_forward, desc, "ilx_short_conv_forward", x.get_device())
+    return out, last, desc
 
 
 class _ShortConvolution(torch.autograd.Function):
@@ -223,28 +258,38 @@ class _ShortConvolution(torch.autograd.Function):
     def forward(ctx, x, weight, bias, state, starts, lengths, silu, want_last):
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(x, weight, bias, state, starts, lengths)
-        ctx.silu = silu
-        return _conv_call(x, weight, bias, state, starts, lengths, silu, want_last)
+        out, last, ctx.desc = _conv_call(x, weight, bias, state, starts, lengths, silu, want_last)
+        return out, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_last):
         x, weight, bias, state, starts, lengths = ctx.saved_tensors
-        grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", tuple(x.shape), x)
+        d = ctx.desc
+        if _moved(d, x=x, weight=weight, bias=bias, state=state, starts=starts, lengths=lengths):
+            d = _conv_desc(x, weight, bias, state, starts, lengths, d.silu)
+        index = x.get_device()
+        grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", x, index)
         grad_last = None if grad_last is None else grad_last.contiguous()
-        grad_x, grad_weight = torch.empty_like(x), torch.empty_like(weight)
+        grad_x, grad_weight = _empty_like(x), torch.empty_like(weight)
         grad_bias = None if bias is None else torch.empty_like(bias)
         grad_state = torch.empty_like(state) if state is not None and ctx.needs_input_grad[3] else None
-        d = _conv_desc(x, weight, bias, state, starts, lengths, ctx.silu)
-        d.grad_out, d.grad_out_batch, d.grad_out_time, d.grad_last = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1), _p(grad_last)
-        d.grad_x, d.grad_x_batch, d.grad_x_time = grad_x.data_ptr(), grad_x.stride(0), grad_x.stride(1)
+        d.grad_out, d.grad_last, d.grad_x = grad_out.data_ptr(), _p(grad_last), grad_x.data_ptr()
+        d.grad_out_batch, d.grad_out_time, _ = grad_out.stride()
+        d.grad_x_batch, d.grad_x_time, _ = grad_x.stride()
         d.grad_weight, d.grad_bias, d.grad_state = grad_weight.data_ptr(), _p(grad_bias), _p(grad_state)
         need = c_int64()
         _abi.check(_conv_workspace(ctypes.byref(d), ctypes.byref(need)), "ilx_short_conv_workspace")
         workspace = torch.empty(need.value, device=x.device)
         d.workspace, d.workspace_floats = workspace.data_ptr(), need.value
-        _launch(_conv_backward, d, "ilx_short_conv_backward", x.device)
+        _launch(_conv_backward, d, "ilx_short_conv_backward", index)
         return grad_x, grad_weight, grad_bias, grad_state, None, None, None, None
+
+
+def _check_filter(weight: torch.Tensor, bias, channels: int, index: int):
+    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
+        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (channels, width) with a width of 1..{MAX_WIDTH}")
+    return _check_parameter(weight, "weight", (channels, weight.shape[1]), index), _check_parameter(bias, "bias", (channels,), index)
 
 
 def short_convolution(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *, activation: str | None = None,
@@ -256,19 +301,17 @@ def short_convolution(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
     (batch, W - 1, channels) holds the rows ahead of the first, oldest first (zeros if None).  With ``return_state`` the
     result is ``(out, last)``, ``last`` being the state ahead of the next row.  Differentiable in ``x``, ``weight``,
     ``bias`` and ``state``."""
-    _check_x(x, 3)
+    x, index = _check_x(x, 3)
     batch, length, channels = x.shape
     silu = _silu(activation)
-    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
-        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (channels, width) with a width of 1..{MAX_WIDTH}")
-    x = _check_activation(x, "x", (batch, length, channels), x)
-    weight = _check_parameter(weight, "weight", (channels, weight.shape[1]), x.device)
-    bias = _check_parameter(bias, "bias", (channels,), x.device)
-    state = _check_parameter(state, "state", (batch, weight.shape[1] - 1, channels), x.device)
-    starts = _check_starts(starts, (batch, length), x.device)
-    lengths = _check_lengths(lengths, batch, x.device)
-    args = (x, weight, bias, state, starts, lengths, silu, return_state)
-    out, last = _ShortConvolution.apply(*args) if _needs_gradients(x, weight, bias, state) else _conv_call(*args)
+    weight, bias = _check_filter(weight, bias, channels, index)
+    state = _check_parameter(state, "state", (batch, weight.shape[1] - 1, channels), index)
+    starts = _check_starts(starts, (batch, length), index)
+    lengths = _check_lengths(lengths, batch, index)
+    if _needs_gradients((x, weight, bias, state)):
+        out, last = _ShortConvolution.apply(x, weight, bias, state, starts, lengths, silu, return_state)
+    else:
+        out, last, _ = _conv_call(x, weight, bias, state, starts, lengths, silu, return_state)
     return (out, last) if return_state else out
 
 
@@ -276,61 +319,60 @@ def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.T
                            activation: str | None = None, starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """One row of :func:`short_convolution` per sequence: ``x`` (batch, channels), ``state`` (batch, W - 1, channels) updated in
     place, ``starts`` (batch) the environments whose episode begins with this row.  ``out`` may name the result's buffer."""
-    _check_x(x, 2)
-    _no_gradients("short_convolution_step", x, weight, bias, state)
+    x, index = _check_x(x, 2)
+    _no_gradients("short_convolution_step", (x, weight, bias, state))
     batch, channels = x.shape
     silu = _silu(activation)
-    if weight.dim() != 2 or not 1 <= weight.shape[1] <= MAX_WIDTH:
-        raise ValueError(f"weight has shape {tuple(weight.shape)}, expected (channels, width) with a width of 1..{MAX_WIDTH}")
-    x = _abi.keep(_check_activation(x, "x", (batch, channels), x))
-    weight = _abi.keep(_check_parameter(weight, "weight", (channels, weight.shape[1]), x.device))
-    bias = _abi.keep(_check_parameter(bias, "bias", (channels,), x.device))
-    _check_state(state, (batch, weight.shape[1] - 1, channels), x)
-    starts = _check_starts(starts, (batch,), x.device)
+    weight, bias = _check_filter(weight, bias, channels, index)
+    width = weight.shape[1]
+    _check_state(state, (batch, width - 1, channels), index)
+    starts = _check_starts(starts, (batch,), index)
     out = _check_out(out, x)
+    _keep(x, weight, bias, out)
+    at = state.data_ptr()
     desc = ShortConvDesc(
-        x=x.data_ptr(), x_batch=x.stride(0), weight=weight.data_ptr(), bias=_p(bias), state=state.data_ptr(), starts=_p(starts),
-        starts_batch=starts.stride(0) if starts is not None else 0, out=out.data_ptr(), out_batch=out.stride(0), last=state.data_ptr(),
-        batch=batch, length=1, channels=channels, width=weight.shape[1], dtype=_DTYPES[x.dtype], silu=silu)
-    _launch(_conv_step, desc, "ilx_short_conv_step", x.device)
+        x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _p(bias), at, _p(starts), starts.stride(0) if starts is not None else 0, 0, None,
+        out.data_ptr(), out.stride(0), 0, at, batch, 1, channels, width, _DTYPES[x.dtype], silu)
+    _launch(_conv_step, desc, "ilx_short_conv_step", index)
     _written((state,))
     return out
 
 
 # ---- state space recurrence -------------------------------------------------------------------------------------------
-def _shared(t: torch.Tensor, name: str, lead: tuple, like: torch.Tensor) -> torch.Tensor:
+def _shared(t: torch.Tensor, name: str, like: torch.Tensor, index: int) -> torch.Tensor:
     """B or C as (*lead, groups, states), dense over the last two: in the activations' type or float32."""
+    lead = like.shape[:-1]
     if t.dim() == len(lead) + 1:
         t = t.unsqueeze(-2)
-    if t.dim() != len(lead) + 2 or tuple(t.shape[:-2]) != lead:
-        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {lead} + (groups, states) or (states,)")
-    if t.dtype not in (like.dtype, torch.float32):
+    if t.dim() != len(lead) + 2 or t.shape[:-2] != lead:
+        raise ValueError(f"{name} has shape {tuple(t.shape)}, expected {tuple(lead)} + (groups, states) or (states,)")
+    if t.dtype is not like.dtype and t.dtype is not torch.float32:
         raise ValueError(f"{name} is {t.dtype} beside {like.dtype} activations")
-    if t.device != like.device:
-        raise ValueError(f"{name} is on {t.device}, the activations on {like.device}")
+    _on(t, name, index)
     g, n = t.shape[-2:]
     return t if (n == 1 or t.stride(-1) == 1) and (g == 1 or t.stride(-2) == n) else _copy(t, name)
 
 
 def _pair(B: torch.Tensor, C: torch.Tensor) -> tuple[torch.Tensor, torch.Tensor]:
     """In one type: in float32 where one is."""
-    if B.dtype != C.dtype:
-        B, C = (t if t.dtype == torch.float32 else _copy(t, "B or C", dtype=torch.float32) for t in (B, C))
+    if B.dtype is not C.dtype:
+        B, C = (t if t.dtype is torch.float32 else _copy(t, "B or C", dtype=torch.float32) for t in (B, C))
     return B, C
 
 
 def _scan_desc(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus) -> StateSpaceDesc:
     batch, length, channels = x.shape
-    d = StateSpaceDesc(
-        x=x.data_ptr(), x_batch=x.stride(0), x_time=x.stride(1), delta=delta.data_ptr(), delta_batch=delta.stride(0), delta_time=delta.stride(1),
-        A=A.data_ptr(), B=B.data_ptr(), B_batch=B.stride(0), B_time=B.stride(1), C=C.data_ptr(), C_batch=C.stride(0), C_time=C.stride(1),
-        D=_p(D), delta_bias=_p(delta_bias), state=_p(state), starts=_p(starts), lengths=_p(lengths), batch=batch, length=length,
-        channels=channels, states=A.shape[1], groups=B.shape[2], dtype=_DTYPES[x.dtype], bc_dtype=_DTYPES[B.dtype], softplus=softplus)
-    if gate is not None:
-        d.gate, d.gate_batch, d.gate_time = gate.data_ptr(), gate.stride(0), gate.stride(1)
-    if starts is not None:
-        d.starts_batch, d.starts_time = starts.stride(0), starts.stride(1)
-    return d
+    x_batch, x_time, _ = x.stride()
+    delta_batch, delta_time, _ = delta.stride()
+    gate_batch, gate_time, _ = gate.stride() if gate is not None else (0, 0, 0)
+    B_batch, B_time, _, _ = B.stride()
+    C_batch, C_time, _, _ = C.stride()
+    starts_batch, starts_time = starts.stride() if starts is not None else (0, 0)
+    # (in the order of the fields)
+    return StateSpaceDesc(
+        x.data_ptr(), x_batch, x_time, delta.data_ptr(), delta_batch, delta_time, _p(gate), gate_batch, gate_time, A.data_ptr(),
+        B.data_ptr(), B_batch, B_time, C.data_ptr(), C_batch, C_time, _p(D), _p(delta_bias), _p(state), _p(starts), starts_batch, starts_time,
+        _p(lengths), None, 0, 0, None, None, batch, length, channels, A.shape[1], B.shape[2], _DTYPES[x.dtype], _DTYPES[B.dtype], softplus)
 
 
 def _scan_scratch(desc: StateSpaceDesc, backward: int, device) -> torch.Tensor | None:
@@ -338,71 +380,82 @@ def _scan_scratch(desc: StateSpaceDesc, backward: int, device) -> torch.Tensor |
     _abi.check(_scan_workspace(ctypes.byref(desc), backward, ctypes.byref(need)), "ilx_state_space_workspace")
     if need.value == 0:
         return None
-    workspace = _abi.keep(torch.empty(need.value, device=device))
+    workspace = torch.empty(need.value, device=device)
     desc.workspace, desc.workspace_floats = workspace.data_ptr(), need.value
     return workspace
 
 
 def _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last, save=False):
     B, C = _pair(B, C)
-    _abi.keep(B), _abi.keep(C)
     desc = _scan_desc(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus)
     batch, length, channels = x.shape
-    out = _abi.keep(torch.empty_like(x))
-    last = _abi.keep(torch.empty(batch, A.shape[1], channels, device=x.device)) if want_last else None
-    saved = torch.empty(batch, (length + _BLOCK - 1) // _BLOCK, A.shape[1], channels, device=x.device) if save else None
-    desc.out, desc.out_batch, desc.out_time, desc.last, desc.saved = out.data_ptr(), out.stride(0), out.stride(1), _p(last), _p(saved)
-    workspace = _scan_scratch(desc, 0, x.device)  # noqa: F841  (alive until the launch is queued)
-    _launch(_scan_forward, desc, "ilx_state_space_forward", x.device)
-    return out, last, saved
+    device = x.device
+    out = _empty_like(x)
+    last = torch.empty(batch, A.shape[1], channels, device=device) if want_last else None
+    saved = torch.empty(batch, (length + _BLOCK - 1) // _BLOCK, A.shape[1], channels, device=device) if save else None
+    desc.out, desc.last, desc.saved = out.data_ptr(), _p(last), _p(saved)
+    desc.out_batch, desc.out_time, _ = out.stride()
+    workspace = _scan_scratch(desc, 0, device)
+    _keep(out, last, workspace)
+    _launch(_scan_forward, desc, "ilx_state_space_forward", x.get_device())
+    return out, last, saved, desc
 
 
 class _StateSpaceScan(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last):
         ctx.set_materialize_grads(False)
-        out, last, saved = _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last, True)
+        out, last, saved, ctx.desc = _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last, True)
         ctx.save_for_backward(x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved)
-        ctx.softplus, ctx.has_state = softplus, state is not None
+        ctx.has_state = state is not None
         return out, last
 
     @staticmethod
     @once_differentiable
     def backward(ctx, grad_out, grad_last):
         x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved = ctx.saved_tensors
-        grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", tuple(x.shape), x)
-        grad_last = None if grad_last is None else grad_last.contiguous()
+        d = ctx.desc
         rB, rC = _pair(B, C)
-        d = _scan_desc(x, delta, A, rB, rC, D, gate, delta_bias, None, starts, lengths, ctx.softplus)
-        gx, gA = torch.empty_like(x), torch.empty_like(A)
+        if _moved(d, x=x, delta=delta, A=A, B=rB, C=rC, D=D, gate=gate, delta_bias=delta_bias, starts=starts, lengths=lengths, saved=saved):
+            d = _scan_desc(x, delta, A, rB, rC, D, gate, delta_bias, None, starts, lengths, d.softplus)
+            d.saved = saved.data_ptr()
+        index, device = x.get_device(), x.device
+        grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", x, index)
+        grad_last = None if grad_last is None else grad_last.contiguous()
+        gx, gA = _empty_like(x), torch.empty_like(A)
         gdelta, ggate = torch.empty_like(gx), None if gate is None else torch.empty_like(gx)
-        gB, gC = torch.empty(rB.shape, dtype=rB.dtype, device=x.device), torch.empty(rC.shape, dtype=rC.dtype, device=x.device)
+        gB, gC = torch.empty(rB.shape, dtype=rB.dtype, device=device), torch.empty(rC.shape, dtype=rC.dtype, device=device)
         gD, gbias = (None if t is None else torch.empty_like(t) for t in (D, delta_bias))
-        gstate = torch.empty(x.shape[0], A.shape[1], x.shape[2], device=x.device) if ctx.has_state and ctx.needs_input_grad[8] else None
-        d.saved = saved.data_ptr()
-        d.grad_out, d.grad_out_batch, d.grad_out_time = grad_out.data_ptr(), grad_out.stride(0), grad_out.stride(1)
-        d.grad_x, d.grad_delta, d.grad_gate, d.grad_batch, d.grad_time = gx.data_ptr(), gdelta.data_ptr(), _p(ggate), gx.stride(0), gx.stride(1)
+        gstate = torch.empty(x.shape[0], A.shape[1], x.shape[2], device=device) if ctx.has_state and ctx.needs_input_grad[8] else None
+        d.grad_out, d.grad_x, d.grad_delta, d.grad_gate = grad_out.data_ptr(), gx.data_ptr(), gdelta.data_ptr(), _p(ggate)
+        d.grad_out_batch, d.grad_out_time, _ = grad_out.stride()
+        d.grad_batch, d.grad_time, _ = gx.stride()
         d.grad_last, d.grad_A, d.grad_B, d.grad_C = _p(grad_last), gA.data_ptr(), gB.data_ptr(), gC.data_ptr()
         d.grad_D, d.grad_delta_bias, d.grad_state = _p(gD), _p(gbias), _p(gstate)
-        workspace = _scan_scratch(d, 1, x.device)  # noqa: F841
-        _launch(_scan_backward, d, "ilx_state_space_backward", x.device)
-        return gx, gdelta, gA, gB.to(B.dtype), gC.to(C.dtype), gD, ggate, gbias, gstate, None, None, None, None
+        workspace = _scan_scratch(d, 1, device)  # noqa: F841  (alive until the launches are queued)
+        _launch(_scan_backward, d, "ilx_state_space_backward", index)
+        if rB is not B:
+            gB = gB.to(B.dtype)
+        if rC is not C:
+            gC = gC.to(C.dtype)
+        return gx, gdelta, gA, gB, gC, gD, ggate, gbias, gstate, None, None, None, None
 
 
-def _scan_operands(x, delta, A, B, C, D, gate, delta_bias):
-    lead, channels = tuple(x.shape[:-1]), x.shape[-1]
+def _scan_operands(x, index, delta, A, B, C, D, gate, delta_bias):
+    channels = x.shape[-1]
     if A.dim() != 2 or not 1 <= A.shape[1] <= MAX_STATES:
         raise ValueError(f"A has shape {tuple(A.shape)}, expected (channels, states) with 1..{MAX_STATES} states")
-    x = _check_activation(x, "x", tuple(x.shape), x)
-    delta = _check_activation(delta, "delta", tuple(x.shape), x)
-    gate = None if gate is None else _check_activation(gate, "gate", tuple(x.shape), x)
-    A = _check_parameter(A, "A", (channels, A.shape[1]), x.device)
-    D = _check_parameter(D, "D", (channels,), x.device)
-    delta_bias = _check_parameter(delta_bias, "delta_bias", (channels,), x.device)
-    B, C = _shared(B, "B", lead, x), _shared(C, "C", lead, x)
-    if B.shape != C.shape or B.shape[-1] != A.shape[1] or B.shape[-2] < 1 or channels % B.shape[-2]:
-        raise ValueError(f"B {tuple(B.shape)} and C {tuple(C.shape)} must have {A.shape[1]} states and groups that divide {channels} channels")
-    return x, delta, A, B, C, D, gate, delta_bias
+    states = A.shape[1]
+    delta = _check_activation(delta, "delta", x, index)
+    gate = None if gate is None else _check_activation(gate, "gate", x, index)
+    A = _check_parameter(A, "A", (channels, states), index)
+    D = _check_parameter(D, "D", (channels,), index)
+    delta_bias = _check_parameter(delta_bias, "delta_bias", (channels,), index)
+    B, C = _shared(B, "B", x, index), _shared(C, "C", x, index)
+    groups, n = B.shape[-2:]
+    if B.shape != C.shape or n != states or groups < 1 or channels % groups:
+        raise ValueError(f"B {tuple(B.shape)} and C {tuple(C.shape)} must have {states} states and groups that divide {channels} channels")
+    return delta, A, B, C, D, gate, delta_bias
 
 
 def state_space_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: torch.Tensor, C: torch.Tensor, *,
@@ -420,17 +473,17 @@ def state_space_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: t
     N, channels) is the state ahead of the first row (zeros if None); with ``return_state`` the result is ``(out, last)``.
     Differentiable in every operand but ``starts`` and ``lengths``; between a forward and its backward pass one state in 8
     rows is kept."""
-    _check_x(x, 3)
+    x, index = _check_x(x, 3)
     batch, length, channels = x.shape
-    x, delta, A, B, C, D, gate, delta_bias = _scan_operands(x, delta, A, B, C, D, gate, delta_bias)
-    state = _check_parameter(state, "state", (batch, A.shape[1], channels), x.device)
-    starts = _check_starts(starts, (batch, length), x.device)
-    lengths = _check_lengths(lengths, batch, x.device)
-    args = (x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, int(bool(softplus)), return_state)
-    if _needs_gradients(x, delta, A, B, C, D, gate, delta_bias, state):
+    delta, A, B, C, D, gate, delta_bias = _scan_operands(x, index, delta, A, B, C, D, gate, delta_bias)
+    state = _check_parameter(state, "state", (batch, A.shape[1], channels), index)
+    starts = _check_starts(starts, (batch, length), index)
+    lengths = _check_lengths(lengths, batch, index)
+    args = (x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, 1 if softplus else 0, return_state)
+    if _needs_gradients(args[:9]):
         out, last = _StateSpaceScan.apply(*args)
     else:
-        out, last, _ = _scan_call(*args)
+        out, last, _, _ = _scan_call(*args)
     return (out, last) if return_state else out
 
 
@@ -440,22 +493,22 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
     """One row of :func:`state_space_scan` per sequence: ``x``, ``delta``, ``gate`` (batch, channels), ``B``, ``C`` (batch, groups,
     N) or (batch, N), ``state`` (batch, N, channels) updated in place, ``starts`` (batch) the environments whose episode begins
     with this row.  ``out`` may name the result's buffer."""
-    _check_x(x, 2)
-    _no_gradients("state_space_step", x, delta, state, A, B, C, D, gate, delta_bias)
+    x, index = _check_x(x, 2)
+    _no_gradients("state_space_step", (x, delta, state, A, B, C, D, gate, delta_bias))
     batch, channels = x.shape
-    x, delta, A, B, C, D, gate, delta_bias = _scan_operands(x, delta, A, B, C, D, gate, delta_bias)
+    delta, A, B, C, D, gate, delta_bias = _scan_operands(x, index, delta, A, B, C, D, gate, delta_bias)
     B, C = _pair(B, C)
-    for t in (x, delta, A, B, C, D, gate, delta_bias):
-        _abi.keep(t)
-    _check_state(state, (batch, A.shape[1], channels), x)
-    starts = _check_starts(starts, (batch,), x.device)
+    states = A.shape[1]
+    _check_state(state, (batch, states, channels), index)
+    starts = _check_starts(starts, (batch,), index)
     out = _check_out(out, x)
+    _keep(x, delta, A, B, C, D, gate, delta_bias, out)
+    at = state.data_ptr()
     desc = StateSpaceDesc(
-        x=x.data_ptr(), x_batch=x.stride(0), delta=delta.data_ptr(), delta_batch=delta.stride(0), gate=_p(gate),
-        gate_batch=gate.stride(0) if gate is not None else 0, A=A.data_ptr(), B=B.data_ptr(), B_batch=B.stride(0), C=C.data_ptr(), C_batch=C.stride(0),
-        D=_p(D), delta_bias=_p(delta_bias), state=state.data_ptr(), starts=_p(starts), starts_batch=starts.stride(0) if starts is not None else 0,
-        out=out.data_ptr(), out_batch=out.stride(0), last=state.data_ptr(), batch=batch, length=1, channels=channels, states=A.shape[1],
-        groups=B.shape[1], dtype=_DTYPES[x.dtype], bc_dtype=_DTYPES[B.dtype], softplus=int(bool(softplus)))
-    _launch(_scan_step, desc, "ilx_state_space_step", x.device)
+        x.data_ptr(), x.stride(0), 0, delta.data_ptr(), delta.stride(0), 0, _p(gate), gate.stride(0) if gate is not None else 0, 0, A.data_ptr(),
+        B.data_ptr(), B.stride(0), 0, C.data_ptr(), C.stride(0), 0, _p(D), _p(delta_bias), at, _p(starts),
+        starts.stride(0) if starts is not None else 0, 0, None, out.data_ptr(), out.stride(0), 0, at, None, batch, 1, channels, states, B.shape[1],
+        _DTYPES[x.dtype], _DTYPES[B.dtype], 1 if softplus else 0)
+    _launch(_scan_step, desc, "ilx_state_space_step", index)
     _written((state,))
     return out

@@ -367,6 +367,27 @@ def test_strides_and_alignment(dev):
             assert torch.equal(ref, got), (dt, off)
 
 
+def test_sliding_windows_over_one_series(dev):
+    """x as overlapping rows of one series: time and channels both have stride 1, and so may the batch."""
+    series = torch.randn(3, 60, device=dev)
+    weight = torch.randn(20, 3, device=dev)
+    for view in (series.unfold(1, 20, 1), series[0].unfold(0, 20, 1).unfold(0, 4, 1).transpose(1, 2)):
+        assert view.stride(1) == 1 and view.stride(2) == 1
+        batch, length, _ = view.shape
+        v = some(dev, batch=batch, length=length, channels=20, states=4)
+        results = []
+        for x in (view, view.contiguous()):
+            x = x.detach().requires_grad_(True)
+            state = torch.zeros(batch, 2, 20, device=dev)
+            out = S.short_convolution(x, weight, activation="silu")
+            y, _ = run_scan({**v, "x": x})
+            with torch.no_grad():
+                step = S.short_convolution_step(x[:, 0], state, weight)
+            results.append((out, y, *torch.autograd.grad(out.square().sum() + y.square().sum(), x), step, state))
+        for got, plain in zip(*results):
+            assert torch.equal(got, plain)
+
+
 def wide_of(t):
     """The same values inside wider rows, at an odd column."""
     big = torch.full((*t.shape[:-1], t.shape[-1] + 5), float("nan"), dtype=t.dtype, device=t.device)
