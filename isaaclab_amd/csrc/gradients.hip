@@ -130,7 +130,9 @@ __global__ void __launch_bounds__(256) gradient_scale_kernel(NormArgs a) {
     s = reduce_block(s, maximum);
     const float norm = static_cast<float>(maximum ? s : __builtin_sqrt(s));
     if (a.norm && blockIdx.x == 0 && threadIdx.x == 0) *a.norm = norm;
-    const float ratio = a.max_norm / (norm + 1e-6f);
+    // The reciprocal is rounded ahead of the product, as torch rounds a number over a tensor: one last bit of the scale moves
+    // every 16-bit gradient whose product lies halfway, one in 128 of them, and a run that changes over keeps its results.
+    const float ratio = a.max_norm * (1.0f / (norm + 1e-6f));
     const float scale = ratio > 1.0f ? 1.0f : ratio;   // NaN stays NaN
     if (scale == 1.0f) return;
     const int chunks = a.t.first_chunk[a.t.count];

@@ -1,8 +1,8 @@
 """GPU: global gradient norm and clipping against float64.
 
-The squares are added in 64 bits, so the norm is off by the rounding to float32 and the square root, 2 u relative (u = 2^-24); the
-factor min(1, max_norm / (norm + 1e-6)) adds two roundings and the product one, 5 u in all, and a 16-bit gradient is rounded
-once more, by at most half a step of its type."""
+The squares are added in 64 bits, so the norm is off by the rounding to float32, u = 2^-24 relative (2 u with the 64-bit sums of
+either side); the factor min(1, max_norm (1 / (norm + 1e-6))) adds three roundings and the product one, 5 u in all, and a 16-bit
+gradient is rounded once more, by at most half a step of its type."""
 
 import math
 
@@ -128,6 +128,17 @@ def test_graph_and_command_list(dev):
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(grads, want)), k
         assert abs(float(norm if k % 2 else norm_graph) - norm64(base)) <= 2 * U * norm64(base)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16, torch.float32])
+def test_rounds_as_torch_does(dev, dtype):
+    """The scale has the bits of torch's ``max_norm / (norm + 1e-6)`` in float32, so no 16-bit gradient rounds another way."""
+    for seed in range(8):
+        grads = make(dev, [50_001, 300], [dtype], seed=seed)
+        before = [g.clone() for g in grads]
+        norm = clip_gradient_norm(grads, 7.3 + seed)
+        scale = torch.clamp((7.3 + seed) / (norm + 1e-6), max=1.0)
+        assert all(torch.equal(g, (b.float() * scale).to(dtype)) for g, b in zip(grads, before))
 
 
 def test_two_runs_agree_bit_for_bit(dev):
