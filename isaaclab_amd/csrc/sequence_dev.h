@@ -50,6 +50,9 @@ template <int V, typename T> __device__ __forceinline__ void store_channels(T* p
     *reinterpret_cast<Pack<T, V>*>(p) = w;
 }
 
+constexpr int64_t kMostThreads = (int64_t{1} << 32) - 1024;   // of one launch
+constexpr int32_t kMostChannels = 1 << 23;
+
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
 // The end of a parameter's gradient: `count` rows of (n0 + extra) x channels partial sums, one row per workgroup that kept

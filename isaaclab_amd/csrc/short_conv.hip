@@ -407,6 +407,7 @@ int conv_check(const ilx_short_conv& c, const char* name) {
                 (long long)c.length, c.channels);
     ILX_REQUIRE(c.width >= 1 && c.width <= ILX_CONV_MAX_WIDTH, ILX_ESHAPE, "%s: width %d (1..%d supported)", name, c.width,
                 ILX_CONV_MAX_WIDTH);
+    ILX_REQUIRE(c.channels <= kMostChannels, ILX_ESHAPE, "%s: %d channels", name, c.channels);
     ILX_REQUIRE(c.dtype >= ILX_F32 && c.dtype <= ILX_F16, ILX_EINVAL, "%s: unknown type %d", name, c.dtype);
     ILX_REQUIRE(c.batch <= INT32_MAX && c.length <= INT32_MAX && c.batch * (c.length + 1) < (int64_t{1} << 40), ILX_ESHAPE,
                 "%s: shape (%lld, %lld) too large", name, (long long)c.batch, (long long)c.length);
@@ -470,7 +471,7 @@ extern "C" int ilx_short_conv_forward(const ilx_short_conv* conv, void* stream) 
     ILX_REQUIRE(!c.last || c.last != c.state, ILX_EINVAL, "ilx_short_conv_forward: last and state are the same buffer");
     const int v = conv_vector(c, false);
     const ConvArgs a = conv_args(c, v, false);
-    ILX_REQUIRE(a.slots * a.channel_blocks <= INT32_MAX, ILX_ESHAPE, "ilx_short_conv_forward: shape too large for one launch");
+    ILX_REQUIRE(a.slots * a.channel_blocks * kConvThreads <= kMostThreads, ILX_ESHAPE, "ilx_short_conv_forward: shape too large for one launch");
     conv_dispatch(kForward, a, v, as_stream(stream));
     ILX_LAUNCH_CHECK("ilx_short_conv_forward");
     return ILX_OK;
@@ -517,7 +518,7 @@ extern "C" int ilx_short_conv_step(const ilx_short_conv* conv, void* stream) {
     const int v = conv_vector(c, false);
     ConvArgs a = conv_args(c, v, false);
     a.items = c.batch * a.groups;
-    ILX_REQUIRE((a.items + kConvThreads - 1) / kConvThreads <= INT32_MAX, ILX_ESHAPE, "ilx_short_conv_step: shape too large for one launch");
+    ILX_REQUIRE(a.items <= kMostThreads, ILX_ESHAPE, "ilx_short_conv_step: shape too large for one launch");
     conv_dispatch(kStep, a, v, as_stream(stream));
     ILX_LAUNCH_CHECK("ilx_short_conv_step");
     return ILX_OK;

@@ -359,6 +359,13 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_part_kernel(StateSpaceAr
     p->part_decay[static_cast<int64_t>(k.item) * p->s.channels + c.d] = any ? __builtin_inff() : sum;
 }
 
+// What a part makes of a state: nothing if an episode starts in it, and nothing of a zero state, however far a part of a growing
+// recurrence multiplies it.  (A decay of exactly 0 still hands on a NaN, as every row does.)
+constexpr float kCut = -1.0f;
+__device__ __forceinline__ float pass_on(float decay, float h, float added) {
+    return decay == kCut || h == 0.0f ? added : __builtin_fmaf(decay, h, added);
+}
+
 // Passes the states through the parts: part_state becomes what enters each part (backward: the gradient that enters it from
 // the part behind).  64 states of a sequence to a workgroup, a sixteenth of the parts to each of its waves: a wave joins its own
 // parts, the waves' joins meet in LDS, and each wave passes what enters it through its parts again, out of registers.
@@ -382,25 +389,28 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(StateSpaceArgs a, int b
         decay[j] = in ? a.part_decay[p * s.channels + d] : 0.0f;
         state[j] = in ? a.part_state[p * columns + at] : 0.0f;
     }
-    float D = 1.0f, H = 0.0f;
+    float total = 0.0f, H = 0.0f;
+    bool cut = false;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
-        decay[j] = decay[j] == __builtin_inff() ? 0.0f : __builtin_amdgcn_exp2f(decay[j] * A2);   // a start cuts: exactly 0
-        H = decay[j] == 0.0f ? state[j] : __builtin_fmaf(decay[j], H, state[j]);
-        D *= decay[j];
+        const bool start = decay[j] == __builtin_inff();
+        cut = cut || start;
+        total += start ? 0.0f : decay[j];
+        decay[j] = start ? kCut : __builtin_amdgcn_exp2f(decay[j] * A2);
+        H = pass_on(decay[j], H, state[j]);
     }
-    s_decay[w][lane] = D;
+    s_decay[w][lane] = cut ? kCut : __builtin_amdgcn_exp2f(total * A2);   // (not the product: factors of it may leave the range)
     s_state[w][lane] = H;
     __syncthreads();
     float h = first ? first[b * columns + at] : 0.0f;
-    for (int k = 0; k < w; ++k) h = s_decay[k][lane] == 0.0f ? s_state[k][lane] : __builtin_fmaf(s_decay[k][lane], h, s_state[k][lane]);
+    for (int k = 0; k < w; ++k) h = pass_on(s_decay[k][lane], h, s_state[k][lane]);
     if (!active) return;
 #pragma unroll
     for (int j = 0; j < kPer; ++j) {
         if (j < per && p0 + j < parts) {
             const int64_t p = b * parts + (backward ? parts - 1 - (p0 + j) : p0 + j);
             a.part_state[p * columns + at] = h;
-            h = decay[j] == 0.0f ? state[j] : __builtin_fmaf(decay[j], h, state[j]);
+            h = pass_on(decay[j], h, state[j]);
         }
     }
 }
@@ -452,7 +462,7 @@ int scan_check(const ilx_state_space& s, const char* name) {
     ILX_REQUIRE(s.channels % s.groups == 0, ILX_ESHAPE, "%s: %d channels do not split into %d groups", name, s.channels, s.groups);
     ILX_REQUIRE(s.states >= 1 && s.states <= ILX_SCAN_MAX_STATES, ILX_ESHAPE, "%s: %d states (1..%d supported)", name, s.states,
                 ILX_SCAN_MAX_STATES);
-    ILX_REQUIRE(s.channels <= (1 << 24), ILX_ESHAPE, "%s: %d channels", name, s.channels);
+    ILX_REQUIRE(s.channels <= kMostChannels, ILX_ESHAPE, "%s: %d channels", name, s.channels);
     ILX_REQUIRE(s.dtype >= ILX_F32 && s.dtype <= ILX_F16, ILX_EINVAL, "%s: unknown type %d", name, s.dtype);
     ILX_REQUIRE(s.bc_dtype == ILX_F32 || s.bc_dtype == s.dtype, ILX_EINVAL, "%s: B and C of type %d beside activations of type %d", name,
                 s.bc_dtype, s.dtype);
@@ -460,7 +470,7 @@ int scan_check(const ilx_state_space& s, const char* name) {
                 "%s: shape (%lld, %lld) too large", name, (long long)s.batch, (long long)s.length);
     if (s.length > 1)
         for (const int64_t stride : {s.x_time, s.delta_time, s.gate_time, s.B_time, s.C_time, s.out_time, s.grad_out_time, s.grad_time, s.starts_time})
-            ILX_REQUIRE(stride >= 0 && stride < (int64_t{1} << 26), ILX_ESHAPE, "%s: a time stride of %lld elements", name, (long long)stride);
+            ILX_REQUIRE(stride >= 0 && stride < (int64_t{1} << 27), ILX_ESHAPE, "%s: a time stride of %lld elements", name, (long long)stride);
     return ILX_OK;
 }
 

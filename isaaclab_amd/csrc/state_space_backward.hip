@@ -472,7 +472,7 @@ extern "C" int ilx_state_space_backward(const ilx_state_space* scan, void* strea
     const StateSpaceArgs a = backward_args(s, &needed);
     ILX_REQUIRE(s.workspace_floats >= needed && (s.workspace || needed == 0), ILX_EINVAL,
                 "ilx_state_space_backward: workspace of %lld floats, %lld needed", (long long)s.workspace_floats, (long long)needed);
-    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX - 65536 && s.batch * s.length * s.groups * s.states / 256 < INT32_MAX, ILX_ESHAPE,
+    ILX_REQUIRE(s.batch * a.parts * a.blocks <= INT32_MAX - 65536 && s.batch * s.length * s.groups * s.states < kMostThreads, ILX_ESHAPE,
                 "ilx_state_space_backward: shape too large for one launch");
     hipStream_t st = as_stream(stream);
     if (s.batch > 0) {

@@ -80,8 +80,8 @@ template <typename T> __device__ __forceinline__ void lane_store(__amdgpu_buffer
         __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), row, lane_bytes, row_bytes, 0);
 }
 
-// Rows of one sequence, from a moving first one.  Time strides are below 2^26 elements, so that the offset of one of the next 15
-// rows fits 32 bits.
+// Rows of one sequence, from a moving first one.  Time strides are below 2^27 elements, so that a lane's offset in one of the next
+// seven rows fits 32 bits.
 template <typename T> struct Stream {
     const T* p;
     uint32_t time;   // bytes

@@ -197,6 +197,8 @@ def _check_out(out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
         return _empty_like(x)
     if out.shape != x.shape or out.dtype is not x.dtype or out.device != x.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
         raise ValueError(f"out must be like x ({tuple(x.shape)}, {x.dtype}) with unit channel stride")
+    if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
+        raise ValueError(f"out's rows overlap (strides {out.stride()})")
     return out
 
 

@@ -95,6 +95,8 @@ def test_state_space_refusals():
     fails(S._scan_forward(scan(dtype=7), None), EINVAL, "unknown type 7")
     fails(S._scan_forward(scan(dtype=1, bc_dtype=2), None), EINVAL, "B and C of type 2")
     fails(S._scan_forward(scan(x_time=1 << 32), None), ESHAPE, "time stride")
+    fails(S._scan_forward(scan(out_time=1 << 27), None), ESHAPE, "time stride")
+    fails(S._scan_forward(scan(channels=(1 << 23) + 8), None), ESHAPE, "8388616 channels")
     fails(S._scan_forward(scan(length=2000, channels=64), None), EINVAL, "workspace")
     fails(S._scan_forward(scan(state=FAKE, last=FAKE), None), EINVAL, "same buffer")
     assert S._scan_forward(scan(batch=0, x=None), None) == 0

@@ -154,6 +154,9 @@ SCAN = [  # batch, length, channels, states, groups, dtype, shared in float32, g
     (2, 130, 72, 16, 1, 0, False, False, False, True, True, True, False),
     (1, 700, 32, 16, 1, 0, False, True, True, False, False, True, False),
     (3, 555, 24, 6, 1, 1, False, True, True, True, True, True, False),
+    (2, 333, 70, 24, 2, 1, True, True, True, True, True, True, True),
+    (1, 520, 40, 32, 1, 0, False, True, False, False, False, True, False),
+    (2, 96, 12, 3, 4, 2, False, False, True, True, False, False, False),
 ]
 
 
@@ -428,6 +431,32 @@ def test_extreme_step_sizes(dev):
     assert abs(float(small[0, 0, 0]) / float(want) - 1) < 60 * U     # relative: all of the step size's bits are there
 
 
+def test_what_is_not_finite_in_a_divided_sequence(dev):
+    """A divided sequence hands on what the rows would: zeros through parts that grow past the range, NaN and infinity through parts
+    that shrink everything else to nothing, and nothing over a start."""
+    gen = torch.Generator().manual_seed(1)
+    length, channels, states = 1000, 64, 4
+    x, B, C = torch.randn(1, length, channels, generator=gen), torch.randn(1, length, 1, states, generator=gen), torch.randn(1, length, 1, states, generator=gen)
+    delta, A = torch.ones(1, length, channels), torch.ones(channels, states) * 4
+    x[:, :990] = 0
+    on = lambda *t: [v.to(dev) for v in t]  # noqa: E731
+    out, last = S.state_space_scan(*on(x, delta, A, B, C), softplus=False, return_state=True)
+    want, state = O.state_space_scan(*(t.double() for t in (x, delta, A, B, C)), softplus=False)
+    magnitude, state_magnitude = O.state_space_scan(x.double().abs(), delta.double(), A.double(), B.double().abs(), C.double().abs(), softplus=False)
+    assert not out[:, :990].any()
+    # per row 40 |dt A| + 2 roundings of the decay, ten rows; the sums of 4 terms
+    close(out, want, magnitude, 10 * 162 + 10, "out")
+    close(last, state, state_magnitude, 10 * 162 + 10, "last")
+
+    starts = torch.zeros(1, length, dtype=torch.bool)
+    starts[:, 800] = True
+    for value in (float("nan"), float("inf")):
+        x = torch.randn(1, length, channels, generator=gen)
+        x[0, 10, 7] = value
+        got = S.state_space_scan(*on(x, delta, -A, B, C), softplus=False, starts=starts.to(dev)).isfinite().cpu()
+        assert not got[0, 10:800, 7].any() and got[0, 800:].all() and got[0, :10].all() and got[..., :7].all() and got[..., 8:].all()
+
+
 def test_a_directional_difference(dev):
     """The gradient against differences of the kernel's own forward: of a smooth function with terms of order 1 a central
     difference with step 1/64 is off by step^2 / 6 of the third derivative (here under 1e-2) and 2 * rounding / step (1e-4)."""
@@ -542,6 +571,45 @@ def test_a_training_step_in_a_graph(dev):
             assert all(torch.equal(a, b) for a, b in zip(eager, want[(i + 1) % 3]))
 
 
+def test_parameters_and_a_divided_sequence_in_a_graph(dev):
+    """A whole step of parameters' ``.grad``, the way a training loop captures it, with a sequence long enough to be divided."""
+    v = some(dev, batch=2, length=300, channels=70)
+    names = ("A", "B", "C", "D", "delta_bias")
+    x, grad = v["x"].clone(), torch.randn(2, 300, 70, device=dev)
+    w = torch.nn.Parameter(torch.randn(70, 4, device=dev))
+    p = {k: torch.nn.Parameter(v[k].clone()) for k in names}
+    leaves = [w, *p.values()]
+
+    def step():
+        u = S.short_convolution(x, w, activation="silu")
+        out, _ = run_scan({**v, **p, "x": u})
+        out.backward(grad)
+
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        step()
+    torch.cuda.current_stream().wait_stream(side)
+    for t in leaves:
+        t.grad = None
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        step()
+    results = [t.grad for t in leaves]
+    for k in range(3):
+        x.copy_(torch.randn(2, 300, 70, device=dev, generator=torch.Generator(dev).manual_seed(k)))
+        for t in leaves:
+            t.grad.zero_()
+        graph.replay()
+        got = [t.clone() for t in results]
+        torch.cuda.synchronize()
+        eager_x, eager = x.clone(), [t.detach().clone().requires_grad_(True) for t in leaves]
+        u = S.short_convolution(eager_x, eager[0], activation="silu")
+        out, _ = run_scan({**v, **dict(zip(names, eager[1:])), "x": u})
+        want = torch.autograd.grad(out, eager, grad)
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
 def test_on_another_stream(dev):
     v = some(dev, batch=4, length=600, channels=64)
     want = run_scan(v)
@@ -621,6 +689,7 @@ def test_refusals(dev):
     refused("carried state", step, x[:, 0], None, w)
     refused("contiguous", step, x[:, 0], torch.zeros(2, 8, 3, device=dev).transpose(1, 2), w)
     refused("out must", step, x[:, 0], torch.zeros(2, 3, 8, device=dev), w, out=x[:, 0].half())
+    refused("overlap", step, x[:, 0], torch.zeros(2, 3, 8, device=dev), w, out=torch.zeros(8, device=dev).expand(2, 8))
     refused("no backward", step, x[:, 0], torch.zeros(2, 3, 8, device=dev), w.clone().requires_grad_(True), error=RuntimeError)
     refused("no backward", S.state_space_step, x[:, 0], x[:, 0], s.clone().requires_grad_(True), w, bc[:, 0], bc[:, 0], error=RuntimeError)
     # a state that a backward pass still needs is not silently the wrong one
