@@ -5,6 +5,8 @@
 // of 1e30 has a norm and small gradients beside large ones count; the adds hide behind the loads.
 // The tensors' pointers and sizes travel as kernel arguments, kTensors of them to a launch: no table in device memory that
 // would have to be copied or kept for a replay.
+// Measured, 200 tensors of 200 M bf16 elements together: 96 us for the sums (400 MB, 4.2 TB/s) and 137 to scale (800 MB; half of what
+// it reads is still in the last-level cache), against 4.97 TB/s of a large copy.  16 tensors of a policy (572 K f32): 6.5 and 6 us.
 #include "sequence_dev.h"
 
 #include <algorithm>

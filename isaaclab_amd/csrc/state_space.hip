@@ -9,6 +9,13 @@
 // for what it adds to the state, a join passes the states through all parts (a part as a whole multiplies a state by
 // exp(A sum dt)), and every part runs again from the state that enters it.  That costs a second pass of exponentials and buys
 // up to 256 times the waves.
+// Measured with 16 states, against a large copy's 4.97 TB/s:
+//   24 x 4096 x 256 f32, gate, state in and out: 136 us, 537 MB, 3.9 TB/s; with the states a backward pass needs 150 us, 738 MB, 4.9
+//   TB/s: bound by memory
+//   1 x 16384 x 1024 bf16 in 256 parts: 57 us for the parts, 11 for the join, 80 for the rows; 134 MB of operands, so bound by the
+//   vector unit (part kernel: 78 instructions a row and wave, 52 of them the recurrence; the unit is busy 81 % of the time)
+//   undivided, the same call takes 19 ms
+//   step, 16384 x 256 bf16: 112 us on states that are not cached (571 MB, 5.1 TB/s), 91 in a loop on one state
 #include "state_space_dev.h"
 #include "uniform_access.h"
 
@@ -16,6 +23,7 @@ namespace ilx {
 
 constexpr int kScanRows = 4;    // rows whose inputs are in registers together; divides ILX_SCAN_BLOCK
 constexpr int kMostParts = 256;
+constexpr int kJoinParts = 16;   // of a wave in the join
 constexpr int kScanWaves = 4;   // to a workgroup: independent, but a workgroup puts one on each SIMD of its CU (single waves end up
                                 // unevenly: two thirds of the waves that fit were resident on average)
 
@@ -367,11 +375,10 @@ __device__ __forceinline__ float pass_on(float decay, float h, float added) {
 }
 
 // Passes the states through the parts: part_state becomes what enters each part (backward: the gradient that enters it from
-// the part behind).  64 states of a sequence to a workgroup, a sixteenth of the parts to each of its waves: a wave joins its own
-// parts, the waves' joins meet in LDS, and each wave passes what enters it through its parts again, out of registers.
+// the part behind).  64 states of a sequence to a workgroup, up to 16 parts to each of its waves: a wave joins its own parts, the
+// waves' joins meet in LDS, and each wave passes what enters it through its parts again, out of registers.
 __global__ void __launch_bounds__(1024) scan_join_kernel(StateSpaceArgs a, int backward, const float* first) {
-    constexpr int kWaves = 16, kPer = kMostParts / kWaves;
-    __shared__ float s_decay[kWaves][64], s_state[kWaves][64];
+    __shared__ float s_decay[kMostParts / kJoinParts][64], s_state[kMostParts / kJoinParts][64];
     const ilx_state_space& s = a.s;
     const int lane = threadIdx.x & 63, w = threadIdx.x >> 6;
     const int columns = s.states * s.channels, column_blocks = (columns + 63) / 64;
@@ -379,11 +386,11 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(StateSpaceArgs a, int b
     const int column = static_cast<int>(blockIdx.x % column_blocks) * 64 + lane;
     const bool active = column < columns;
     const int at = active ? column : columns - 1, n = at / s.channels, d = at - n * s.channels;
-    const int parts = static_cast<int>(a.parts), per = (parts + kWaves - 1) / kWaves, p0 = w * per;
+    const int parts = static_cast<int>(a.parts), waves = blockDim.x >> 6, per = (parts + waves - 1) / waves, p0 = w * per;
     const float A2 = s.A[static_cast<int64_t>(d) * s.states + n] * kLog2e;
-    float decay[kPer], state[kPer];
+    float decay[kJoinParts], state[kJoinParts];
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < kJoinParts; ++j) {
         const bool in = j < per && p0 + j < parts;
         const int64_t p = b * parts + (backward ? parts - 1 - (p0 + j) : p0 + j);
         decay[j] = in ? a.part_decay[p * s.channels + d] : 0.0f;
@@ -392,7 +399,7 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(StateSpaceArgs a, int b
     float total = 0.0f, H = 0.0f;
     bool cut = false;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < kJoinParts; ++j) {
         const bool start = decay[j] == __builtin_inff();
         cut = cut || start;
         total += start ? 0.0f : decay[j];
@@ -406,7 +413,7 @@ __global__ void __launch_bounds__(1024) scan_join_kernel(StateSpaceArgs a, int b
     for (int k = 0; k < w; ++k) h = pass_on(s_decay[k][lane], h, s_state[k][lane]);
     if (!active) return;
 #pragma unroll
-    for (int j = 0; j < kPer; ++j) {
+    for (int j = 0; j < kJoinParts; ++j) {
         if (j < per && p0 + j < parts) {
             const int64_t p = b * parts + (backward ? parts - 1 - (p0 + j) : p0 + j);
             a.part_state[p * columns + at] = h;
@@ -493,16 +500,21 @@ StateSpaceArgs scan_args(const ilx_state_space& s) {
     return a;
 }
 
-// Two waves per SIMD hide a row's latency well enough that a second pass does not pay; below that a sequence is divided towards
-// four per SIMD, in parts of at least 32 rows (a part's cost ahead of its first row is that of about eight).
+// With a wave on every SIMD a sequence is not divided: a wave alone on a SIMD takes 430 ns for a row of 16 states, four together 650 for
+// four, and the second pass costs as much again (400 x 100 rows x 256 channels: 69 us, in two parts 128; 256 x 500 x 256: 276 against 258).
+// Below that it is divided towards four waves a SIMD (128 x 500 x 256: 139 us, undivided 260), short ones only where the chip would be
+// three quarters empty (128 x 64 x 256 with gradients: 82 us, divided 105; 1 x 64 x 256: 27 us, divided 15).  A part has at least 16
+// rows, or 8 while parts of 16 leave half of the SIMDs without a wave (1 x 512 x 512: 18 us with 8, 23 with 16, 33 with 32; 4 x 215 x 1150:
+// 30, 28 and 35).  More than 256 parts gain nothing and take 31 us for the join in the place of 11.
 int64_t divide_scan(StateSpaceArgs& a, float* workspace) {
     const ilx_state_space& s = a.s;
     const int64_t waves = s.batch * a.blocks, full = 4 * device_cu_count();   // one per SIMD
-    if (waves == 0 || waves >= 2 * full || s.length < 64) return 0;
+    if (waves == 0 || waves >= full || s.length < (waves > full / 4 ? 128 : 64)) return 0;
     int64_t parts = 4 * full / waves;
     if (parts > kMostParts) parts = kMostParts;
+    const int64_t least = waves * ((s.length + 15) / 16) > full / 2 ? 16 : ILX_SCAN_BLOCK;
     int64_t rows = (s.length + parts - 1) / parts;
-    if (rows < 32) rows = 32;
+    if (rows < least) rows = least;
     rows = (rows + ILX_SCAN_BLOCK - 1) / ILX_SCAN_BLOCK * ILX_SCAN_BLOCK;
     a.part_rows = rows, a.parts = (s.length + rows - 1) / rows;
     if (a.parts == 1) return 0;
@@ -553,7 +565,7 @@ void scan_dispatch(ScanKind kind, const StateSpaceArgs& a, hipStream_t s) {
 void ilx::launch_part_states(const StateSpaceArgs& a, bool backward, hipStream_t s) {
     scan_dispatch(backward ? kPartsBackward : kParts, a, s);
     const int64_t column_blocks = (static_cast<int64_t>(a.s.states) * a.s.channels + 63) / 64;
-    ILX_LAUNCH(scan_join_kernel, dim3(static_cast<unsigned>(a.s.batch * column_blocks)), dim3(1024), 0, s, a, backward ? 1 : 0,
+    ILX_LAUNCH(scan_join_kernel, dim3(static_cast<unsigned>(a.s.batch * column_blocks)), dim3(blocks_for(a.parts, kJoinParts) * 64), 0, s, a, backward ? 1 : 0,
                backward ? a.s.grad_last : a.s.state);
 }
 
