@@ -10,6 +10,7 @@ from __future__ import annotations
 
 import contextlib
 import math
+import operator
 from array import array
 from collections.abc import Iterable
 from ctypes import c_float, c_int32, c_int64
@@ -20,6 +21,7 @@ from .. import _abi
 from .sequence import _DTYPES, _current_device, _written
 
 _norm = _abi._sig("ilx_gradient_norm", _abi.P, _abi.P, _abi.P, c_int32, c_int32, c_int32, c_float, _abi.P, _abi.P, c_int64, _abi.P)
+_T, _dtype, _KIND = torch.Tensor, operator.attrgetter("dtype"), _DTYPES.get
 _WORKSPACE = 4096   # floats, what ilx_gradient_norm_workspace says for any list
 
 
@@ -40,8 +42,8 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
     if not first.is_cuda:
         raise _abi.IlxError("isaaclab_amd kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")
     index = first.get_device()
-    kinds = [_DTYPES.get(g.dtype, -1) for g in tensors]
-    if min(kinds) < 0 or not all([g.is_contiguous() and g.get_device() == index for g in tensors]):
+    kinds = list(map(_KIND, map(_dtype, tensors)))   # (map: a training step may have hundreds of tensors)
+    if None in kinds or set(map(_T.get_device, tensors)) != {index} or not all(map(_T.is_contiguous, tensors)):
         for i, g in enumerate(tensors):
             if g.get_device() != index:
                 raise ValueError(f"gradient {i} is on {g.device}, the first on {first.device}")
@@ -49,7 +51,7 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
                 raise ValueError(f"gradient {i} is {g.dtype}: float32, bfloat16 or float16 expected")
             if g.layout != torch.strided or not _is_dense(g):
                 raise ValueError(f"gradient {i} is not dense: strides {g.stride() if g.layout == torch.strided else g.layout} of shape {tuple(g.shape)}")
-    pointers, sizes, dtypes = array("q", [g.data_ptr() for g in tensors]), array("q", [g.numel() for g in tensors]), array("i", kinds)
+    pointers, sizes, dtypes = array("q", map(_T.data_ptr, tensors)), array("q", map(_T.numel, tensors)), array("i", kinds)
     norm = _abi.keep(torch.empty((), device=first.device))
     workspace = _abi.keep(torch.empty(_WORKSPACE, device=first.device))
     with contextlib.nullcontext() if index == _current_device() else torch.cuda.device(index):

@@ -217,9 +217,9 @@ def _keep(*tensors):
 
 def _written(tensors):
     """Autograd sees the in-place update: a backward pass that needs a value from before it fails loudly."""
-    tensors = [t for t in tensors if not t.is_inference()]
-    if tensors:
-        torch.autograd.graph.increment_version(tensors)
+    if any(map(torch.Tensor.is_inference, tensors)):
+        tensors = [t for t in tensors if not t.is_inference()]
+    torch.autograd.graph.increment_version(tensors)
 
 
 def _moved(desc, **pointers) -> bool:
