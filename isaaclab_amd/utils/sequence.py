@@ -222,9 +222,18 @@ def _written(tensors):
     torch.autograd.graph.increment_version(tensors)
 
 
-def _moved(desc, **pointers) -> bool:
-    """Whether a saved tensor came back from another place than the forward pass saw it (hooks may pack saved tensors)."""
-    return any(getattr(desc, name) != _p(t) for name, t in pointers.items())
+def _places(tensors) -> list:
+    return [None if t is None else (t.data_ptr(), t.stride()) for t in tensors]
+
+
+def _once(backward):
+    """A backward pass that cannot be differentiated again; without ``create_graph`` there is nothing to guard."""
+    guarded = once_differentiable(backward)
+
+    def either(ctx, *grads):
+        return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
+
+    return either
 
 
 # ---- short convolution ----------------------------------------------------------------------------------------------
@@ -259,16 +268,18 @@ class _ShortConvolution(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, weight, bias, state, starts, lengths, silu, want_last):
         ctx.set_materialize_grads(False)
-        ctx.save_for_backward(x, weight, bias, state, starts, lengths)
+        saved = (x, weight, bias, state, starts, lengths)
+        ctx.save_for_backward(*saved)
+        ctx.places = _places(saved)
         out, last, ctx.desc = _conv_call(x, weight, bias, state, starts, lengths, silu, want_last)
         return out, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out, grad_last):
-        x, weight, bias, state, starts, lengths = ctx.saved_tensors
+        x, weight, bias, state, starts, lengths = saved = ctx.saved_tensors
         d = ctx.desc
-        if _moved(d, x=x, weight=weight, bias=bias, state=state, starts=starts, lengths=lengths):
+        if _places(saved) != ctx.places:   # (hooks may pack saved tensors and unpack them elsewhere)
             d = _conv_desc(x, weight, bias, state, starts, lengths, d.silu)
         index = x.get_device()
         grad_out = torch.zeros_like(x) if grad_out is None else _check_activation(grad_out, "the output's gradient", x, index)
@@ -408,17 +419,19 @@ class _StateSpaceScan(torch.autograd.Function):
     def forward(ctx, x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last):
         ctx.set_materialize_grads(False)
         out, last, saved, ctx.desc = _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, softplus, want_last, True)
-        ctx.save_for_backward(x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved)
+        kept = (x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved)
+        ctx.save_for_backward(*kept)
+        ctx.places = _places(kept)
         ctx.has_state = state is not None
         return out, last
 
     @staticmethod
-    @once_differentiable
+    @_once
     def backward(ctx, grad_out, grad_last):
-        x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved = ctx.saved_tensors
+        x, delta, A, B, C, D, gate, delta_bias, starts, lengths, saved = kept = ctx.saved_tensors
         d = ctx.desc
         rB, rC = _pair(B, C)
-        if _moved(d, x=x, delta=delta, A=A, B=rB, C=rC, D=D, gate=gate, delta_bias=delta_bias, starts=starts, lengths=lengths, saved=saved):
+        if _places(kept) != ctx.places or rB is not B or rC is not C:   # (hooks may pack saved tensors and unpack them elsewhere)
             d = _scan_desc(x, delta, A, rB, rC, D, gate, delta_bias, None, starts, lengths, d.softplus)
             d.saved = saved.data_ptr()
         index, device = x.get_device(), x.device

@@ -10,6 +10,7 @@ rounded once more, by at most half a step of its type.  Sums over channels, stat
 
 import pytest
 import torch
+import torch.utils.checkpoint
 
 from isaaclab_amd import _abi
 from isaaclab_amd.utils import sequence as S
@@ -429,6 +430,41 @@ def test_extreme_step_sizes(dev):
     small = S.state_space_scan(x[:, :1], torch.full_like(x[:, :1], -16.0), a, b[:, :1], b[:, :1] / 4)
     want = torch.log1p(torch.exp(torch.tensor(-16.0, dtype=torch.float64)))
     assert abs(float(small[0, 0, 0]) / float(want) - 1) < 60 * U     # relative: all of the step size's bits are there
+
+
+def test_saved_tensors_that_move_and_second_derivatives(dev):
+    """Packed and unpacked saved tensors (other addresses and strides), checkpointing, and no silent second derivative."""
+    v = some(dev, batch=3, length=70, channels=20)
+    v["x"] = v["x"].transpose(0, 1).contiguous().transpose(0, 1)
+    w, names = torch.randn(20, 4, device=dev), ("x", "delta", "A", "B", "C", "D", "delta_bias", "state")
+
+    def run(leaves):
+        u = S.short_convolution(leaves["x"], w, activation="silu")
+        return run_scan({**v, **leaves, "x": u})[0]
+
+    def gradients(how):
+        leaves = {k: v[k].detach().clone(memory_format=torch.preserve_format).requires_grad_(True) for k in names}
+        return torch.autograd.grad(how(leaves).square().sum(), list(leaves.values()))
+
+    want = gradients(run)
+
+    def on_cpu(leaves):
+        with torch.autograd.graph.save_on_cpu():
+            return run(leaves)
+
+    def checkpointed(leaves):
+        return torch.utils.checkpoint.checkpoint(run, leaves, use_reentrant=False)
+
+    def doubled(leaves):   # unpacked beside other values: other strides, perhaps the old address
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: torch.stack([t, t], -1).cpu(), lambda t: t.to(dev)[..., 0].contiguous()):
+            return run(leaves)
+
+    for how in (on_cpu, checkpointed, doubled):
+        assert all(torch.equal(a, b) for a, b in zip(gradients(how), want)), how.__name__
+    x = v["x"].clone().requires_grad_(True)
+    first, = torch.autograd.grad(S.short_convolution(x, w, activation="silu").square().sum(), x, create_graph=True)
+    with pytest.raises(RuntimeError, match="differentiat"):
+        torch.autograd.grad(first.sum(), x)
 
 
 def test_what_is_not_finite_in_a_divided_sequence(dev):
