@@ -10,7 +10,7 @@
 // exp(A sum dt)), and every part runs again from the state that enters it.  That costs a second pass of exponentials and buys
 // up to 256 times the waves.
 // Measured with 16 states, against a large copy's 4.97 TB/s:
-//   24 x 4096 x 256 f32, gate, state in and out: 136 us, 537 MB, 3.9 TB/s; with the states a backward pass needs 150 us, 738 MB, 4.9
+//   24 x 4096 x 256 f32, gate, state in and out: 133 us, 537 MB, 4.0 TB/s; with the states a backward pass needs 147 us, 738 MB, 5.0
 //   TB/s: bound by memory
 //   1 x 16384 x 1024 bf16 in 256 parts: 57 us for the parts, 11 for the join, 80 for the rows; 134 MB of operands, so bound by the
 //   vector unit (part kernel: 78 instructions a row and wave, 52 of them the recurrence; the unit is busy 81 % of the time)
@@ -97,6 +97,14 @@ template <typename T, typename TB, int W, bool WITH_GATE, bool WITH_DOT> struct 
         for (int j = 0; j < W; ++j) o[j] = lane_load<TB>(bo, row + o_state[j], 0);
         start = 0;
         if ((k.flags & kHasStarts) && lane < count) start = k.starts.p[lane * k.starts.time];
+    }
+    __device__ __forceinline__ void arrived() {
+        arrive(x), arrive(delta), arrive(o), arrive(start);
+        if (WITH_GATE) arrive(gate);
+        if (WITH_DOT) {
+#pragma unroll
+            for (int i = 0; i < kScanRows; ++i) arrive(c[i]);
+        }
     }
     __device__ __forceinline__ uint32_t starts() const { return static_cast<uint32_t>(__ballot(start != 0)); }   // a bit a row
 };
@@ -202,7 +210,8 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_forward_kernel(StateSpac
     const int items = static_cast<int>(a.s.batch * a.parts), slots = static_cast<int>(a.slots);
     f32x4 A2[V], h[V];
     load_decays<V>(a, c.d, A2);
-    const float bias = a.s.delta_bias ? a.s.delta_bias[c.d] : 0.0f, skip = a.s.D ? a.s.D[c.d] : 0.0f;
+    float bias = a.s.delta_bias ? a.s.delta_bias[c.d] : 0.0f, skip = a.s.D ? a.s.D[c.d] : 0.0f;
+    arrive(bias), arrive(skip);
     ScanRows<T, TB, W, true, true> rows;
     ScanStreams<T, TB> k;
     k.flags = scan_flags<V>(a.s);
@@ -260,6 +269,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_forward_kernel(StateSpac
 #pragma unroll
                 for (int i = 0; i < kScanRows; ++i) y[i] *= z[i] * sigmoid_fast(z[i]);
             }
+            rows.arrived();
             if (c.active) {
 #pragma unroll
                 for (int i = 0; i < kScanRows; ++i)
@@ -500,12 +510,12 @@ StateSpaceArgs scan_args(const ilx_state_space& s) {
     return a;
 }
 
-// With a wave on every SIMD a sequence is not divided: a wave alone on a SIMD takes 430 ns for a row of 16 states, four together 650 for
-// four, and the second pass costs as much again (400 x 100 rows x 256 channels: 69 us, in two parts 128; 256 x 500 x 256: 276 against 258).
-// Below that it is divided towards four waves a SIMD (128 x 500 x 256: 139 us, undivided 260), short ones only where the chip would be
-// three quarters empty (128 x 64 x 256 with gradients: 82 us, divided 105; 1 x 64 x 256: 27 us, divided 15).  A part has at least 16
-// rows, or 8 while parts of 16 leave half of the SIMDs without a wave (1 x 512 x 512: 18 us with 8, 23 with 16, 33 with 32; 4 x 215 x 1150:
-// 30, 28 and 35).  More than 256 parts gain nothing and take 31 us for the join in the place of 11.
+// With a wave on every SIMD a sequence is not divided: a wave alone on a SIMD takes 420 ns for a row of 16 states, two together 650 for
+// two, four 1190 for four, and the second pass costs as much again (400 x 100 rows x 256 channels: 65 us, in two parts 128; 256 x 500 x
+// 256: 211 against 258).  Below that it is divided towards four waves a SIMD (128 x 500 x 256: 136 us, undivided 260), short ones only
+// where the chip would be three quarters empty (128 x 64 x 256 with gradients: 78 us, divided 105; 1 x 64 x 256: 27 us, divided 15).  A
+// part has at least 16 rows, or 8 while parts of 16 leave half of the SIMDs without a wave (1 x 512 x 512: 18 us with 8, 23 with 16, 33
+// with 32; 4 x 215 x 1150: 30, 27 and 35).  More than 256 parts gain nothing and take 31 us for the join in the place of 11.
 int64_t divide_scan(StateSpaceArgs& a, float* workspace) {
     const ilx_state_space& s = a.s;
     const int64_t waves = s.batch * a.blocks, full = 4 * device_cu_count();   // one per SIMD

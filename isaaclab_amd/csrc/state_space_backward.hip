@@ -13,9 +13,9 @@
 //  * sums over the channels (dB, dC) are first halved twice inside 16 lanes, each step leaving half of the lanes one value and
 //    half another (twelve adds for eight values, where a plain tree takes 32); what is left, 16 numbers of a workgroup's four waves
 //    (64 channels) to a result, is added from LDS behind the block's one barrier.
-// Measured, 24 x 4096 x 256 f32 with gate and 16 states: 410 us (16 for the sums of dB and dC over blocks of channels, 6 for the
+// Measured, 24 x 4096 x 256 f32 with gate and 16 states: 402 us (16 for the sums of dB and dC over blocks of channels, 6 for the
 // parameters), 0.97 GB, 2.4 TB/s.  Bound by instructions: 89 in the vector unit for a row and wave (four states a lane), which is
-// busy 70 % of the time with three waves on a SIMD; without the loads it takes 348 us, without the stores 379.
+// busy 70 % of the time with three waves on a SIMD.  Reads that were waited for behind the stores took 411.
 #include "state_space_dev.h"
 
 namespace ilx {
@@ -146,7 +146,8 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
         A2[j] = n < states ? s.A[static_cast<int64_t>(d) * states + n] * kLog2e : 0.0f;
         dA[j] = 0.0f;
     }
-    const float bias = s.delta_bias ? s.delta_bias[d] : 0.0f, skip = s.D ? s.D[d] : 0.0f;
+    float bias = s.delta_bias ? s.delta_bias[d] : 0.0f, skip = s.D ? s.D[d] : 0.0f;
+    arrive(A2), arrive(bias), arrive(skip);
     float dD = 0.0f, dbias = 0.0f;
     // where the lane's values are: its channel, its quarter's states (clamped to the last), its element of the operands
     const uint32_t channel = static_cast<uint32_t>(d) * sizeof(T);
@@ -217,8 +218,17 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
         if (p->s.starts && lane < k.count) in_start = (p->s.starts + k.b * p->s.starts_batch + k.t0 * p->s.starts_time)[lane * p->s.starts_time];
     };
 
+    auto arrived = [&] {
+        arrive(in_d), arrive(in_x), arrive(in_g), arrive(in_z), arrive(in_h), arrive(in_start);
+#pragma unroll
+        for (int e = 0; e < 2; ++e) arrive(in_B[e]), arrive(in_C[e]);
+    };
+
     ScanBlock k = item_end(slot);
-    if (k.count > 0) read(k);
+    if (k.count > 0) {
+        read(k);
+        arrived();
+    }
     float r[S];
     bool fresh = true;
     int buffer = 0;
@@ -233,6 +243,7 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
                 const auto from = row_buffer(enters);
 #pragma unroll
                 for (int j = 0; j < S; ++j) r[j] = active && S * quarter + j < states ? lane_load<float>(from, state_at[j], 0) : 0.0f;
+                arrive(r);
             }
             const int length = static_cast<int>(p->s.length), part_rows = static_cast<int>(p->part_rows), limit = k.begin + part_rows < length ? k.begin + part_rows : length;
             for (int t = (k.end > k.begin ? k.end : k.begin) + quarter; t < limit; t += 4) {
@@ -334,6 +345,7 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
                 walk(std::true_type{});
             else
                 walk(std::false_type{});
+            arrived();
             {
                 const ArgsPtr p = arguments_again();
                 const uint32_t time = static_cast<uint32_t>(p->s.grad_time) * sizeof(T);
@@ -369,6 +381,7 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
             buffer ^= 1;   // (this one is written again behind the next block's barrier)
         } else if (next.count > 0) {
             read(next);
+            arrived();
         }
         fresh = next.item != k.item;
         if (fresh && k.begin == 0 && s.grad_state && active) {

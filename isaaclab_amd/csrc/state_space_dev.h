@@ -80,6 +80,26 @@ template <typename T> __device__ __forceinline__ void lane_store(__amdgpu_buffer
         __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(uint16_t, v), row, lane_bytes, row_bytes, 0);
 }
 
+// Here the value has arrived.  Loads and stores come back in one order and a wait counts what may still be out, so a value read ahead is
+// waited for before the stores that follow: a wait behind them, at the value's use, would be one for the stores as well.
+template <typename T> __device__ __forceinline__ void arrive(T& v) {
+    if constexpr (sizeof(T) == 4) {
+        asm volatile("" : "+v"(v));
+    } else if constexpr (sizeof(T) == 2) {
+        uint32_t u = __builtin_bit_cast(uint16_t, v);
+        asm volatile("" : "+v"(u));
+        v = __builtin_bit_cast(T, static_cast<uint16_t>(u));
+    } else {
+        uint32_t u = v;
+        asm volatile("" : "+v"(u));
+        v = static_cast<T>(u);
+    }
+}
+template <typename T, int N> __device__ __forceinline__ void arrive(T (&v)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; ++i) arrive(v[i]);
+}
+
 // Rows of one sequence, from a moving first one.  Time strides are below 2^27 elements, so that a lane's offset in one of the next
 // seven rows fits 32 bits.
 template <typename T> struct Stream {
