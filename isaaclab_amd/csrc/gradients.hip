@@ -38,17 +38,22 @@ struct NormArgs {
 };
 static_assert(sizeof(NormArgs) <= 4096 - 256, "kernel arguments");
 
-__device__ __forceinline__ int find_tensor(const TensorTable& t, int chunk) {
-    int lo = 0, hi = t.count - 1;   // the last entry whose first chunk is not past `chunk`
-    while (lo < hi) {
-        const int mid = (lo + hi + 1) >> 1;
-        if (t.first_chunk[mid] <= chunk)
-            lo = mid;
-        else
-            hi = mid - 1;
+// The entry of a chunk: the last one whose first chunk is not past it.  A wave holds all first chunks, read together (a search of the
+// table would wait for one read of the arguments after the other), and counts.
+struct ChunkFinder {
+    int32_t first[(kTensors + 63) / 64];
+    __device__ __forceinline__ explicit ChunkFinder(const TensorTable& t) {
+        const int lane = threadIdx.x & 63;
+#pragma unroll
+        for (int k = 0; k < (kTensors + 63) / 64; ++k) first[k] = 64 * k + lane < t.count ? t.first_chunk[64 * k + lane] : INT32_MAX;
     }
-    return lo;
-}
+    __device__ __forceinline__ int operator()(int chunk) const {
+        int n = 0;
+#pragma unroll
+        for (int k = 0; k < (kTensors + 63) / 64; ++k) n += __popcll(__ballot(first[k] <= chunk));
+        return n - 1;
+    }
+};
 
 // Calls f(value) for the elements of a chunk that fall to this thread, and with STORE writes back what it returns.
 template <bool STORE, typename T, typename F> __device__ __forceinline__ void each_element(T* p, uint32_t n, F f) {
@@ -84,8 +89,8 @@ template <bool STORE, typename T, typename F> __device__ __forceinline__ void ea
     }
 }
 
-template <bool STORE, typename F> __device__ __forceinline__ void each_in_chunk(const TensorTable& t, int chunk, F f) {
-    const int i = find_tensor(t, chunk);
+template <bool STORE, typename F> __device__ __forceinline__ void each_in_chunk(const TensorTable& t, const ChunkFinder& entry_of, int chunk, F f) {
+    const int i = entry_of(chunk);
     const uint32_t at = static_cast<uint32_t>(chunk - t.first_chunk[i]) * kChunk, left = t.size[i] - at;
     const uint32_t n = left < kChunk ? left : kChunk;
     switch (t.dtype[i]) {
@@ -115,8 +120,9 @@ __global__ void __launch_bounds__(256) gradient_partials_kernel(NormArgs a) {
     double s = 0.0;
     const int chunks = a.t.first_chunk[a.t.count];
     const bool maximum = a.maximum;
+    const ChunkFinder entry_of(a.t);
     for (int chunk = blockIdx.x; chunk < chunks; chunk += a.partials_here)
-        each_in_chunk<false>(a.t, chunk, [&](float v) {
+        each_in_chunk<false>(a.t, entry_of, chunk, [&](float v) {
             const double d = v;
             s = maximum ? larger(__builtin_fabs(d), s) : __builtin_fma(d, d, s);
             return v;
@@ -127,6 +133,7 @@ __global__ void __launch_bounds__(256) gradient_partials_kernel(NormArgs a) {
 
 __global__ void __launch_bounds__(256) gradient_scale_kernel(NormArgs a) {
     const bool maximum = a.maximum;
+    const ChunkFinder entry_of(a.t);
     double s = 0.0;
     for (int i = threadIdx.x; i < a.partials_all; i += 256) s = maximum ? larger(a.partials[i], s) : s + a.partials[i];
     s = reduce_block(s, maximum);
@@ -138,7 +145,7 @@ __global__ void __launch_bounds__(256) gradient_scale_kernel(NormArgs a) {
     const float scale = ratio > 1.0f ? 1.0f : ratio;   // NaN stays NaN
     if (scale == 1.0f) return;
     const int chunks = a.t.first_chunk[a.t.count];
-    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) each_in_chunk<true>(a.t, chunk, [&](float v) { return v * scale; });
+    for (int chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) each_in_chunk<true>(a.t, entry_of, chunk, [&](float v) { return v * scale; });
 }
 
 }  // namespace ilx
