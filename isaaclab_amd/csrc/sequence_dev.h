@@ -35,19 +35,23 @@ __device__ __forceinline__ float softplus_f(float x) {
     return __builtin_fmaf(p, s, __builtin_fmaxf(x, 0.0f));   // (a NaN comes through e)
 }
 
-// V neighbouring channels of one row, as one load or store of up to 16 bytes.
+// V elements on their own boundary, up to 16 bytes.
 template <typename T, int V> struct alignas(sizeof(T) * V < 16 ? sizeof(T) * V : 16) Pack { T v[V]; };
 
+// V neighbouring channels of one row, as one load or store of up to 16 bytes on any element's boundary (the chip reads and writes
+// global memory unaligned).
+template <typename T, int V> struct __attribute__((packed, aligned(sizeof(T)))) Channels { T v[V]; };
+
 template <int V, typename T> __device__ __forceinline__ void load_channels(const T* p, float (&v)[V]) {
-    const Pack<T, V> w = *reinterpret_cast<const Pack<T, V>*>(p);
+    const Channels<T, V> w = *reinterpret_cast<const Channels<T, V>*>(p);
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = to_f32(w.v[k]);
 }
 template <int V, typename T> __device__ __forceinline__ void store_channels(T* p, const float (&v)[V]) {
-    Pack<T, V> w;
+    Channels<T, V> w;
 #pragma unroll
     for (int k = 0; k < V; ++k) w.v[k] = from_f32<T>(v[k]);
-    *reinterpret_cast<Pack<T, V>*>(p) = w;
+    *reinterpret_cast<Channels<T, V>*>(p) = w;
 }
 
 constexpr int64_t kMostThreads = (int64_t{1} << 32) - 1024;   // of one launch

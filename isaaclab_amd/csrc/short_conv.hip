@@ -3,7 +3,9 @@
 // All three kernels move each input once and have 2 W + 6 flops per element, so they are bound by memory.  A thread owns V
 // neighbouring channels (one access of 16 bytes per row, or 8 where the backward pass has 16-bit elements) of a segment of rows
 // and keeps the last W - 1 rows in registers; a segment re-reads the W - 1 rows ahead of it, which the thread beside it has just
-// brought into the cache.  An episode start clears the registers, so no row looks past it.
+// brought into the cache.  An episode start clears the registers, so no row looks past it.  Where V does not divide the
+// channels, the last thread's V channels end with the row's and overlap its neighbour's: both come to the same values and store
+// them, but for the step, which writes what its neighbour reads and stores its own only.
 // Measured, W = 4, against a large copy's 4.97 TB/s on the same card:
 //   forward, 24 x 4096 x 256 f32: 36 us, 201 MB, 5.5 TB/s (part of it stays in the last-level cache between passes)
 //   forward, 3 x 8190 x 1536 bf16: 36 us, 151 MB, 4.1 TB/s
@@ -18,7 +20,7 @@ constexpr int kConvRows = 2;   // read ahead; 4: a recording of 16384 x 1024 in 
 
 struct ConvArgs {
     ilx_short_conv c;
-    int groups;        // of V channels
+    int groups;        // of V channels, the last one's shifted to end with the row
     int cx_log2;       // lanes side by side over channel groups; 256 >> cx_log2 rows of threads over segments
     int channel_blocks;
     int segment;       // rows per segment
@@ -27,10 +29,9 @@ struct ConvArgs {
     int64_t slots;     // rows of threads in the grid / rows per block (backward: partial sums)
 };
 
-struct ConvThread {
-    int d0;
-    int64_t item, b, t0, t1, len;
-};
+template <int V> __device__ __forceinline__ int first_channel(const ConvArgs& a, int group) {
+    return group * V + V <= a.c.channels ? group * V : a.c.channels - V;
+}
 
 __device__ __forceinline__ int64_t sequence_length(const int32_t* lengths, int64_t b, int64_t length) {
     if (!lengths) return length;
@@ -96,7 +97,7 @@ template <int W, int V> __device__ __forceinline__ void forget(float (&win)[W][V
 
 // The next kConvRows rows of x (and of the output's gradient) and their start flags, read while the rows ahead are worked on.
 template <typename T, int V, bool GRAD> struct ConvRows {
-    Pack<T, V> x[kConvRows], g[kConvRows];
+    Channels<T, V> x[kConvRows], g[kConvRows];
     uint8_t start[kConvRows];
 
     __device__ __forceinline__ void read(const ConvArgs& a, int d0, int64_t b, int64_t t, int64_t end) {
@@ -106,14 +107,14 @@ template <typename T, int V, bool GRAD> struct ConvRows {
 #pragma unroll
         for (int i = 0; i < kConvRows; ++i) {
             const int64_t r = t + i < end ? t + i : end - 1;
-            x[i] = *reinterpret_cast<const Pack<T, V>*>(px + r * a.c.x_time);
-            if (GRAD) g[i] = *reinterpret_cast<const Pack<T, V>*>(pg + r * a.c.grad_out_time);
+            x[i] = *reinterpret_cast<const Channels<T, V>*>(px + r * a.c.x_time);
+            if (GRAD) g[i] = *reinterpret_cast<const Channels<T, V>*>(pg + r * a.c.grad_out_time);
             start[i] = 0;
             if (a.c.starts) start[i] = ps[r * a.c.starts_time];
         }
     }
 };
-template <int V, typename T> __device__ __forceinline__ void unpack(const Pack<T, V>& p, float (&v)[V]) {
+template <int V, typename T> __device__ __forceinline__ void unpack(const Channels<T, V>& p, float (&v)[V]) {
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = to_f32(p.v[k]);
 }
@@ -124,7 +125,7 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_forward_kernel(ConvAr
     const int group = static_cast<int>(blockIdx.x % a.channel_blocks) * (1 << a.cx_log2) + cx;
     const int64_t item = static_cast<int64_t>(blockIdx.x / a.channel_blocks) * (kConvThreads >> a.cx_log2) + row;
     if (group >= a.groups || item >= a.items) return;
-    const int d0 = group * V;
+    const int d0 = first_channel<V>(a, group);
     const int64_t b = item / a.segments, t0 = (item - b * a.segments) * a.segment;
     const int64_t t1 = t0 + a.segment < a.c.length ? t0 + a.segment : a.c.length;
     const int64_t len = sequence_length(a.c.lengths, b, a.c.length), te = t1 < len ? t1 : len;
@@ -175,7 +176,7 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvA
     const int group = static_cast<int>(blockIdx.x % a.channel_blocks) * (1 << a.cx_log2) + cx;
     const int64_t slot = blockIdx.x / a.channel_blocks;
     const bool active = group < a.groups;
-    const int d0 = (active ? group : a.groups - 1) * V;
+    const int d0 = first_channel<V>(a, active ? group : a.groups - 1);
     float w[W][V], bias[V], dw[W][V], db[V];
     load_weights<W, V>(a, d0, w, bias);
 #pragma unroll
@@ -294,7 +295,7 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvA
         if (g >= a.groups) continue;
         float s = 0.0f;
         for (int r = 0; r < rows; ++r) s += sums[(r * lanes + lane) * P + kv];
-        a.c.workspace[(slot * (W + 1) + k) * a.c.channels + g * V + v] = s;
+        a.c.workspace[(slot * (W + 1) + k) * a.c.channels + first_channel<V>(a, g) + v] = s;
     }
 }
 
@@ -304,7 +305,7 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvArgs 
     const int64_t i = static_cast<int64_t>(blockIdx.x) * kConvThreads + threadIdx.x;
     if (i >= a.items) return;
     const int64_t b = i / a.groups;
-    const int d0 = static_cast<int>(i - b * a.groups) * V;
+    const int group = static_cast<int>(i - b * a.groups), d0 = first_channel<V>(a, group), shared = group * V - d0;   // the neighbour's channels
     float w[W][V], bias[V], win[W][V], p[V];
     const bool start = a.c.starts && a.c.starts[b * a.c.starts_batch];
     float* last = a.c.last + b * (W - 1) * a.c.channels + d0;
@@ -318,9 +319,20 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_step_kernel(ConvArgs 
 #pragma unroll
         for (int v = 0; v < V; ++v) p[v] *= sigmoid_fast(p[v]);
     }
-    store_channels<V>(static_cast<T*>(a.c.out) + b * a.c.out_batch + d0, p);
+    T* out = static_cast<T*>(a.c.out) + b * a.c.out_batch + d0;
+    if (shared == 0) {
+        store_channels<V>(out, p);
 #pragma unroll
-    for (int k = 0; k < W - 1; ++k) store_channels<V>(last + k * static_cast<int64_t>(a.c.channels), win[k + 1]);
+        for (int k = 0; k < W - 1; ++k) store_channels<V>(last + k * static_cast<int64_t>(a.c.channels), win[k + 1]);
+    } else {
+#pragma unroll
+        for (int v = 0; v < V; ++v) {
+            if (v < shared) continue;
+            out[v] = from_f32<T>(p[v]);
+#pragma unroll
+            for (int k = 0; k < W - 1; ++k) last[k * static_cast<int64_t>(a.c.channels) + v] = win[k + 1][v];
+        }
+    }
 }
 
 // out0[d, k] = sum over the partial rows of value (k, d): kSumColumns columns to a workgroup, kSumParts threads to a column, eight rows of
@@ -369,35 +381,31 @@ using namespace ilx;
 
 namespace {
 
+constexpr int kMostSegment = 64, kLeastSegment = 8;   // rows
+
 size_t conv_item_bytes(int dtype) { return dtype == ILX_F32 ? 4 : 2; }
 
-// V channels to an access need every row of every operand on its boundary.
-bool conv_rows_aligned(const void* p, int64_t batch, int64_t time, int64_t batches, int64_t rows, size_t item, int v) {
-    return !p || (aligned_to(p, item * v) && (batches <= 1 || batch % v == 0) && (rows <= 1 || time % v == 0));
-}
-
+// Channels of a thread: 16 bytes of them (four in the backward pass, which keeps five rows of values a channel), fewer where that
+// would leave less than two waves a SIMD with the shortest segments.  Measured in bf16, forward: 3 x 8190 x 1535 channels 38 us with 8,
+// 55 with one; 1000 x 24 x 256 9 us with 4, 13 with 8; 1 x 2048 x 256 4 us with one, 8 with 8.
 int conv_vector(const ilx_short_conv& c, bool backward) {
-    const size_t item = conv_item_bytes(c.dtype);
-    const int v = !backward && item == 2 ? 8 : 4;   // 16 bytes; backward keeps five rows of values a channel, four channels fit
-    const auto rows = [&](const void* p, int64_t sb, int64_t st) { return conv_rows_aligned(p, sb, st, c.batch, c.length, item, v); };
-    bool ok = c.channels % v == 0 && rows(c.x, c.x_batch, c.x_time) && rows(c.out, c.out_batch, c.out_time) && aligned_to(c.state, 16) &&
-              aligned_to(c.last, 16);
-    if (backward)
-        ok = ok && rows(c.grad_out, c.grad_out_batch, c.grad_out_time) && rows(c.grad_x, c.grad_x_batch, c.grad_x_time) &&
-             aligned_to(c.grad_last, 16) && aligned_to(c.grad_state, 16);
-    return ok ? v : 1;
+    for (const int v : {8, 4}) {
+        if (c.channels < v || (v == 8 && (backward || conv_item_bytes(c.dtype) == 4))) continue;
+        if (c.batch * ((c.length + kLeastSegment - 1) / kLeastSegment) * ((c.channels + v - 1) / v) >= 512 * device_cu_count()) return v;
+    }
+    return 1;
 }
 
 ConvArgs conv_args(const ilx_short_conv& c, int v, bool backward) {
     ConvArgs a{};
     a.c = c;
-    a.groups = c.channels / v;
+    a.groups = (c.channels + v - 1) / v;
     a.cx_log2 = 0;
     while (a.cx_log2 < 6 && (1 << a.cx_log2) < a.groups) ++a.cx_log2;
     a.channel_blocks = (a.groups + (1 << a.cx_log2) - 1) >> a.cx_log2;
     // A long segment reads few rows twice; it is halved while there are too few threads for two waves a SIMD.
-    a.segment = 64;
-    while (a.segment > 8 && c.batch * ((c.length + a.segment - 1) / a.segment) * a.groups < 512 * device_cu_count()) a.segment /= 2;
+    a.segment = kMostSegment;
+    while (a.segment > kLeastSegment && c.batch * ((c.length + a.segment - 1) / a.segment) * a.groups < 512 * device_cu_count()) a.segment /= 2;
     a.segments = c.length > 0 ? (c.length + a.segment - 1) / a.segment : 1;
     a.items = c.batch * a.segments;
     const int rows = kConvThreads >> a.cx_log2;

@@ -74,6 +74,13 @@ CONV = [  # batch, length, channels, width, dtype, silu, starts, lengths, state,
     (2, 32, 300, 7, 2, False, False, False, True, False),
     (3, 64, 7, 6, 1, True, True, True, True, True),
     (2, 300, 520, 4, 1, True, True, True, True, False),
+    # enough rows for four or eight channels a thread, whole and overlapping at the end of a row
+    (300, 8, 1801, 4, 0, True, True, True, True, True),
+    (600, 5, 1803, 3, 1, True, True, True, True, False),
+    (550, 6, 2048, 4, 1, True, True, False, True, True),
+    (1100, 16, 258, 8, 2, True, False, True, False, False),
+    (24, 180, 1210, 4, 1, True, True, True, True, False),
+    (300, 8, 1800, 2, 0, False, False, False, True, False),
 ]
 
 
@@ -125,7 +132,7 @@ def test_convolution_steps_are_the_sequence(dev):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("batch,channels,width", [(1, 1, 1), (1, 256, 4), (7, 30, 2), (1000, 36, 4), (3, 1025, 8), (5, 12, 5)])
+@pytest.mark.parametrize("batch,channels,width", [(1, 1, 1), (1, 256, 4), (7, 30, 2), (1000, 36, 4), (3, 1025, 8), (5, 12, 5), (9000, 61, 4), (20000, 61, 3), (20000, 64, 2), (17000, 30, 8)])
 def test_convolution_step(dev, dtype, batch, channels, width):
     gen = torch.Generator().manual_seed(batch + channels)
     x, w = torch.randn(batch, channels, generator=gen).to(dtype), torch.randn(channels, width, generator=gen)
@@ -390,6 +397,27 @@ def test_sliding_windows_over_one_series(dev):
             results.append((out, y, *torch.autograd.grad(out.square().sum() + y.square().sum(), x), step, state))
         for got, plain in zip(*results):
             assert torch.equal(got, plain)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+def test_unaligned_rows_of_many_channels(dev, dtype):
+    """Slices that begin at any element and rows of odd lengths, at sizes that take several channels a thread."""
+    wide = torch.randn(800, 8, 1611, device=dev).to(dtype)
+    weight, bias = torch.randn(1600, 4, device=dev, requires_grad=True), torch.randn(1600, device=dev)
+    grad = torch.randn(800, 8, 1605, device=dev).to(dtype)
+    results = []
+    for x, g in ((wide[:, :, 3:1603], grad[..., 1:1601]), (wide[:, :, 3:1603].contiguous(), grad[..., 1:1601].contiguous())):
+        x = x.detach().requires_grad_(True)
+        out = S.short_convolution(x, weight, bias, activation="silu")
+        grads = torch.autograd.grad(out, (x, weight), g)
+        rows = x.detach().flatten(0, 1) if x.is_contiguous() else wide.flatten(0, 1)[:, 3:1603]
+        state, to = torch.zeros(6400, 3, 1600, device=dev), torch.zeros(6400, 1607, dtype=dtype, device=dev)
+        with torch.no_grad():
+            S.short_convolution_step(rows, state, weight, bias, out=to[:, 5:1605] if not x.is_contiguous() else to[:, :1600])
+        results.append((out, *grads, state, to[:, 5:1605] if not x.is_contiguous() else to[:, :1600]))
+        outside = to[:, :5] if not x.is_contiguous() else to[:, 1600:]
+        assert not outside.any()
+    assert all(torch.equal(a, b) for a, b in zip(*results))
 
 
 def wide_of(t):
