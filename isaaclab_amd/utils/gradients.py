@@ -1,9 +1,9 @@
 """Global gradient norm and clipping on ``ilx_gradient_norm`` (include/isaaclab_amd_sequence.h): the end of a training step.
 
 No counterpart in the reference, whose RL libraries call torch.  All tensors, of any mix of float32, bfloat16 and float16, are
-reduced in one launch per 200 tensors and scaled in place in another; nothing is read back to the host.  Squares are added
-in 64 bits in a fixed order, so the norm neither overflows nor depends on scheduling: replicas with equal gradients clip
-alike.
+reduced in one launch per 200 tensors and scaled in place in another; nothing is read back to the host.  No derivative goes
+through the norm or the scaling (forward mode is refused).  Squares are added in 64 bits in a fixed order, so their sum
+neither overflows nor depends on scheduling: replicas with equal gradients clip alike.
 """
 
 from __future__ import annotations
@@ -18,7 +18,7 @@ from ctypes import c_float, c_int32, c_int64
 import torch
 
 from .. import _abi
-from .sequence import _DTYPES, _current_device, _written
+from .sequence import _DTYPES, _current_device, _no_tangents, _written
 
 _norm = _abi._sig("ilx_gradient_norm", _abi.P, _abi.P, _abi.P, c_int32, c_int32, c_int32, c_float, _abi.P, _abi.P, c_int64, _abi.P)
 _T, _dtype, _KIND = torch.Tensor, operator.attrgetter("dtype"), _DTYPES.get
@@ -38,6 +38,7 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
     tensors = [g for g in gradients if g is not None]
     if not tensors:
         raise ValueError("no gradients")
+    _no_tangents(tensors)
     first = tensors[0]
     if not first.is_cuda:
         raise _abi.IlxError("isaaclab_amd kernels need GPU tensors (got a CPU tensor); there is no CPU fallback")

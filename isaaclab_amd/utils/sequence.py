@@ -21,7 +21,7 @@ not read, their outputs and gradients are zero, and the state skips them.
 
 As everywhere in this package there is no CPU fallback.  Inside ``CommandList.record`` the calls are recorded with the buffers
 they allocate, which the list keeps; a call whose operands need gradients is refused there (its backward pass runs on
-another thread).
+another thread).  Forward-mode differentiation is refused, and so are second derivatives.
 """
 
 from __future__ import annotations
@@ -30,6 +30,7 @@ import ctypes
 from ctypes import c_int32, c_int64, c_void_p
 
 import torch
+from torch.autograd import forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _abi
@@ -179,12 +180,22 @@ def _wants_gradients(tensors) -> bool:
     return False
 
 
+def _no_tangents(tensors):
+    """A dual tensor of forward-mode differentiation does not say ``requires_grad``: its tangent would be lost without a word."""
+    if forward_ad._current_level >= 0:
+        for t in tensors:
+            if isinstance(t, torch.Tensor) and forward_ad.unpack_dual(t).tangent is not None:
+                raise RuntimeError("forward-mode differentiation is not supported: an operand carries a tangent")
+
+
 def _no_gradients(what: str, tensors):
+    _no_tangents(tensors)
     if _wants_gradients(tensors):
         raise RuntimeError(f"{what} has no backward pass: call it under torch.no_grad(), or use the form over sequences")
 
 
 def _needs_gradients(tensors) -> bool:
+    _no_tangents(tensors)
     if not _wants_gradients(tensors):
         return False
     if _abi.recording():

@@ -1,0 +1,48 @@
+"""GPU: calls of the sequence operators at the edges of what autograd, command lists and the argument types allow."""
+
+import pytest
+import torch
+from torch.autograd import forward_ad
+
+from isaaclab_amd.utils import sequence as S
+
+pytestmark = pytest.mark.gpu
+
+
+def operands(dev, batch=3, length=20, channels=24, states=4, seed=0):
+    gen = torch.Generator().manual_seed(seed)
+    r = lambda *s: torch.randn(*s, generator=gen).to(dev)  # noqa: E731
+    return dict(x=r(batch, length, channels), delta=r(batch, length, channels), A=-torch.rand(channels, states, generator=gen).to(dev) - 0.5,
+                B=r(batch, length, states), C=r(batch, length, states), D=r(channels), gate=r(batch, length, channels), delta_bias=r(channels),
+                state=r(batch, states, channels))
+
+
+def scan(v, **kw):
+    return S.state_space_scan(v["x"], v["delta"], v["A"], v["B"], v["C"], D=v["D"], gate=v["gate"], delta_bias=v["delta_bias"], state=v["state"], **kw)
+
+
+def step(v, t, state, **kw):
+    return S.state_space_step(v["x"][:, t], v["delta"][:, t], state, v["A"], v["B"][:, t], v["C"][:, t], D=v["D"], gate=v["gate"][:, t],
+                              delta_bias=v["delta_bias"], **kw)
+
+
+def test_forward_mode_is_refused(dev):
+    """Each operand in turn as a dual tensor: an error and not a result without its tangent."""
+    v = operands(dev)
+    conv = dict(x=v["x"], weight=torch.randn(24, 4, device=dev), bias=torch.randn(24, device=dev), state=torch.randn(3, 3, 24, device=dev))
+    with forward_ad.dual_level():
+        dual = lambda t: forward_ad.make_dual(t, torch.ones_like(t))  # noqa: E731
+        for k in v:
+            w = {**v, k: dual(v[k])}
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                scan(w)
+            with pytest.raises(RuntimeError, match="forward-mode"), torch.no_grad():   # (which stops reverse mode only)
+                step(w, 0, w["state"])
+        for k in conv:
+            w = {**conv, k: dual(conv[k])}
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                S.short_convolution(w["x"], w["weight"], w["bias"], state=w["state"])
+            with pytest.raises(RuntimeError, match="forward-mode"):
+                S.short_convolution_step(w["x"][:, 0], w["state"], w["weight"], w["bias"])
+        inside = scan(v)
+    assert torch.equal(inside, scan(v))
