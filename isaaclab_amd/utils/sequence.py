@@ -344,13 +344,14 @@ def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.T
     """One row of :func:`short_convolution` per sequence: ``x`` (batch, channels), ``state`` (batch, W - 1, channels) updated in
     place, ``starts`` (batch) the environments whose episode begins with this row.  ``out`` may name the result's buffer."""
     x, index = _check_x(x, 2)
-    _no_gradients("short_convolution_step", (x, weight, bias, state))
+    _no_gradients("short_convolution_step", (x, weight, bias, state, out))
     batch, channels = x.shape
     silu = _silu(activation)
     weight, bias = _check_filter(weight, bias, channels, index)
     width = weight.shape[1]
     _check_state(state, (batch, width - 1, channels), index)
     starts = _check_starts(starts, (batch,), index)
+    written = (state,) if out is None else (state, out)
     out = _check_out(out, x)
     _keep(x, weight, bias, out)
     at = state.data_ptr()
@@ -358,7 +359,7 @@ def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.T
         x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _p(bias), at, _p(starts), starts.stride(0) if starts is not None else 0, 0, None,
         out.data_ptr(), out.stride(0), 0, at, batch, 1, channels, width, _DTYPES[x.dtype], silu)
     _launch(_conv_step, desc, "ilx_short_conv_step", index)
-    _written((state,))
+    _written(written)
     return out
 
 
@@ -520,13 +521,14 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
     N) or (batch, N), ``state`` (batch, N, channels) updated in place, ``starts`` (batch) the environments whose episode begins
     with this row.  ``out`` may name the result's buffer."""
     x, index = _check_x(x, 2)
-    _no_gradients("state_space_step", (x, delta, state, A, B, C, D, gate, delta_bias))
+    _no_gradients("state_space_step", (x, delta, state, A, B, C, D, gate, delta_bias, out))
     batch, channels = x.shape
     delta, A, B, C, D, gate, delta_bias = _scan_operands(x, index, delta, A, B, C, D, gate, delta_bias)
     B, C = _pair(B, C)
     states = A.shape[1]
     _check_state(state, (batch, states, channels), index)
     starts = _check_starts(starts, (batch,), index)
+    written = (state,) if out is None else (state, out)
     out = _check_out(out, x)
     _keep(x, delta, A, B, C, D, gate, delta_bias, out)
     at = state.data_ptr()
@@ -536,5 +538,5 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
         starts.stride(0) if starts is not None else 0, 0, None, out.data_ptr(), out.stride(0), 0, at, None, batch, 1, channels, states, B.shape[1],
         _DTYPES[x.dtype], _DTYPES[B.dtype], 1 if softplus else 0)
     _launch(_scan_step, desc, "ilx_state_space_step", index)
-    _written((state,))
+    _written(written)
     return out

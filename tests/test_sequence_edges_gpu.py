@@ -46,3 +46,25 @@ def test_forward_mode_is_refused(dev):
                 S.short_convolution_step(w["x"][:, 0], w["state"], w["weight"], w["bias"])
         inside = scan(v)
     assert torch.equal(inside, scan(v))
+
+
+def test_out_is_written_in_sight_of_autograd(dev):
+    """A buffer that a graph has saved and a step then writes fails the backward pass; a leaf that needs gradients is refused."""
+    v, weight = operands(dev), torch.randn(24, 4, device=dev)
+    conv = torch.zeros(3, 3, 24, device=dev)
+    for call in (lambda out: S.short_convolution_step(v["x"][:, 0], conv, weight, out=out), lambda out: step(v, 0, v["state"], out=out)):
+        for buffer in (torch.ones(5, 3, 24, device=dev)[2], torch.ones(3, 30, device=dev)[:, :24]):
+            leaf = torch.ones(3, 24, device=dev, requires_grad=True)
+            product = (leaf * buffer).sum()
+            before = buffer._version
+            with torch.no_grad():
+                assert call(buffer) is buffer
+            assert buffer._version > before
+            with pytest.raises(RuntimeError, match="modified by an inplace"):
+                torch.autograd.grad(product, leaf)
+        leaf = torch.ones(3, 24, device=dev, requires_grad=True)
+        with pytest.raises(RuntimeError, match="no backward"):
+            call(leaf)
+        assert torch.equal(leaf, torch.ones_like(leaf))
+        with torch.inference_mode():
+            call(torch.empty(3, 24, device=dev))
