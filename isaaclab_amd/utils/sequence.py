@@ -203,13 +203,26 @@ def _needs_gradients(tensors) -> bool:
     return True
 
 
-def _check_out(out: torch.Tensor | None, x: torch.Tensor) -> torch.Tensor:
+def _overlap(rows: torch.Tensor, dense: torch.Tensor) -> bool:
+    """Whether a row of ``rows`` (unit channel stride) touches the memory of ``dense``."""
+    if rows.numel() == 0 or dense.numel() == 0:
+        return False
+    size = rows.element_size()
+    begin, step, width = rows.data_ptr(), rows.stride(0) * size, rows.shape[1] * size
+    lo, hi = dense.data_ptr(), dense.data_ptr() + dense.numel() * dense.element_size()
+    first = 0 if begin + width > lo or step == 0 else (lo - begin - width) // step + 1   # the first row that ends behind lo
+    return first < rows.shape[0] and begin + first * step < hi and begin + first * step + width > lo
+
+
+def _check_out(out: torch.Tensor | None, x: torch.Tensor, state: torch.Tensor) -> torch.Tensor:
     if out is None:
         return _empty_like(x)
     if out.shape != x.shape or out.dtype is not x.dtype or out.device != x.device or (out.stride(-1) != 1 and out.shape[-1] != 1):
         raise ValueError(f"out must be like x ({tuple(x.shape)}, {x.dtype}) with unit channel stride")
     if out.shape[0] > 1 and out.stride(0) < out.shape[1]:
         raise ValueError(f"out's rows overlap (strides {out.stride()})")
+    if _overlap(out, state):
+        raise ValueError("out and state share memory, and both are written")
     return out
 
 
@@ -342,7 +355,8 @@ def short_convolution(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
 def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor | None = None, *,
                            activation: str | None = None, starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """One row of :func:`short_convolution` per sequence: ``x`` (batch, channels), ``state`` (batch, W - 1, channels) updated in
-    place, ``starts`` (batch) the environments whose episode begins with this row.  ``out`` may name the result's buffer."""
+    place, ``starts`` (batch) the environments whose episode begins with this row.  ``out`` may name the
+    result's buffer, ``x`` itself for one, and shares memory with no other operand."""
     x, index = _check_x(x, 2)
     _no_gradients("short_convolution_step", (x, weight, bias, state, out))
     batch, channels = x.shape
@@ -352,7 +366,7 @@ def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.T
     _check_state(state, (batch, width - 1, channels), index)
     starts = _check_starts(starts, (batch,), index)
     written = (state,) if out is None else (state, out)
-    out = _check_out(out, x)
+    out = _check_out(out, x, state)
     _keep(x, weight, bias, out)
     at = state.data_ptr()
     desc = ShortConvDesc(
@@ -519,7 +533,7 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
                      softplus: bool = True, starts: torch.Tensor | None = None, out: torch.Tensor | None = None) -> torch.Tensor:
     """One row of :func:`state_space_scan` per sequence: ``x``, ``delta``, ``gate`` (batch, channels), ``B``, ``C`` (batch, groups,
     N) or (batch, N), ``state`` (batch, N, channels) updated in place, ``starts`` (batch) the environments whose episode begins
-    with this row.  ``out`` may name the result's buffer."""
+    with this row.  ``out`` may name the result's buffer, ``x``, ``delta`` or ``gate`` itself for one, and shares memory with no other operand."""
     x, index = _check_x(x, 2)
     _no_gradients("state_space_step", (x, delta, state, A, B, C, D, gate, delta_bias, out))
     batch, channels = x.shape
@@ -529,7 +543,7 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
     _check_state(state, (batch, states, channels), index)
     starts = _check_starts(starts, (batch,), index)
     written = (state,) if out is None else (state, out)
-    out = _check_out(out, x)
+    out = _check_out(out, x, state)
     _keep(x, delta, A, B, C, D, gate, delta_bias, out)
     at = state.data_ptr()
     desc = StateSpaceDesc(

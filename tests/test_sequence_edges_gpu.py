@@ -68,3 +68,30 @@ def test_out_is_written_in_sight_of_autograd(dev):
         assert torch.equal(leaf, torch.ones_like(leaf))
         with torch.inference_mode():
             call(torch.empty(3, 24, device=dev))
+
+
+def test_out_in_the_place_of_an_operand(dev):
+    """x, delta or gate may be the result's buffer; the state may not, not even in part."""
+    for channels in (24, 130, 61):
+        v, weight = operands(dev, batch=9000, length=1, channels=channels), torch.randn(channels, 4, device=dev)
+        rows = lambda k: v[k][:, 0].clone()  # noqa: E731
+        for name in ("x", "delta", "gate"):
+            w = {k: rows(k) for k in ("x", "delta", "gate", "B", "C")}
+            s1, s2 = v["state"].clone(), v["state"].clone()
+            args = lambda s: (w["x"], w["delta"], s, v["A"], w["B"], w["C"])  # noqa: E731
+            want = S.state_space_step(*args(s1), D=v["D"], gate=w["gate"], delta_bias=v["delta_bias"])
+            got = S.state_space_step(*args(s2), D=v["D"], gate=w["gate"], delta_bias=v["delta_bias"], out=w[name])
+            assert got is w[name] and torch.equal(got, want) and torch.equal(s1, s2)
+        s1, s2, x = torch.randn(9000, 3, channels, device=dev), None, rows("x")
+        s2 = s1.clone()
+        want = S.short_convolution_step(x, s1, weight, activation="silu")
+        assert torch.equal(S.short_convolution_step(x, s2, weight, activation="silu", out=x), want) and torch.equal(s1, s2)
+    block = torch.zeros(3 * 4 * 24 + 40, device=dev)
+    state, over = block[:3 * 4 * 24].view(3, 4, 24), block[-3 * 24:].view(3, 24)
+    v = operands(dev)
+    with pytest.raises(ValueError, match="share memory"):
+        step(v, 0, state, out=over)
+    state = block[:3 * 3 * 24].view(3, 3, 24)
+    with pytest.raises(ValueError, match="share memory"):
+        S.short_convolution_step(v["x"][:, 0], state, torch.randn(24, 4, device=dev), out=state[:, 1])
+    assert not block.any()
