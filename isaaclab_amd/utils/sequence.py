@@ -154,12 +154,14 @@ def _check_starts(starts: torch.Tensor | None, shape: tuple, index: int) -> torc
     return starts
 
 
-def _check_lengths(lengths: torch.Tensor | None, batch: int, index: int) -> torch.Tensor | None:
+def _check_lengths(lengths: torch.Tensor | None, batch: int, length: int, index: int) -> torch.Tensor | None:
     if lengths is None:
         return None
     if lengths.shape != (batch,) or lengths.dtype not in (torch.int32, torch.int64):
         raise ValueError(f"lengths is {lengths.dtype} {tuple(lengths.shape)}, expected int32 or int64 {(batch,)}")
     _on(lengths, "lengths", index)
+    if lengths.dtype is torch.int64 and not _abi.recording():
+        lengths = lengths.clamp(0, length)   # (ahead of the narrowing, which would wrap)
     return lengths if lengths.dtype is torch.int32 and lengths.is_contiguous() else _copy(lengths, "lengths", dtype=torch.int32)
 
 
@@ -344,7 +346,7 @@ def short_convolution(x: torch.Tensor, weight: torch.Tensor, bias: torch.Tensor 
     weight, bias = _check_filter(weight, bias, channels, index)
     state = _check_parameter(state, "state", (batch, weight.shape[1] - 1, channels), index)
     starts = _check_starts(starts, (batch, length), index)
-    lengths = _check_lengths(lengths, batch, index)
+    lengths = _check_lengths(lengths, batch, length, index)
     if _needs_gradients((x, weight, bias, state)):
         out, last = _ShortConvolution.apply(x, weight, bias, state, starts, lengths, silu, return_state)
     else:
@@ -519,7 +521,7 @@ def state_space_scan(x: torch.Tensor, delta: torch.Tensor, A: torch.Tensor, B: t
     delta, A, B, C, D, gate, delta_bias = _scan_operands(x, index, delta, A, B, C, D, gate, delta_bias)
     state = _check_parameter(state, "state", (batch, A.shape[1], channels), index)
     starts = _check_starts(starts, (batch, length), index)
-    lengths = _check_lengths(lengths, batch, index)
+    lengths = _check_lengths(lengths, batch, length, index)
     args = (x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, 1 if softplus else 0, return_state)
     if _needs_gradients(args[:9]):
         out, last = _StateSpaceScan.apply(*args)

@@ -95,3 +95,13 @@ def test_out_in_the_place_of_an_operand(dev):
     with pytest.raises(ValueError, match="share memory"):
         S.short_convolution_step(v["x"][:, 0], state, torch.randn(24, 4, device=dev), out=state[:, 1])
     assert not block.any()
+
+
+def test_lengths_past_32_bits(dev):
+    """64-bit lengths are clamped as they are, not as what is left of them in 32 bits."""
+    v, weight = operands(dev), torch.randn(24, 4, device=dev)
+    lengths = torch.tensor([2 ** 32 + 5, torch.iinfo(torch.int64).max, -2 ** 40 + 7], device=dev)
+    clamped = torch.tensor([20, 20, 0], dtype=torch.int32, device=dev)
+    for call in (lambda n: scan(v, lengths=n, return_state=True), lambda n: S.short_convolution(v["x"], weight, lengths=n, return_state=True)):
+        assert all(torch.equal(a, b) for a, b in zip(call(lengths), call(clamped)))
+    assert torch.equal(scan(v, lengths=lengths)[:2], scan(v)[:2])
