@@ -22,7 +22,7 @@ from .. import _abi
 class CommandList:
     def __init__(self):
         self._handle = None
-        self._kept = []   # buffers that recorded calls allocated for themselves
+        self._kept = []   # buffers that recorded calls allocated for themselves, and operands they asked to keep
 
     @contextlib.contextmanager
     def record(self):

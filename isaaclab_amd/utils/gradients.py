@@ -18,7 +18,7 @@ from ctypes import c_float, c_int32, c_int64
 import torch
 
 from .. import _abi
-from .sequence import _DTYPES, _current_device, _no_tangents, _written
+from .sequence import _DTYPES, _current_device, _keep, _no_tangents, _written
 
 _norm = _abi._sig("ilx_gradient_norm", _abi.P, _abi.P, _abi.P, c_int32, c_int32, c_int32, c_float, _abi.P, _abi.P, c_int64, _abi.P)
 _T, _dtype, _KIND = torch.Tensor, operator.attrgetter("dtype"), _DTYPES.get
@@ -55,6 +55,7 @@ def _call(gradients: Iterable[torch.Tensor | None], norm_type: float, clip: bool
     pointers, sizes, dtypes = array("q", map(_T.data_ptr, tensors)), array("q", map(_T.numel, tensors)), array("i", kinds)
     norm = _abi.keep(torch.empty((), device=first.device))
     workspace = _abi.keep(torch.empty(_WORKSPACE, device=first.device))
+    _keep(*tensors)
     with contextlib.nullcontext() if index == _current_device() else torch.cuda.device(index):
         status = _norm(pointers.buffer_info()[0], sizes.buffer_info()[0], dtypes.buffer_info()[0], len(tensors), int(norm_type == math.inf),
                        int(clip), max_norm, norm.data_ptr(), workspace.data_ptr(), _WORKSPACE, _abi.stream())

@@ -19,8 +19,8 @@ everything is computed in float32.  ``starts`` (batch, length) marks the rows on
 such a row, the carried state included, reaches it.  ``lengths`` (batch) says where a padded sequence ends: rows behind are
 not read, their outputs and gradients are zero, and the state skips them.
 
-As everywhere in this package there is no CPU fallback.  Inside ``CommandList.record`` the calls are recorded with the buffers
-they allocate, which the list keeps; a call whose operands need gradients is refused there (its backward pass runs on
+As everywhere in this package there is no CPU fallback.  Inside ``CommandList.record`` the calls are recorded, and the list keeps
+their operands and the buffers they allocate; a call whose operands need gradients is refused there (its backward pass runs on
 another thread).  Forward-mode differentiation is refused, and so are second derivatives.
 """
 
@@ -283,7 +283,7 @@ def _conv_call(x, weight, bias, state, starts, lengths, silu, want_last):
     desc = _conv_desc(x, weight, bias, state, starts, lengths, silu)
     out = _empty_like(x)
     last = torch.empty(x.shape[0], weight.shape[1] - 1, x.shape[2], device=x.device) if want_last else None
-    _keep(out, last)
+    _keep(x, weight, bias, state, starts, lengths, out, last)
     desc.out, desc.last = out.data_ptr(), _p(last)
     desc.out_batch, desc.out_time, _ = out.stride()
     _launch(_conv_forward, desc, "ilx_short_conv_forward", x.get_device())
@@ -369,7 +369,7 @@ def short_convolution_step(x: torch.Tensor, state: torch.Tensor, weight: torch.T
     starts = _check_starts(starts, (batch,), index)
     written = (state,) if out is None else (state, out)
     out = _check_out(out, x, state)
-    _keep(x, weight, bias, out)
+    _keep(x, weight, bias, state, starts, out)
     at = state.data_ptr()
     desc = ShortConvDesc(
         x.data_ptr(), x.stride(0), 0, weight.data_ptr(), _p(bias), at, _p(starts), starts.stride(0) if starts is not None else 0, 0, None,
@@ -437,7 +437,7 @@ def _scan_call(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, s
     desc.out, desc.last, desc.saved = out.data_ptr(), _p(last), _p(saved)
     desc.out_batch, desc.out_time, _ = out.stride()
     workspace = _scan_scratch(desc, 0, device)
-    _keep(out, last, workspace)
+    _keep(x, delta, A, B, C, D, gate, delta_bias, state, starts, lengths, out, last, workspace)
     _launch(_scan_forward, desc, "ilx_state_space_forward", x.get_device())
     return out, last, saved, desc
 
@@ -546,7 +546,7 @@ def state_space_step(x: torch.Tensor, delta: torch.Tensor, state: torch.Tensor, 
     starts = _check_starts(starts, (batch,), index)
     written = (state,) if out is None else (state, out)
     out = _check_out(out, x, state)
-    _keep(x, delta, A, B, C, D, gate, delta_bias, out)
+    _keep(x, delta, A, B, C, D, gate, delta_bias, state, starts, out)
     at = state.data_ptr()
     desc = StateSpaceDesc(
         x.data_ptr(), x.stride(0), 0, delta.data_ptr(), delta.stride(0), 0, _p(gate), gate.stride(0) if gate is not None else 0, 0, A.data_ptr(),

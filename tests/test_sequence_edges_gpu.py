@@ -5,6 +5,8 @@ import torch
 from torch.autograd import forward_ad
 
 from isaaclab_amd.utils import sequence as S
+from isaaclab_amd.utils.command_list import CommandList
+from isaaclab_amd.utils.gradients import gradient_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -105,3 +107,30 @@ def test_lengths_past_32_bits(dev):
     for call in (lambda n: scan(v, lengths=n, return_state=True), lambda n: S.short_convolution(v["x"], weight, lengths=n, return_state=True)):
         assert all(torch.equal(a, b) for a, b in zip(call(lengths), call(clamped)))
     assert torch.equal(scan(v, lengths=lengths)[:2], scan(v)[:2])
+
+
+def test_a_command_list_holds_what_its_calls_read(dev):
+    """Operands that only the recorded call named: their memory stays theirs until the list goes."""
+    v, weight = operands(dev), torch.randn(24, 4, device=dev)
+    flags, lengths = torch.zeros(3, 20, device=dev), torch.tensor([3, 20, 11], dtype=torch.int32, device=dev)
+    flags[:, 9] = 1.0
+    conv, state = torch.zeros(3, 3, 24, device=dev), v["state"].clone()
+    copies = lambda: {k: t.clone() for k, t in v.items()}  # noqa: E731
+
+    def calls(conv, state):
+        yield scan(copies(), starts=flags > 0, lengths=lengths + 0, return_state=True)
+        yield S.short_convolution(v["x"] + 0, weight + 0, state=conv + 1, starts=flags > 0, lengths=lengths + 0, return_state=True)
+        yield (S.short_convolution_step(v["x"][:, 0] + 0, conv, weight + 0, starts=flags[:, 9] > 0),)
+        yield (step(copies(), 0, state, starts=flags[:, 9] > 0),)
+        yield (gradient_norm([v["x"] + 0, weight + 0]),)
+
+    commands = CommandList()
+    with torch.no_grad(), commands.record():
+        recorded = [call for call in calls(conv, state)]
+        junk = [torch.full((n,), float("nan"), device=dev) for n in (12, 24, 72, 96, 240, 288, 1440) for _ in range(40)]
+    commands.replay()
+    fresh_conv, fresh_state = torch.zeros_like(conv), v["state"].clone()
+    for got, want in zip(recorded, calls(fresh_conv, fresh_state)):
+        assert all(torch.equal(a, b) for a, b in zip(got, want))
+    assert torch.equal(conv, fresh_conv) and torch.equal(state, fresh_state)
+    del junk
