@@ -253,10 +253,12 @@ def _places(tensors) -> list:
 
 
 def _once(backward):
-    """A backward pass that cannot be differentiated again; without ``create_graph`` there is nothing to guard."""
+    """A backward pass that cannot be differentiated again (without ``create_graph`` there is nothing to guard) nor recorded."""
     guarded = once_differentiable(backward)
 
     def either(ctx, *grads):
+        if _abi.recording():   # (autograd on the calling thread: torch.autograd.set_multithreading_enabled(False))
+            raise _abi.IlxError("a backward pass cannot be recorded in a command list")
         return (guarded if torch.is_grad_enabled() else backward)(ctx, *grads)
 
     return either

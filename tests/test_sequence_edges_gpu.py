@@ -4,6 +4,7 @@ import pytest
 import torch
 from torch.autograd import forward_ad
 
+from isaaclab_amd import _abi
 from isaaclab_amd.utils import sequence as S
 from isaaclab_amd.utils.command_list import CommandList
 from isaaclab_amd.utils.gradients import gradient_norm
@@ -134,3 +135,16 @@ def test_a_command_list_holds_what_its_calls_read(dev):
         assert all(torch.equal(a, b) for a, b in zip(got, want))
     assert torch.equal(conv, fresh_conv) and torch.equal(state, fresh_state)
     del junk
+
+
+def test_a_backward_pass_is_not_recorded(dev):
+    """Autograd on the recording thread itself: refused, where the launches would be kept and the gradients left unwritten."""
+    v, weight = operands(dev), torch.randn(24, 4, device=dev)
+    for call in (lambda x: S.short_convolution(x, weight), lambda x: scan({**v, "x": x})):
+        x = v["x"].clone().requires_grad_(True)
+        out = call(x)
+        with torch.autograd.set_multithreading_enabled(False):
+            with CommandList().record(), pytest.raises(_abi.IlxError, match="backward pass cannot be recorded"):
+                torch.autograd.grad(out.sum(), x, retain_graph=True)
+            same_thread, = torch.autograd.grad(out.sum(), x, retain_graph=True)
+        assert torch.equal(same_thread, torch.autograd.grad(out.sum(), x)[0])
