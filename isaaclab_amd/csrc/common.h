@@ -67,8 +67,10 @@ struct CommandList {
 };
 CommandList*& recording_list();     // thread-local; null: launches are issued
 
+// (static: an instance is its file's own.  The linker merges the files' instances of an inline template, by the name of the
+// argument type alone; of two types of one name the one would then be copied with the other's size.)
 template <typename... P, typename... A>
-inline void launch(void (*kernel)(P...), dim3 grid, dim3 block, unsigned shmem, hipStream_t stream, A&&... a) {
+static inline void launch(void (*kernel)(P...), dim3 grid, dim3 block, unsigned shmem, hipStream_t stream, A&&... a) {
     static_assert(sizeof...(P) == sizeof...(A), "one argument per kernel parameter");
     std::tuple<P...> params{static_cast<P>(std::forward<A>(a))...};   // converted to the parameter types, as a call would
     CommandList* list = recording_list();

@@ -74,7 +74,7 @@ __global__ void __launch_bounds__(256) pose_op_kernel(PoseArgs s) {
     }
 }
 
-struct CameraArgs {
+struct CameraOpArgs {
     int op;
     const float* data;        // depth (n, h, w) or points (n, p, 3)
     const float* intrinsics;  // (k, 3, 3), k = 1 or n
@@ -84,7 +84,7 @@ struct CameraArgs {
     int32_t h, w;             // image size; project: h = points per batch, w unused
 };
 
-__global__ void __launch_bounds__(256) camera_op_kernel(CameraArgs s) {
+__global__ void __launch_bounds__(256) camera_op_kernel(CameraOpArgs s) {
     const int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.x + threadIdx.x;
     const int64_t per = s.op == ILX_CAMERA_PROJECT ? s.h : static_cast<int64_t>(s.h) * s.w;
     if (i >= s.n * per) return;
@@ -170,7 +170,7 @@ extern "C" int ilx_camera_op(int32_t op, const float* data, const float* intrins
     ILX_REQUIRE(data && intrinsics && out, ILX_EINVAL, "ilx_camera_op: NULL operand");
     ILX_REQUIRE(intrinsics_batch == 1 || intrinsics_batch == n, ILX_ESHAPE, "ilx_camera_op: %lld calibration matrices for %lld images",
                 static_cast<long long>(intrinsics_batch), static_cast<long long>(n));
-    CameraArgs s{op, data, intrinsics, intrinsics_batch, out, n, h, w};
+    CameraOpArgs s{op, data, intrinsics, intrinsics_batch, out, n, h, w};
     ILX_LAUNCH(camera_op_kernel, dim3(blocks_for(n * per)), dim3(256), 0, as_stream(stream), s);
     ILX_LAUNCH_CHECK("ilx_camera_op");
     return ILX_OK;

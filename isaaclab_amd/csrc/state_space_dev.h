@@ -9,7 +9,6 @@
 
 namespace ilx {
 
-// (One name, one layout in the whole library: ilx::launch is instantiated by the type and its instances are merged between files.)
 struct StateSpaceArgs {
     ilx_state_space s;
     int group_channels;    // channels / groups
