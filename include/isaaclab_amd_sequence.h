@@ -8,7 +8,7 @@
  * strided: a tensor of activations is (batch, length, channels) with unit channel stride, `*_batch` and `*_time` are its
  * other two strides in elements, so a time-major rollout buffer is passed as it is.  Parameters, states and their
  * gradients are dense float32.  There are at most 2^23 channels and, in the recurrence, time strides are below 2^27
- * elements; a larger shape is refused (ILX_ESHAPE).
+ * elements and a sequence has at most 2^31 - 4097 rows; a larger shape is refused (ILX_ESHAPE).
  *
  * `starts` (batch, length) bytes, non-zero where an episode begins: nothing from before that row reaches it or any later
  * row.  `lengths` (batch) int32: rows from lengths[b] on are not read, their outputs and gradients are written as zeros

@@ -473,6 +473,11 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_step_kernel(StateSpaceAr
     }
 }
 
+// The kernels count rows in 32 bits, up to the end of the last part, which may lie behind the sequence's: parts are rounded up to
+// ILX_SCAN_BLOCK rows and there are at most kMostParts.
+constexpr int64_t kMostRows = INT32_MAX - 4096;
+static_assert(kMostParts * ILX_SCAN_BLOCK + 64 <= 4096, "rows behind a sequence's end");
+
 int scan_check(const ilx_state_space& s, const char* name) {
     ILX_REQUIRE(s.batch >= 0 && s.length >= 0 && s.channels > 0 && s.groups > 0, ILX_EINVAL, "%s: bad shape (%lld, %lld, %d), %d groups", name,
                 (long long)s.batch, (long long)s.length, s.channels, s.groups);
@@ -483,7 +488,7 @@ int scan_check(const ilx_state_space& s, const char* name) {
     ILX_REQUIRE(s.dtype >= ILX_F32 && s.dtype <= ILX_F16, ILX_EINVAL, "%s: unknown type %d", name, s.dtype);
     ILX_REQUIRE(s.bc_dtype == ILX_F32 || s.bc_dtype == s.dtype, ILX_EINVAL, "%s: B and C of type %d beside activations of type %d", name,
                 s.bc_dtype, s.dtype);
-    ILX_REQUIRE(s.batch <= INT32_MAX && s.length <= INT32_MAX - 64 && s.batch * (s.length + 1) < (int64_t{1} << 40), ILX_ESHAPE,
+    ILX_REQUIRE(s.batch <= INT32_MAX && s.length <= kMostRows && s.batch * (s.length + 1) < (int64_t{1} << 40), ILX_ESHAPE,
                 "%s: shape (%lld, %lld) too large", name, (long long)s.batch, (long long)s.length);
     if (s.length > 1)
         for (const int64_t stride : {s.x_time, s.delta_time, s.gate_time, s.B_time, s.C_time, s.out_time, s.grad_out_time, s.grad_time, s.starts_time})

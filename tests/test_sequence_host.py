@@ -1,9 +1,12 @@
 """What the sequence and gradient operators decide on the host (no GPU needed)."""
 
+import ctypes
+
 import pytest
 import torch
 from torch.autograd import forward_ad
 
+from isaaclab_amd import _abi
 from isaaclab_amd.utils import gradients as G
 from isaaclab_amd.utils import sequence as S
 
@@ -36,3 +39,24 @@ def test_overlap_of_rows_and_a_dense_block():
                 seen.add(want)
     assert seen == {True, False}
     assert not S._overlap(memory[:0].view(0, 4), memory) and not S._overlap(memory.view(20, 20), memory[:0])
+
+
+def test_rows_are_counted_in_32_bits():
+    """Where the last part of a divided sequence ends stays below 2^31 for every accepted length; longer ones are refused."""
+    most = 2 ** 31 - 4097
+    need = ctypes.c_int64()
+
+    def parts_of(length, batch, channels):
+        desc = S.StateSpaceDesc(batch=batch, length=length, channels=channels, states=1, groups=1)
+        status = S._scan_workspace(ctypes.byref(desc), 0, ctypes.byref(need))
+        return status, need.value // (2 * batch * channels)   # a state and a decay per part and channel
+
+    for batch, channels in ((1, 1), (1, 64), (3, 64), (7, 640), (250, 256)):
+        for length in (most, most - 1, most - 57, 2 ** 31 - 2 ** 23, 2 ** 30 + 1, 2 ** 24 + 9):
+            status, parts = parts_of(length, batch, channels)
+            assert status == 0 and 1 < parts <= 256
+            rows = -(-(-(-length // parts)) // 8) * 8   # the fewest rows, a multiple of 8, that make as many parts ...
+            while -(-length // rows) > parts:
+                rows += 8
+            assert parts * rows < 2 ** 31, (batch, channels, length, parts)   # ... and its last part ends here
+        assert parts_of(most + 1, batch, channels)[0] == -2 and b"too large" in _abi.lib.ilx_last_error()
