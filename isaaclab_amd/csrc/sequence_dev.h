@@ -59,6 +59,10 @@ constexpr int32_t kMostChannels = 1 << 23;
 
 inline bool aligned_to(const void* p, size_t bytes) { return (reinterpret_cast<uintptr_t>(p) & (bytes - 1)) == 0; }
 
+// Rows that one thread's or wave's sums of a parameter's gradient span in 32 bits: n adds are off by up to n 2^-24 of their terms'
+// magnitudes, so a longer chain ends in another row of partial sums, and those are added in 64 bits.
+constexpr int kChainRows = 512;
+
 // The end of a parameter's gradient: `count` rows of (n0 + extra) x channels partial sums, one row per workgroup that kept
 // some, are added in a fixed order, in 64 bits.  Value k of channel d goes to out0[d, k] for k < n0, then out1[d], out2[d];
 // outputs that are NULL are left out.

@@ -278,7 +278,7 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvA
         for (int v = 0; v < V; ++v) zero[v] = 0.0f;
         for (int64_t t = len > t0 ? len : t0; t < t1; ++t) store_channels<V>(dx + t * a.c.grad_x_time, zero);
     }
-    // the workgroup's part of dw and db: one row of partial sums, added over the rows of threads in order
+    // the workgroup's part of dw and db: one row of partial sums, added over the rows of threads in order and in 64 bits
     constexpr int P = (W + 1) * V;
     float* mine = sums + threadIdx.x * P;
 #pragma unroll
@@ -293,9 +293,9 @@ __global__ void __launch_bounds__(kConvThreads) short_conv_backward_kernel(ConvA
         const int lane = i / P, kv = i - lane * P, k = kv / V, v = kv - k * V;
         const int g = static_cast<int>(blockIdx.x % a.channel_blocks) * lanes + lane;
         if (g >= a.groups) continue;
-        float s = 0.0f;
-        for (int r = 0; r < rows; ++r) s += sums[(r * lanes + lane) * P + kv];
-        a.c.workspace[(slot * (W + 1) + k) * a.c.channels + first_channel<V>(a, g) + v] = s;
+        double s = 0.0;
+        for (int r = 0; r < rows; ++r) s += static_cast<double>(sums[(r * lanes + lane) * P + kv]);
+        a.c.workspace[(slot * (W + 1) + k) * a.c.channels + first_channel<V>(a, g) + v] = static_cast<float>(s);
     }
 }
 
@@ -411,8 +411,11 @@ ConvArgs conv_args(const ilx_short_conv& c, int v, bool backward) {
     const int rows = kConvThreads >> a.cx_log2;
     a.slots = (a.items + rows - 1) / rows;
     if (backward) {
+        // a thousand workgroups, and more where a thread's segments would hold more than kChainRows rows
         const int64_t most = 1024 / a.channel_blocks > 0 ? 1024 / a.channel_blocks : 1;
-        if (a.slots > most) a.slots = most;
+        const int64_t chain = kChainRows / (c.length < 1 ? 1 : c.length < a.segment ? c.length : a.segment) * rows, least = (a.items + chain - 1) / chain;
+        const int64_t wanted = most > least ? most : least;
+        if (a.slots > wanted) a.slots = wanted;
     }
     return a;
 }
@@ -510,6 +513,7 @@ extern "C" int ilx_short_conv_backward(const ilx_short_conv* conv, void* stream)
                 "ilx_short_conv_backward: NULL operand");
     const int v = conv_vector(c, true);
     const ConvArgs a = conv_args(c, v, true);
+    ILX_REQUIRE(a.slots * a.channel_blocks * kConvThreads <= kMostThreads, ILX_ESHAPE, "ilx_short_conv_backward: shape too large for one launch");
     ILX_REQUIRE(c.workspace_floats >= a.slots * (c.width + 1) * c.channels && (c.workspace || a.slots == 0), ILX_EINVAL,
                 "ilx_short_conv_backward: workspace of %lld floats, %lld needed", (long long)c.workspace_floats,
                 (long long)(a.slots * (c.width + 1) * c.channels));
