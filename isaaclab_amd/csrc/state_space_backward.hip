@@ -24,6 +24,7 @@ namespace ilx {
 constexpr int kRows = ILX_SCAN_BLOCK;
 constexpr int kWaves = 4;
 constexpr int kChannels = 16;   // per wave
+constexpr int kChainBlocks = kChainRows / kRows;
 constexpr float kLn2 = 0.693147180559945309417f;
 static_assert(kRows == 8, "two sets of four rows");
 
@@ -225,6 +226,29 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
         for (int e = 0; e < 2; ++e) arrive(in_B[e]), arrive(in_C[e]);
     };
 
+    // a row of the workgroup's partial sums of the parameters' gradients
+    int chain = 0, summed = 0;   // rows written; blocks in the sums
+    auto end_chain = [&] {
+        const ArgsPtr p = arguments_again();
+        dD = fold32(dD, dD), dbias = fold32(dbias, dbias);
+        dD = fold16(dD, dD), dbias = fold16(dbias, dbias);
+        const uint32_t n = p->s.states, row = p->s.channels * 4;
+        const auto to = row_buffer(p->sums + (slot * p->chains + chain) * (static_cast<int64_t>(n) + 2) * p->s.channels);
+        if (active) {
+#pragma unroll
+            for (int j = 0; j < S; ++j)
+                if (S * quarter + j < n) lane_store<float>(to, state_at[j], 0, dA[j]);
+            uint32_t at = channel;   // (made here: the compiler would hold the channel's offset in another register through all rows)
+            asm volatile("" : "+v"(at));
+            at *= 4 / sizeof(T);
+            if (quarter == 0) lane_store<float>(to, at, n * row, dD), lane_store<float>(to, at, (n + 1) * row, dbias);
+        }
+#pragma unroll
+        for (int j = 0; j < S; ++j) dA[j] = 0.0f;
+        dD = 0.0f, dbias = 0.0f;
+        ++chain, summed = 0;
+    };
+
     ScanBlock k = item_end(slot);
     if (k.count > 0) {
         read(k);
@@ -264,6 +288,8 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
             next.item = items, next.count = 0;
         }
         if (k.count > 0) {
+            if (summed == kChainBlocks) end_chain();
+            ++summed;
             // rows past the end act as rows that leave the state alone: dt = x = dy = 0
             float slope[2], dgate[2], x[2], dt[2], dy[2];
 #pragma unroll
@@ -392,18 +418,8 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
         }
         k = next;
     }
-    // the workgroup's part of the parameters' gradients
-    dD = fold32(dD, dD), dbias = fold32(dbias, dbias);
-    dD = fold16(dD, dD), dbias = fold16(dbias, dbias);
-    if (!active) return;
-    float* sums = a.sums + static_cast<int64_t>(slot) * (states + 2) * channels;
-#pragma unroll
-    for (int j = 0; j < S; ++j)
-        if (S * quarter + j < states) sums[state_at[j] >> 2] = dA[j];
-    if (quarter == 0) {
-        sums[static_cast<int64_t>(states) * channels + d] = dD;
-        sums[static_cast<int64_t>(states + 1) * channels + d] = dbias;
-    }
+    // the last sums, and zeros for the rows of partial sums that are left (sequences that end early)
+    for (const int chains = static_cast<int>(a.chains); chain < chains;) end_chain();
 }
 
 // dB and dC: the sums of the blocks of channels of a group, in order; rows past a sequence's end are zeros.
@@ -440,7 +456,9 @@ StateSpaceArgs backward_args(const ilx_state_space& s, int64_t* floats) {
     const int64_t items = s.batch * a.parts, wanted = 6 * device_cu_count(), most = wanted / a.blocks > 0 ? wanted / a.blocks : 1;
     const int64_t each = (items + most - 1) / most;
     a.slots = each > 0 ? (items + each - 1) / each : 0;
-    const int64_t sums = a.slots * (s.states + 2) * s.channels;
+    const int64_t summed = each * ((a.part_rows + kRows - 1) / kRows);   // blocks of a workgroup
+    a.chains = summed > kChainBlocks ? (summed + kChainBlocks - 1) / kChainBlocks : 1;
+    const int64_t sums = a.slots * a.chains * (s.states + 2) * s.channels;
     const int64_t shared = a.group_blocks * s.batch * s.length * s.groups * 8 * lane_states(s.states);
     a.sums = s.workspace + part_floats;
     a.shared = a.sums + sums;
@@ -501,7 +519,7 @@ extern "C" int ilx_state_space_backward(const ilx_state_space* scan, void* strea
             default: wide ? backward_states<f16_t, float>(a, st) : backward_states<f16_t, f16_t>(a, st); break;
         }
     }
-    launch_parameter_sums(a.sums, a.slots, s.channels, s.states, 2, s.grad_A, s.grad_D, s.grad_delta_bias, st);
+    launch_parameter_sums(a.sums, a.slots * a.chains, s.channels, s.states, 2, s.grad_A, s.grad_D, s.grad_delta_bias, st);
     ILX_LAUNCH_CHECK("ilx_state_space_backward");
     return ILX_OK;
 }

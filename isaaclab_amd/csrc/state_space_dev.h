@@ -22,7 +22,8 @@ struct StateSpaceArgs {
     int64_t slots;       // workgroups per block of channels
     int units;           // waves of a launch whose waves are independent
     bool decays_aligned; // A on a 16-byte boundary
-    float* sums;         // backward: (slots, states + 2, channels) partial sums of dA, dD and d delta_bias
+    int64_t chains;      // backward: partial sums of a workgroup, each over kChainRows rows at most
+    float* sums;         // backward: (slots, chains, states + 2, channels) partial sums of dA, dD and d delta_bias
     float* shared;       // backward: (group_blocks, batch, length, groups, 2 * padded states) partial sums of dB, dC
 };
 

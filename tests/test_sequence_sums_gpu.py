@@ -35,3 +35,34 @@ def test_convolution_of_many_rows(dev):
     out = S.short_convolution(x, weight, bias)
     for name, g in zip(("weight", "bias"), torch.autograd.grad(out, (weight, bias), grad)):
         check(g, want, name)
+
+
+def test_recurrence_of_many_sequences(dev):
+    """4096 sequences of one row to a workgroup: dA, dD and d delta_bias are each the sum of the output's gradients."""
+    batch, channels = 4096, 64 * 1536
+    x = ones(dev, torch.bfloat16, batch, 1, channels)
+    bc = ones(dev, torch.bfloat16, batch, 1, 1, 1)
+    leaves = dict(A=torch.zeros(channels, 1, device=dev), D=torch.ones(channels, device=dev), delta_bias=torch.zeros(channels, device=dev))
+    leaves = {k: t.requires_grad_(True) for k, t in leaves.items()}
+    grad = torch.full((batch, 1, channels), E, dtype=torch.bfloat16, device=dev)
+    grad[0] = 1.0
+    out = S.state_space_scan(x, x, leaves["A"], bc, bc, D=leaves["D"], delta_bias=leaves["delta_bias"], softplus=False,
+                             state=torch.ones(batch, 1, channels, device=dev))
+    for name, g in zip(leaves, torch.autograd.grad(out, tuple(leaves.values()), grad)):
+        check(g, 1 + (batch - 1) * E, name)
+
+
+@pytest.mark.parametrize("with_lengths", [False, True])
+def test_recurrence_of_many_rows(dev, with_lengths):
+    """Sequences of 16384 and fewer rows, undivided, and workgroups whose sequences end early: dD (a lane adds every fourth row)."""
+    batch, length, channels = 12, 2 ** 14, 64 * 160   # two sequences to a workgroup, 64 rows of partial sums
+    x = ones(dev, torch.bfloat16, batch, length, channels)
+    bc, zero = ones(dev, torch.bfloat16, batch, length, 1, 1), torch.zeros(1, 1, 1, dtype=torch.bfloat16, device=dev).expand(batch, length, channels)
+    D = torch.ones(channels, device=dev, requires_grad=True)
+    lengths = torch.tensor(([length, length - 1, 0, 513, 512, 1, 9000] * 2)[:batch] if with_lengths else [length] * batch)
+    grad = torch.full((batch, length, channels), E, dtype=torch.bfloat16, device=dev)
+    grad[:, -1] = 1.0   # (the walk back begins there)
+    out = S.state_space_scan(x, zero, torch.zeros(channels, 1, device=dev), bc, bc, D=D, softplus=False, lengths=lengths.to(dev, torch.int32))
+    got, = torch.autograd.grad(out, D, grad)
+    full = int((lengths == length).sum())
+    check(got, full + (int(lengths.sum()) - full) * E, "D")
