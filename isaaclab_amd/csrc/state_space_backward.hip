@@ -422,7 +422,8 @@ __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_ker
     for (const int chains = static_cast<int>(a.chains); chain < chains;) end_chain();
 }
 
-// dB and dC: the sums of the blocks of channels of a group, in order; rows past a sequence's end are zeros.
+// dB and dC: the sums of the blocks of channels of a group, in order and in 64 bits (there may be thousands of them); rows past a
+// sequence's end are zeros.
 template <typename TB> __global__ void __launch_bounds__(256) scan_shared_sums_kernel(StateSpaceArgs a, int padded) {
     const ilx_state_space& s = a.s;
     const int64_t i = static_cast<int64_t>(blockIdx.x) * 256 + threadIdx.x, rows = s.batch * s.length * s.groups;
@@ -430,15 +431,15 @@ template <typename TB> __global__ void __launch_bounds__(256) scan_shared_sums_k
     const int64_t row = i / s.states;
     const int n = static_cast<int>(i - row * s.states);
     const int64_t bt = row / s.groups, b = bt / s.length, t = bt - b * s.length;
-    float dB = 0.0f, dC = 0.0f;
+    double dB = 0.0, dC = 0.0;
     if (t < scan_length(s, b))
         for (int k = 0; k < a.group_blocks; ++k) {
             const float* p = a.shared + (k * rows + row) * 2 * padded + n;
-            dB += p[0];
-            dC += p[padded];
+            dB += static_cast<double>(p[0]);
+            dC += static_cast<double>(p[padded]);
         }
-    static_cast<TB*>(s.grad_B)[i] = from_f32<TB>(dB);
-    static_cast<TB*>(s.grad_C)[i] = from_f32<TB>(dC);
+    static_cast<TB*>(s.grad_B)[i] = from_f32<TB>(static_cast<float>(dB));
+    static_cast<TB*>(s.grad_C)[i] = from_f32<TB>(static_cast<float>(dC));
 }
 
 }  // namespace ilx

@@ -66,3 +66,16 @@ def test_recurrence_of_many_rows(dev, with_lengths):
     got, = torch.autograd.grad(out, D, grad)
     full = int((lengths == length).sum())
     check(got, full + (int(lengths.sum()) - full) * E, "D")
+
+
+def test_shared_gradients_of_many_channels(dev):
+    """dB and dC are sums over the channels: 64 in a workgroup, in float32 (8 roundings), and 4096 such blocks."""
+    channels = 64 * 4096
+    x = ones(dev, torch.bfloat16, 1, 1, channels)
+    B, C = torch.ones(1, 1, 1, 1, device=dev, requires_grad=True), torch.ones(1, 1, 1, 1, device=dev, requires_grad=True)
+    grad = torch.zeros(1, 1, channels, dtype=torch.bfloat16, device=dev)
+    grad[..., ::64] = E
+    grad[..., 0] = 1.0
+    out = S.state_space_scan(x, x, torch.zeros(channels, 1, device=dev), B, C, softplus=False)
+    for name, g in zip("BC", torch.autograd.grad(out, (B, C), grad)):
+        check(g, 1 + 4095 * E, name, 10)
