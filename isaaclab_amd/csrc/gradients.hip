@@ -14,7 +14,8 @@
 
 namespace ilx {
 
-constexpr int kTensors = 200;             // per launch: what fits the 4 KB of a kernel's arguments
+constexpr size_t kArgumentBytes = 4096 - 256;   // of a kernel: 4 KB with the runtime's own
+constexpr int kTensors = 223;             // per launch: as many as fit the arguments
 constexpr uint32_t kChunk = 16384;        // elements: one share of a tensor
 constexpr int64_t kMostElements = int64_t{1} << 30;   // of an entry; a larger tensor takes several
 constexpr int kMostPartials = 2048;
@@ -36,7 +37,7 @@ struct NormArgs {
     float max_norm;
     float* norm;
 };
-static_assert(sizeof(NormArgs) <= 4096 - 256, "kernel arguments");
+static_assert(sizeof(NormArgs) <= kArgumentBytes && sizeof(NormArgs) + 8 + 4 + 4 + 1 > kArgumentBytes, "kernel arguments");
 
 // The entry of a chunk: the last one whose first chunk is not past it.  A wave holds all first chunks, read together (a search of the
 // table would wait for one read of the arguments after the other), and counts.

@@ -1,7 +1,7 @@
 """Global gradient norm and clipping on ``ilx_gradient_norm`` (include/isaaclab_amd_sequence.h): the end of a training step.
 
 No counterpart in the reference, whose RL libraries call torch.  All tensors, of any mix of float32, bfloat16 and float16, are
-reduced in one launch per 200 tensors and scaled in place in another; nothing is read back to the host.  No derivative goes
+reduced in one launch per 223 tensors and scaled in place in another; nothing is read back to the host.  No derivative goes
 through the norm or the scaling (forward mode is refused).  Squares are added in 64 bits in a fixed order, so their sum
 neither overflows nor depends on scheduling: replicas with equal gradients clip alike.
 """

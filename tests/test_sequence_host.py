@@ -9,6 +9,7 @@ from torch.autograd import forward_ad
 from isaaclab_amd import _abi
 from isaaclab_amd.utils import gradients as G
 from isaaclab_amd.utils import sequence as S
+from isaaclab_amd.utils.command_list import CommandList
 
 
 def test_forward_mode_is_refused():
@@ -60,3 +61,21 @@ def test_rows_are_counted_in_32_bits():
                 rows += 8
             assert parts * rows < 2 ** 31, (batch, channels, length, parts)   # ... and its last part ends here
         assert parts_of(most + 1, batch, channels)[0] == -2 and b"too large" in _abi.lib.ilx_last_error()
+
+
+def test_launches_of_a_gradient_list():
+    """Two launches (one and one more for the norm alone) for as many tensors as fit a kernel's arguments; empty tensors take no place."""
+    most = 223
+
+    def launches(sizes, clip):
+        n, at = len(sizes), 0x100000
+        pointers = [at := at + 0x10000 for _ in sizes]
+        commands = CommandList()
+        with commands.record():   # (what the call answers without a device does not matter)
+            G._norm((ctypes.c_void_p * n)(*pointers), (ctypes.c_int64 * n)(*sizes), (ctypes.c_int32 * n)(), n, 0, clip, 1.0, 0x1000, 0x2000, 4096, None)
+        return len(commands)
+
+    for count, tables in ((1, 1), (16, 1), (200, 1), (201, 1), (most, 1), (most + 1, 2), (2 * most, 2), (2 * most + 1, 3)):
+        assert launches([7] * count, 1) == 2 * tables and launches([7] * count, 0) == tables + 1, count
+        assert launches([0, 7] * count, 1) == 2 * tables, count
+    assert launches([0], 1) == 2
