@@ -29,7 +29,7 @@ constexpr int kScanWaves = 4;   // to a workgroup: independent, but a workgroup 
 
 __device__ __forceinline__ int wave_unit() { return uni(static_cast<int>(blockIdx.x * kScanWaves + (threadIdx.x >> 6))); }
 
-enum { kHasGate = 1, kSoftplus = 2, kHasStarts = 4, kFull = 8 };   // kFull: as many states as the lane has registers
+enum { kHasGate = 1, kSoftplus = 2, kHasStarts = 4 };
 
 // What stays in scalar registers through a wave's life; all else is read again where an item begins (arguments_again).
 template <typename T, typename TB> struct ScanStreams {
@@ -195,8 +195,8 @@ template <typename TB, int W> struct SharedStates {
     }
 };
 
-template <int V> __device__ __forceinline__ int scan_flags(const ilx_state_space& s) {
-    return (s.gate ? kHasGate : 0) | (s.softplus ? kSoftplus : 0) | (s.starts ? kHasStarts : 0) | (s.states == 4 * V ? kFull : 0);
+__device__ __forceinline__ int scan_flags(const ilx_state_space& s) {
+    return (s.gate ? kHasGate : 0) | (s.softplus ? kSoftplus : 0) | (s.starts ? kHasStarts : 0);
 }
 
 template <typename T, typename TB, int S>
@@ -214,7 +214,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_forward_kernel(StateSpac
     arrive(bias), arrive(skip);
     ScanRows<T, TB, W, true, true> rows;
     ScanStreams<T, TB> k;
-    k.flags = scan_flags<V>(a.s);
+    k.flags = scan_flags(a.s);
     k.template open<false>(unit / a.blocks, c.group);
     if (k.begin < k.end) rows.read(k, channel, shared.o, shared.c, lane);
     float* saved = nullptr;
@@ -320,7 +320,7 @@ __global__ void __launch_bounds__(64 * kScanWaves) scan_part_kernel(StateSpaceAr
     const float bias = a.s.delta_bias ? a.s.delta_bias[c.d] : 0.0f;
     ScanRows<T, TB, W, REVERSE, false> rows;
     ScanStreams<T, TB> k;
-    k.flags = scan_flags<V>(a.s);
+    k.flags = scan_flags(a.s);
     k.template open<REVERSE>(unit / a.blocks, c.group);
     if (k.begin < k.end) {
         rows.read(k, channel, shared.o, shared.c, lane);

@@ -47,11 +47,6 @@ __device__ __forceinline__ int64_t scan_length(const ilx_state_space& s, int64_t
     return n < 0 ? 0 : (n > s.length ? s.length : n);
 }
 
-// Offset of a row: row and stride below 2^32, so one 32 x 32 bit product (scalar instructions).
-__device__ __forceinline__ int64_t row_offset(uint32_t row, int64_t stride) {
-    return static_cast<int64_t>(static_cast<uint64_t>(row) * static_cast<uint32_t>(stride));
-}
-
 // The kernel's arguments, read anew: a value that an item needs once must not hold scalar registers through all of its rows
 // (the compiler would keep all of them, and spill into vector registers, two to four cycles an access).
 typedef const __attribute__((address_space(4))) StateSpaceArgs* ArgsPtr;
@@ -115,14 +110,6 @@ template <typename T> struct Stream {
     }
     __device__ __forceinline__ __amdgpu_buffer_rsrc_t buffer() const { return row_buffer(p); }
 };
-
-// Bit i: an episode begins at row t0 + i (i < count <= 64).
-__device__ __forceinline__ uint64_t start_bits(const ilx_state_space& s, int64_t b, int64_t t0, int count, int lane) {
-    if (!s.starts) return 0;
-    bool on = false;
-    if (lane < count) on = s.starts[b * s.starts_batch + (t0 + lane) * s.starts_time] != 0;
-    return __ballot(on);
-}
 
 template <typename F, int... I> __device__ __forceinline__ void static_for_(F f, std::integer_sequence<int, I...>) {
     (f(std::integral_constant<int, I>{}), ...);
