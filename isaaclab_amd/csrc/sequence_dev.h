@@ -23,7 +23,9 @@ __device__ __forceinline__ float sigmoid_fast(float x) { return rcp_fast(1.0f + 
 
 // log(1 + e^x) = max(x, 0) + log1p(e^-|x|), the second term as 2 artanh(s), s = e / (2 + e) with e in (0, 1] (a logarithm of 1 + e
 // would lose e's last bits, which for a step size of 1e-4 are all it has).  s is at most 1/3; the polynomial in s^2 is the one of degree
-// 4 with the least largest relative error on [0, 1/9], 2^-27.9.  In float32 the result is off by at most 5 units of 2^-24.
+// 4 with the least largest relative error on [0, 1/9], 2^-27.9.  Relative error in units of 2^-24: at most 9 for x >= 0 and 9 + 1.3 |x|
+// below (|x| from the product with log2 e and a quarter of it from log2 e itself; exponential and reciprocal 2 each, five roundings).
+// Measured: 4 above -1, 10 down to -10, 32 down to -40.
 __device__ __forceinline__ float softplus_f(float x) {
     const float e = exp_fast(-__builtin_fabsf(x));
     const float s = e * rcp_fast(2.0f + e), q = s * s;

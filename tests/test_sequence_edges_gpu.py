@@ -148,3 +148,20 @@ def test_a_backward_pass_is_not_recorded(dev):
                 torch.autograd.grad(out.sum(), x, retain_graph=True)
             same_thread, = torch.autograd.grad(out.sum(), x, retain_graph=True)
         assert torch.equal(same_thread, torch.autograd.grad(out.sum(), x)[0])
+
+
+@pytest.mark.parametrize("lo,hi", [(-85.0, -40.0), (-40.0, -20.0), (-20.0, -10.0), (-10.0, -3.0), (-3.0, -1.0), (-1.0, 0.0), (0.0, 1.0), (1.0, 30.0)])
+def test_softplus_relative_error(dev, lo, hi):
+    """The step size keeps its relative accuracy however small it is: dt = softplus(delta) itself, by x = B = C = 1 and no state.
+    In units of 2^-24: 9 + 1.3 |delta| below zero (the exponent's rounding), 9 above."""
+    rows, channels = 64, 1024
+    delta = torch.rand(1, rows, channels, generator=torch.Generator().manual_seed(int(lo))).to(dev) * (hi - lo) + lo
+    starts = torch.ones(1, rows, dtype=torch.bool, device=dev)
+    one = torch.ones(1, rows, 1, device=dev)
+    dt = S.state_space_scan(torch.ones_like(delta), delta, torch.zeros(channels, 1, device=dev), one, one, starts=starts)
+    x = delta.double()
+    want = x.clamp(min=0) + torch.log1p(torch.exp(-x.abs()))
+    units = (dt.double() / want - 1).abs() * 2 ** 24
+    bound = 9 + 1.3 * (-x).clamp(min=0)
+    print(f"softplus on [{lo}, {hi}]: {float(units.max()):.1f} units")
+    assert (units <= bound).all(), float((units / bound).max())
