@@ -131,7 +131,7 @@ template <typename T, typename TB, int S>
 __global__ void __launch_bounds__(64 * kWaves, S == 8 ? 2 : 3) scan_backward_kernel(StateSpaceArgs a) {
     constexpr int O = (S + 3) / 4, R = S / 2 > 0 ? S / 2 : 1;
     __shared__ float4 s_row[kWaves][kRows][kChannels];   // dt, dt x, dy
-    __shared__ float s_part[2][kWaves][R][kRows][64];    // halved sums of this block and the one before
+    alignas(16) __shared__ float s_part[2][kWaves][R][kRows][64];    // halved sums of this block and the one before
     const int lane = threadIdx.x & 63, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), quarter = lane >> 4;
     const int block = blockIdx.x % a.blocks, slot = blockIdx.x / a.blocks;
     const int group = block / a.group_blocks, group_block = block - group * a.group_blocks;
