@@ -17,6 +17,11 @@
  * Scratch memory is the caller's: the *_workspace functions say how many floats a call needs (0 if none).  The same
  * descriptor must be given to both; the contents need not survive the call.  Results do not depend on what it held, and no
  * sum's order depends on scheduling: two runs give the same bits.
+ *
+ * All arithmetic is in 32 bits.  Sums of parameters' gradients span at most 512 rows in 32 bits, longer ones are added in 64, and so
+ * are those of grad_B and grad_C over blocks of 64 channels and the squares of a norm.  Inputs that are infinite or NaN make
+ * what depends on them infinite or NaN, though not always the one of the two that the formula says (and grad_A, in which the
+ * state behind the last row does not occur, may become NaN where that state is infinite).
  */
 #ifndef ISAACLAB_AMD_SEQUENCE_H
 #define ISAACLAB_AMD_SEQUENCE_H

@@ -5,8 +5,9 @@
 // of 1e30 has a norm and small gradients beside large ones count; the adds hide behind the loads.
 // The tensors' pointers and sizes travel as kernel arguments, kTensors of them to a launch: no table in device memory that
 // would have to be copied or kept for a replay.
-// Measured, 200 tensors of 200 M bf16 elements together: 96 us for the sums (400 MB, 4.2 TB/s) and 137 to scale (800 MB; half of what
-// it reads is still in the last-level cache), against 4.97 TB/s of a large copy.  16 tensors of a policy (572 K f32): 6.5 and 6 us.
+// Measured, 200 tensors of 200 M bf16 elements together: 121 us for the sums (400 MB, 3.3 TB/s; 94 where the last-level cache holds part of
+// them) and 126 to scale (800 MB; part of what it reads is still in that cache), against 4.97 TB/s of a large copy.  16 tensors of a
+// policy (572 K f32): 6.2 and 5.6 us in 46 shares: most of the chip has none.
 #include "sequence_dev.h"
 
 #include <algorithm>

@@ -7,9 +7,9 @@
 // channels, the last thread's V channels end with the row's and overlap its neighbour's: both come to the same values and store
 // them, but for the step, which writes what its neighbour reads and stores its own only.
 // Measured, W = 4, against a large copy's 4.97 TB/s on the same card:
-//   forward, 24 x 4096 x 256 f32: 36 us, 201 MB, 5.5 TB/s (part of it stays in the last-level cache between passes)
-//   forward, 3 x 8190 x 1536 bf16: 36 us, 151 MB, 4.1 TB/s
-//   backward, 24 x 4096 x 256 f32: 67 us, 302 MB, 4.5 TB/s, and 8 us for the sums of 1024 workgroups' parts of dw and dbias
+//   forward, 24 x 4096 x 256 f32: 41 us, 201 MB, 4.9 TB/s
+//   forward, 3 x 8190 x 1536 bf16: 37 us (32 to 40), 151 MB, 4.1 TB/s
+//   backward, 24 x 4096 x 256 f32: 70 us, 302 MB, 4.3 TB/s, and 7 us for the sums of 1024 workgroups' parts of dw and dbias
 //   step, 16384 x 512 f32: 41 us in a loop on one state, 52 on states that are not cached (268 MB, 5.1 TB/s)
 #include "sequence_dev.h"
 

@@ -10,12 +10,12 @@
 // exp(A sum dt)), and every part runs again from the state that enters it.  That costs a second pass of exponentials and buys
 // up to 256 times the waves.
 // Measured with 16 states, against a large copy's 4.97 TB/s:
-//   24 x 4096 x 256 f32, gate, state in and out: 133 us, 537 MB, 4.0 TB/s; with the states a backward pass needs 147 us, 738 MB, 5.0
+//   24 x 4096 x 256 f32, gate, state in and out: 133 us, 537 MB, 4.0 TB/s; with the states a backward pass needs 142 us, 738 MB, 5.2
 //   TB/s: bound by memory
-//   1 x 16384 x 1024 bf16 in 256 parts: 57 us for the parts, 11 for the join, 80 for the rows; 134 MB of operands, so bound by the
-//   vector unit (part kernel: 78 instructions a row and wave, 52 of them the recurrence; the unit is busy 81 % of the time)
+//   1 x 16384 x 1024 bf16 in 256 parts: 60 us for the parts, 11 for the join, 82 for the rows; 134 MB of operands, so bound by the
+//   vector unit (part kernel: 78 instructions a row and wave, 52 of them the recurrence; the unit is busy 76 % of the time)
 //   undivided, the same call takes 19 ms
-//   step, 16384 x 256 bf16: 112 us on states that are not cached (571 MB, 5.1 TB/s), 91 in a loop on one state
+//   step, 16384 x 256 bf16: 113 us on states that are not cached (571 MB, 5.1 TB/s), 91 in a loop on one state
 #include "state_space_dev.h"
 #include "uniform_access.h"
 

@@ -13,9 +13,9 @@
 //  * sums over the channels (dB, dC) are first halved twice inside 16 lanes, each step leaving half of the lanes one value and
 //    half another (twelve adds for eight values, where a plain tree takes 32); what is left, 16 numbers of a workgroup's four waves
 //    (64 channels) to a result, is added from LDS behind the block's one barrier.
-// Measured, 24 x 4096 x 256 f32 with gate and 16 states: 390 to 425 us from run to run (and 16 for the sums of dB and dC over blocks of
-// channels, 6 for the parameters), 0.97 GB, 2.4 TB/s.  Bound by instructions: 89 in the vector unit for a row and wave (four states a
-// lane), which is busy 70 % of the time with three waves on a SIMD.  Waiting for reads behind the stores costs 10 us, running pointers in
+// Measured, 24 x 4096 x 256 f32 with gate and 16 states: 378 us (351 to 436 from pass to pass; and 15 for the sums of dB and dC over blocks
+// of channels, 6 for the parameters), 0.97 GB, 2.6 TB/s.  Bound by instructions: 89 in the vector unit for a row and wave (four states a
+// lane), which is busy 72 % of the time with three waves on a SIMD.  Waiting for reads behind the stores costs 10 us, running pointers in
 // the place of the arguments read again 30 (they spill).
 #include "state_space_dev.h"
 
