@@ -11,7 +11,7 @@ def _gate(p):
 
 
 def _softplus(v):
-    return torch.clamp(v, min=0) + torch.log1p(torch.exp(-v.abs()))
+    return torch.logaddexp(v, torch.zeros_like(v))   # (a maximum and an absolute value would have slope 1 at exactly 0)
 
 
 def _lengths(lengths, batch, length):

@@ -10,6 +10,7 @@ from isaaclab_amd import _abi
 from isaaclab_amd.utils import gradients as G
 from isaaclab_amd.utils import sequence as S
 from isaaclab_amd.utils.command_list import CommandList
+from oracle import sequence as O
 
 
 def test_forward_mode_is_refused():
@@ -79,3 +80,13 @@ def test_launches_of_a_gradient_list():
         assert launches([7] * count, 1) == 2 * tables and launches([7] * count, 0) == tables + 1, count
         assert launches([0, 7] * count, 1) == 2 * tables, count
     assert launches([0], 1) == 2
+
+
+def test_the_oracle_s_step_size():
+    """log(1 + e^x) and its slope 1 / (1 + e^-x), at zero too."""
+    x = torch.tensor([0.0, 1e-300, -1e-12, 0.5, -0.5, 3.0, -3.0, 30.0, -30.0, 700.0, -700.0], dtype=torch.float64, requires_grad=True)
+    value = O._softplus(x)
+    slope, = torch.autograd.grad(value.sum(), x)
+    want = torch.where(x > 0, x + torch.log1p(torch.exp(-x.abs())), torch.log1p(torch.exp(x)))
+    torch.testing.assert_close(value, want, rtol=1e-15, atol=0)
+    torch.testing.assert_close(slope, 1 / (1 + torch.exp(-x.detach())), rtol=1e-13, atol=0)
